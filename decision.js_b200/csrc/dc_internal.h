@@ -1,5 +1,6 @@
 // Internal declarations shared by the library's translation units.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -103,6 +104,22 @@ struct dc_ctx {
   std::vector<cudaEvent_t> free_events;
   double prof_ms[DC_K_KINDS] = {}, prof_flops[DC_K_KINDS] = {}, prof_bytes[DC_K_KINDS] = {};
   long long prof_n[DC_K_KINDS] = {};
+};
+
+// A rotation plan (dc_rope_plan_create): the pairs' frequencies on the device, in turns per position as 64-bit
+// fractions, and the factor on cos and sin.
+struct dc_rope_plan {
+  int device = 0, rot = 0, layout = 0;
+  float factor = 1.0f;
+  uint64_t *d_freq = nullptr;
+};
+
+// A paged key/value cache (dc_kv_cache_create): the caller's two buffers [pages, kv, page, D] of f16 and their tensor
+// maps, boxes of 64 dims x min(page, 64) rows.
+struct dc_kv_cache {
+  int device = 0, pages = 0, page = 0, kv = 0, D = 0;
+  void *K = nullptr, *V = nullptr;
+  CUtensorMap mapK, mapV;
 };
 
 // Make `ctx`'s device current on this thread.

@@ -1,0 +1,861 @@
+// Attention of a batch of sequences over a paged cache, with a prefix that a group of sequences shares.
+//
+// For a query row, o = sum_j p_j v_j / sum_j p_j with p_j = exp(scale q . k_j), j over its group's prefix and its own
+// keys up to its own. A tile is 128 rows of one kv head: TPT = 128 / r consecutive tokens of a group (r query heads to
+// a kv head), so tokens of several sequences share the tile and the prefix passes through the tensor cores once for
+// all of them. The keys of a tile are a list of 64-key blocks: the prefix's, then, sequence by sequence, the own
+// blocks of the sequences that the tile's tokens belong to, seen by that sequence's rows alone.
+//
+// The blocks of all tiles of all kv heads in a row make one line of B units (a sequence piece without keys counts as
+// one unit, so that every tile is visited). Each CTA of a resident grid takes an equal stretch of it, whatever the
+// lengths: a long prefix is cut over many CTAs, short tiles are walked one after the other. Every CTA works the line
+// out for itself from the offsets and lengths (one scan over the sequences), so nothing is planned on the host and a
+// captured call follows new contents. A tile inside one stretch is written straight to Y; a tile that was cut leaves
+// f32 parts (value sums, row maximum and weight sum) that a second kernel joins in order of the stretches, so results
+// do not depend on timing.
+//
+// Within a CTA:
+//   warps 0-7  softmax, as in the attention over packed rows: two warps per TMEM lane quadrant, thread = row, each
+//              half of a block's keys; the exp2 weights are scaled by 2^7 (the row reference moves when the maximum
+//              grows past 2^8, so they stay under 2^15) to keep small ones out of f16's subnormals, and the sum adds
+//              the rounded weights that the product uses
+//   warp 8     walks the line, hands runs of blocks to the others through a ring of descriptors, loads Q and K
+//   warp 9     loads V
+//   warp 10    the MMAs (and TMEM)
+//   warp 11    looks over V blocks that some row of the tile does not see: rows past the last key are zeroed, and
+//              values that are not finite too (a weight of 0 times them would be NaN in every row), with a mark on
+//              the rows that see them
+// All roles run ahead across tiles: only Q (single buffer) and the accumulator wait for a tile's end.
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <float.h>
+
+#include <algorithm>
+
+#include "dc_internal.h"
+#include "dc_ptx.cuh"
+
+using namespace dcx;
+
+namespace {
+
+constexpr int PA_SOFT = 8;
+constexpr int PA_WK = 8, PA_WV = 9, PA_WM = 10, PA_WC = 11;
+constexpr int PA_THREADS = 12 * 32;
+constexpr int PA_RING = 4;
+constexpr int PA_GOFF = 512;  // group offsets kept in shared memory when there are at most so many
+
+enum { RUN_FIRST = 1, RUN_LAST = 2, RUN_TFIRST = 4, RUN_TLAST = 8, RUN_END = 16 };
+
+// A run of blocks of one segment (the prefix or one sequence's own keys) for one tile.
+struct Run {
+  const int *tab;          // its page row
+  int tok0, ntok, kvh;     // the tile
+  int flags, item;
+  int seg;                 // sequence, or -1: the prefix
+  int s;                   // the sequence the run was found at
+  int kb, nb, kend;        // first block, blocks, keys of the segment that the tile's last row in it sees
+  int qb, qe, len;         // own runs: the sequence's rows and own keys
+};
+
+template <int D>
+struct PCfg {
+  static constexpr int KB = 64, NA = D / 64;
+  static constexpr int NST = D == 64 ? 4 : 2;  // stages of the K and of the V ring
+  static constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = KB * D * 2;
+  static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + NST * KV_BYTES;
+  static constexpr int BAR_OFF = V_OFF + NST * KV_BYTES;
+  static constexpr int B_QF = 0, B_QE = 1, B_OD = 2, B_OE = 3, B_OR = 4, B_SF = 5, B_PF = 7, B_XB = 9, B_KF = 13,
+                       B_KE = B_KF + NST, B_VF = B_KE + NST, B_VE = B_VF + NST, B_VS = B_VE + NST,
+                       B_IF = B_VS + NST, B_IE = B_IF + PA_RING, NBARS = B_IE + PA_RING;
+  static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15);
+  // misc: tmem slot, abort, start (s, g, off), poison [4][4], scan [12], runs, goff
+  static constexpr int POISON_OFF = MISC_OFF + 64, SCAN_OFF = POISON_OFF + 64, RUN_OFF = SCAN_OFF + 128,
+                       GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run), XCH_OFF = GOFF_OFF + (PA_GOFF + 4) * 4;
+  static constexpr int SMEM = XCH_OFF + 2 * 2 * 128 * 4 + 1024;
+  static constexpr int S_COL = 0, O_COL = 2 * KB;
+  static constexpr int TCOLS = O_COL + D <= 256 ? 256 : 512;
+  static constexpr int CTAS = TCOLS == 256 ? 2 : 1;
+  static_assert(SMEM * CTAS <= 227 * 1024, "shared memory");
+};
+
+struct PArgs {
+  __half *Y;
+  const int *table, *lens, *qoff, *ptable, *plens, *goff;
+  int *hdr, *recF, *recL;
+  float2 *ml;
+  float *O;
+  uint32_t *err;
+  long ystride;
+  int tstride, pstride, S, G, T, heads, kv, r, tpt, page, pages, chunk_min;
+  float scale_log2;
+};
+
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t lbo) {
+  // MN-major operand in 128-byte-swizzled {64, rows} boxes: 8-row groups 1024 bytes apart, 64-wide chunks `lbo` apart
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+__device__ __forceinline__ void st_global_v8(float *p, const uint32_t *r) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// own keys that query row `t` of a sequence [.., qe) with `len` own tokens sees
+__device__ __forceinline__ int own_limit(int t, int qe, int len) { return max(len - (qe - 1 - t), 0); }
+__device__ __forceinline__ int own_cost(int lim) { return max(1, (lim + 63) >> 6); }
+
+struct Groups {  // the group offsets, from shared memory when they fit
+  const int *p;
+  int G;
+  __device__ __forceinline__ int of(int s) const {  // the last g with goff[g] <= s
+    int lo = 0, hi = G;
+    while (hi - lo > 1) {
+      const int m = (lo + hi) >> 1;
+      if (p[m] <= s) lo = m; else hi = m;
+    }
+    return lo;
+  }
+};
+
+struct Group {
+  int tg, te, pb;  // its rows, its prefix's blocks
+};
+__device__ __forceinline__ Group group_of(const PArgs &a, const Groups &gs, int g) {
+  Group r;
+  if (a.G == 0) {
+    r.tg = a.qoff[0], r.te = a.qoff[a.S], r.pb = 0;
+  } else {
+    r.tg = a.qoff[gs.p[g]], r.te = a.qoff[gs.p[g + 1]], r.pb = (a.plens[g] + 63) >> 6;
+  }
+  return r;
+}
+
+// The units of a sequence: for each tile its rows touch, the prefix's blocks if the tile starts in it, and its own.
+__device__ __forceinline__ long seq_cost(const PArgs &a, const Group &g, int qb, int qe, int len) {
+  long c = 0;
+  const int lo = qb - g.tg, hi = qe - g.tg;
+  if (hi <= lo) return 0;
+  for (int ts = lo / a.tpt * a.tpt; ts < hi; ts += a.tpt) {
+    if (ts >= lo) c += g.pb;
+    c += own_cost(own_limit(g.tg + min(hi, ts + a.tpt) - 1, qe, len));
+  }
+  return c;
+}
+
+// Page ids of a run in order, 32 at a time, the next 32 on their way.
+struct Pages {
+  const int *tab;
+  int base, count, cur, nxt;
+  __device__ __forceinline__ int ld(int i) const { return i < count ? tab[i] : -1; }
+  __device__ __forceinline__ void start(const Run &r, int page, int lane) {
+    tab = r.tab, count = (r.kend + page - 1) / page, base = r.kb * 64 / page;
+    cur = ld(base + lane), nxt = ld(base + 32 + lane);
+  }
+  __device__ __forceinline__ int get(int i, int lane, int add) {  // i: the warp's, add: the lane's
+    if (i - base >= 32) base += 32, cur = nxt, nxt = ld(base + 32 + lane);
+    return __shfl_sync(0xffffffffu, cur, (i - base + add) & 31);
+  }
+};
+
+// The whole warp loads block `b` of the run into `dst` (64 rows; pages that hold none of the run's keys are left out):
+// one box of 64 dims x min(page, 64) rows a lane. Every lane has waited for the stage.
+template <int D>
+__device__ __forceinline__ void load_block(const PArgs &a, const CUtensorMap *map, const Run &r, Pages &pg, int b,
+                                           uint32_t dst, uint32_t full, int lane) {
+  constexpr int NA = D / 64;
+  const int prow = min(a.page, 64), ppb = 64 / prow;
+  const int key0 = (r.kb + b) * 64;
+  const int np = min(ppb, (r.kend - key0 + prow - 1) / prow);
+  const int p = lane / NA, at = lane % NA;
+  const int id = pg.get(key0 / a.page, lane, p);
+  if (lane == 0) mbar_expect_tx(full, (uint32_t)(np * NA * prow * 128));
+  __syncwarp();
+  if (p < np) {
+    int row = a.pages * a.kv * a.page;  // past the cache: zeros
+    if (id >= 0 && id < a.pages)
+      row = (id * a.kv + r.kvh) * a.page + (key0 & (a.page - 1) & ~(prow - 1));
+    else
+      atomicOr(a.err, (uint32_t)DC_DEVERR_BOUNDS);
+    tma_load_2d(dst + at * (64 * 128) + p * prow * 128, map, 64 * at, row, full);
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
+    attention_paged_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                           const __grid_constant__ CUtensorMap tmV, const PArgs a) {
+  using C = PCfg<D>;
+  constexpr int KB = C::KB, NST = C::NST, NA = C::NA;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  auto bar = [&](int i) { return sbase + C::BAR_OFF + 8u * (uint32_t)i; };
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::MISC_OFF);
+  volatile int *abort = reinterpret_cast<volatile int *>(smem + C::MISC_OFF + 4);
+  int *s_start = reinterpret_cast<int *>(smem + C::MISC_OFF + 8);          // s, offset (low, high)
+  volatile uint32_t *poison = reinterpret_cast<volatile uint32_t *>(smem + C::POISON_OFF);  // [item % 4][4 words]
+  long *s_scan = reinterpret_cast<long *>(smem + C::SCAN_OFF);
+  Run *runs = reinterpret_cast<Run *>(smem + C::RUN_OFF);
+  int *s_goff = reinterpret_cast<int *>(smem + C::GOFF_OFF);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int i = 0; i < C::NBARS; i++) {
+      const int n = i == C::B_OE || i == C::B_PF || i == C::B_PF + 1 ? PA_SOFT
+                    : i >= C::B_XB && i < C::B_XB + 4                ? 2
+                    : i >= C::B_IE                                   ? PA_SOFT + 3
+                                                                     : 1;
+      mbar_init(bar(i), n);
+    }
+    *abort = 0;
+    mbar_init_fence();
+  }
+  if (warp == PA_WK && lane == 0) tma_prefetch_desc(&tmQ), tma_prefetch_desc(&tmK);
+  if (warp == PA_WV && lane == 0) tma_prefetch_desc(&tmV);
+  // Tensor memory is taken only when the kernels before are done, and the next kernel is let in only when every CTA
+  // here has its own: of two kernels on an SM, neither can hold columns while it waits for the other.
+  dc_pdl_wait();
+  if (warp == PA_WM) tmem_alloc(smem_u32(tmem_slot), C::TCOLS);
+
+  // ---- the line: units per sequence, their sum, this CTA's stretch
+  Groups gs{a.goff, a.G};
+  if (a.G > 0 && a.G <= PA_GOFF) {
+    for (int i = tid; i <= a.G; i += PA_THREADS) s_goff[i] = a.goff[i];
+    gs.p = s_goff;
+  }
+  __syncthreads();
+  dc_pdl_launch_dependents();
+  bool bad = false;
+  if (a.G > 0) {
+    for (int i = tid; i < a.G; i += PA_THREADS) {
+      const int x = gs.p[i], y = gs.p[i + 1], n = a.plens[i];
+      bad |= x < 0 || y < x || y > a.S || n < 0 || n > (long)a.pstride * a.page || n > (1 << 30);
+    }
+    if (tid == 0) bad |= gs.p[0] != 0 || gs.p[a.G] != a.S;
+  }
+  for (int i = tid; i < a.S; i += PA_THREADS) {
+    const int x = a.qoff[i], y = a.qoff[i + 1], n = a.lens[i];
+    bad |= x < 0 || y < x || y > a.T || n < 0 || n > (long)a.tstride * a.page || n > (1 << 30);
+  }
+  if (__syncthreads_or(bad)) {  // the same in every CTA
+    if (blockIdx.x == 0 && tid == 0) a.hdr[0] = 1, atomicOr(a.err, (uint32_t)DC_DEVERR_BOUNDS);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == PA_WM) tc_fence_after(), tmem_dealloc(*tmem_slot, C::TCOLS);
+    return;
+  }
+  if (blockIdx.x == 0 && tid == 0) a.hdr[0] = 0;
+  const int per = (a.S + PA_THREADS - 1) / PA_THREADS;
+  const int sb = min(tid * per, a.S), se = min(sb + per, a.S);
+  long mine = 0;
+  for (int s = sb; s < se; s++) {
+    const int qb = a.qoff[s], qe = a.qoff[s + 1];
+    if (qe > qb) mine += seq_cost(a, group_of(a, gs, a.G ? gs.of(s) : 0), qb, qe, a.lens[s]);
+  }
+  long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) s_scan[warp] = incl;
+  __syncthreads();
+  long before = incl - mine, line = 0;
+#pragma unroll
+  for (int w = 0; w < PA_THREADS / 32; w++) {
+    if (w < warp) before += s_scan[w];
+    line += s_scan[w];
+  }
+  const long B = line * a.kv;
+  const long chunk = max((long)a.chunk_min, (B + gridDim.x - 1) / gridDim.x);
+  const long p0 = chunk * blockIdx.x, p1 = min(p0 + chunk, B);
+  const bool work = p0 < p1;
+  const int kvh0 = work ? (int)(p0 / line) : 0;
+  if (work && mine > 0) {
+    long off = p0 % line - before;
+    if (off >= 0 && off < mine) {
+      for (int s = sb; s < se; s++) {
+        const int qb = a.qoff[s], qe = a.qoff[s + 1];
+        const long c = qe > qb ? seq_cost(a, group_of(a, gs, a.G ? gs.of(s) : 0), qb, qe, a.lens[s]) : 0;
+        if (off < c) {
+          s_start[0] = s, s_start[1] = (int)(uint32_t)off, s_start[2] = (int)(off >> 32);
+          break;
+        }
+        off -= c;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  auto wait = [&](int i, int parity) {
+    return mbar_wait(bar(i), (uint32_t)parity & 1u, abort, a.err, DC_DEVERR_ATTN_WAIT);
+  };
+  // the whole warp waits, and goes on or gives up together
+  auto wait_warp = [&](int i, int parity) { return __all_sync(0xffffffffu, wait(i, parity)) != 0; };
+  // a consumer's next run: false at the end (or on abort)
+  auto next_run = [&](int n, Run &r) -> bool {
+    if (!wait_warp(C::B_IF + n % PA_RING, n / PA_RING)) return false;
+    r = runs[n % PA_RING];
+    return !(r.flags & RUN_END);
+  };
+  auto done_run = [&](int n) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(C::B_IE + n % PA_RING));
+  };
+
+  if (!work) {
+  } else if (warp == PA_WK) {
+    int n = 0, g = 0, item = -1;  // runs, blocks, tiles
+    bool ok = true, first = true;
+    long pos = p0, off = (long)(uint32_t)s_start[1] | (long)s_start[2] << 32;
+    auto emit = [&](Run &r) -> bool {
+      if (!wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1)) return false;
+      if (r.flags & RUN_FIRST) item++;
+      r.item = item;
+      if (lane == 0) {
+        runs[n % PA_RING] = r;
+        mbar_arrive(bar(C::B_IF + n % PA_RING));
+      }
+      __syncwarp();
+      n++;
+      if (r.flags & RUN_END) return true;
+      if (r.flags & RUN_FIRST) {
+        if (!wait_warp(C::B_QE, item + 1)) return false;
+        if (lane == 0) {
+          mbar_expect_tx(bar(C::B_QF), (uint32_t)(a.r * a.tpt * 128 * NA));
+          for (int j = 0; j < NA; j++)
+            tma_load_3d(sbase + j * 128 * 128, &tmQ, 64 * j, r.kvh * a.r, r.tok0, bar(C::B_QF));
+        }
+        __syncwarp();
+      }
+      if (r.nb > 0) {
+        Pages pg;
+        pg.start(r, a.page, lane);
+        for (int b = 0; b < r.nb; b++, g++) {
+          const int st = g % NST;
+          if (!wait_warp(C::B_KE + st, g / NST + 1)) return false;
+          load_block<D>(a, &tmK, r, pg, b, sbase + C::K_OFF + st * C::KV_BYTES, bar(C::B_KF + st), lane);
+        }
+      }
+      return true;
+    };
+    int s = s_start[0], kvh = kvh0;
+    while (ok && pos < p1 && kvh < a.kv) {
+      const int qb = a.qoff[s], qe = a.qoff[s + 1], len = a.lens[s];
+      if (qe > qb) {
+        const int gi = a.G ? gs.of(s) : 0;
+        const Group gr = group_of(a, gs, gi);
+        const int lo = qb - gr.tg, hi = qe - gr.tg, rows = gr.te - gr.tg;
+        for (int ts = lo / a.tpt * a.tpt; ok && pos < p1 && ts < hi; ts += a.tpt) {
+          const int pe = min(hi, ts + a.tpt);
+          const bool starts = ts >= lo, ends = pe == min(rows, ts + a.tpt);
+          const int pc = starts ? gr.pb : 0;
+          const int lim = own_limit(gr.tg + pe - 1, qe, len), oc = own_cost(lim);
+          if (off >= pc + oc) {
+            off -= pc + oc;
+            continue;
+          }
+          Run r;
+          r.tok0 = gr.tg + ts, r.ntok = min(rows - ts, a.tpt), r.kvh = kvh, r.s = s;
+          r.qb = qb, r.qe = qe, r.len = len;
+          if (off < pc) {
+            const int units = (int)min((long)(pc - off), p1 - pos);
+            r.tab = a.ptable + (long)gi * a.pstride, r.seg = -1, r.kend = a.plens[gi];
+            r.kb = (int)off, r.nb = units;
+            r.flags = (first ? RUN_FIRST : 0) | (off == 0 ? RUN_TFIRST : 0) | (pos + units == p1 ? RUN_LAST : 0);
+            pos += units, off += units;
+            first = false;
+            ok = emit(r);
+            if (!ok || pos == p1) break;
+          }
+          const int o2 = (int)(off - pc), units = (int)min((long)(oc - o2), p1 - pos);
+          const bool last = ends && o2 + units == oc;
+          r.tab = a.table + (long)s * a.tstride, r.seg = s, r.kend = lim;
+          r.kb = o2, r.nb = lim > 0 ? units : 0;
+          r.flags = (first ? RUN_FIRST : 0) | (starts && off == 0 ? RUN_TFIRST : 0) |
+                    (last || pos + units == p1 ? RUN_LAST : 0) | (last ? RUN_TLAST : 0);
+          pos += units, off = 0;
+          first = (r.flags & RUN_LAST) != 0;
+          ok = emit(r);
+        }
+      }
+      if (++s == a.S) s = 0, kvh++;
+    }
+    if (ok) {
+      Run r = {};
+      r.flags = RUN_END;
+      emit(r);
+    }
+  } else if (warp == PA_WV) {
+    Run r;
+    int g = 0;
+    bool ok = true;
+    for (int n = 0; ok && next_run(n, r); n++) {
+      if (r.nb > 0) {
+        Pages pg;
+        pg.start(r, a.page, lane);
+        for (int b = 0; b < r.nb; b++, g++) {
+          const int st = g % NST;
+          if (!(ok = wait_warp(C::B_VE + st, g / NST + 1))) break;
+          load_block<D>(a, &tmV, r, pg, b, sbase + C::V_OFF + st * C::KV_BYTES, bar(C::B_VF + st), lane);
+        }
+      }
+      if (ok) done_run(n);
+    }
+  } else if (warp == PA_WC) {
+    Run r;
+    int g = 0;
+    bool ok = true;
+    for (int n = 0; ok && next_run(n, r); n++) {
+      volatile uint32_t *mark = poison + 4 * (r.item & 3);
+      if ((r.flags & RUN_FIRST) && lane < 4) mark[lane] = 0;
+      __syncwarp();
+      const bool whole = r.seg < 0 || (r.qb <= r.tok0 && r.qe >= r.tok0 + r.ntok);
+      const int sure = r.seg < 0 ? r.kend : own_limit(r.tok0, r.qe, r.len);  // keys that every row sees, if `whole`
+      for (int b = 0; b < r.nb; b++, g++) {
+        const int st = g % NST;
+        if (!(ok = wait_warp(C::B_VF + st, g / NST))) break;
+        const int key0 = (r.kb + b) * 64, valid = min(64, r.kend - key0);
+        const bool scan = !(whole && key0 + valid <= sure);
+        if (scan || valid < 64) {
+          uint8_t *v = smem + C::V_OFF + st * C::KV_BYTES;
+          int worst = 64;  // the first row with a value that is not finite
+          for (int i = 0; i < 16; i++) {
+            const int row = 4 * i + lane / 8;
+            if (row < valid && !scan) continue;
+#pragma unroll
+            for (int at = 0; at < NA; at++) {
+              uint4 *q = reinterpret_cast<uint4 *>(v + at * (64 * 128) + row * 128 + (lane & 7) * 16);
+              if (row >= valid) {
+                *q = make_uint4(0, 0, 0, 0);
+              } else {
+                const uint4 x = *q;
+                auto big = [](uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; };
+                if (big(x.x) | big(x.y) | big(x.z) | big(x.w)) *q = make_uint4(0, 0, 0, 0), worst = min(worst, row);
+              }
+            }
+          }
+          worst = __reduce_min_sync(0xffffffffu, worst);
+          if (worst < 64 && lane < 4) {
+            // rows of the sequence in this tile that see key key0 + worst
+            const int from = max(max(r.tok0, r.qb), key0 + worst - r.len + r.qe) - r.tok0;
+            const int to = min(r.qe, r.tok0 + r.ntok) - r.tok0;
+            const int x = min(max(from - 32 * lane, 0), 32), y = min(max(to - 32 * lane, 0), 32);
+            const uint32_t upto = y >= 32 ? ~0u : (1u << y) - 1u, under = x >= 32 ? ~0u : (1u << x) - 1u;
+            if (y > x) mark[lane] |= upto & ~under;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(bar(C::B_VS + st));
+      }
+      if (ok) done_run(n);
+    }
+  } else if (warp == PA_WM) {
+    constexpr uint32_t idesc_qk = idesc_f16_f32(128, KB);
+    constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // V MN-major
+    Run r = {};
+    int g = 0;
+    bool ok = true, pend = false, fresh = true;
+    auto pv = [&](int x) -> bool {
+      const int st = x % NST;
+      if (!wait(C::B_PF + (x & 1), x >> 1) || !wait(C::B_VF + st, x / NST) || !wait(C::B_VS + st, x / NST)) return false;
+      if (fresh && !wait(C::B_OE, r.item + 1)) return false;
+      tc_fence_after();
+      const uint32_t v = sbase + C::V_OFF + st * C::KV_BYTES, p = tmem + (uint32_t)(C::S_COL + (x & 1) * KB);
+#pragma unroll
+      for (int kk = 0; kk < KB / 16; kk++)
+        mma_f16_ts(tmem + C::O_COL, p + 8 * kk, desc_mn(v + kk * 2048, KB * 128), idesc_pv, !fresh || kk > 0);
+      fresh = false;
+      mma_commit(bar(C::B_VE + st));
+      mma_commit(bar(C::B_OR));
+      return true;
+    };
+    for (int n = 0; ok && next_run(n, r); n++) {
+      if (lane == 0) {
+        if (r.flags & RUN_FIRST) ok = wait(C::B_QF, r.item), fresh = true;
+        for (int b = 0; ok && b < r.nb; b++, g++) {
+          const int st = g % NST;
+          if (!(ok = wait(C::B_KF + st, g / NST))) break;
+          tc_fence_after();
+          const uint32_t k = sbase + C::K_OFF + st * C::KV_BYTES;
+#pragma unroll
+          for (int kd = 0; kd < D / 16; kd++)
+            mma_f16(tmem + (uint32_t)(C::S_COL + (g & 1) * KB), desc_sw128(sbase + (kd >> 2) * 128 * 128 + (kd & 3) * 32),
+                    desc_sw128(k + (kd >> 2) * KB * 128 + (kd & 3) * 32), idesc_qk, kd > 0);
+          mma_commit(bar(C::B_SF + (g & 1)));
+          mma_commit(bar(C::B_KE + st));
+          if (pend && !(ok = pv(g - 1))) break;
+          pend = true;
+        }
+        if (ok && (r.flags & RUN_LAST)) {
+          mma_commit(bar(C::B_QE));
+          if (pend) ok = pv(g - 1);
+          pend = false;
+          // the accumulator is free for the next tile's first product once this tile's was read
+          if (ok && fresh) ok = wait(C::B_OE, r.item + 1);
+          if (ok) mma_commit(bar(C::B_OD));
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      if (ok) done_run(n);
+    }
+  } else {
+    const int q = warp & 3, hf = warp >> 2;
+    const int row = 32 * q + lane, irow = row / a.r, jrow = row - irow * a.r;
+    const uint32_t lrow = (uint32_t)(32 * q) << 16;
+    float *xch = reinterpret_cast<float *>(smem + C::XCH_OFF);
+    Run r;
+    int g = 0, meets = 0;
+    bool ok = true;
+    // the tile's state
+    bool valid = false, anyv = false, had = false, tfirst = false;
+    int t = 0, seq = -1, lim = 0;
+    float m_ref = -FLT_MAX, l = 0.f;
+    auto meet = [&]() -> bool {  // both warps of the quadrant have written their halves
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::B_XB + q));
+      return wait_warp(C::B_XB + q, meets++);
+    };
+    for (int n = 0; ok && next_run(n, r); n++) {
+      if (r.flags & RUN_FIRST) {
+        t = r.tok0 + irow;
+        valid = irow < r.ntok && irow < a.tpt;
+        anyv = __any_sync(0xffffffffu, valid);
+        had = false, tfirst = (r.flags & RUN_TFIRST) != 0;
+        m_ref = -FLT_MAX, l = 0.f;
+        seq = -1, lim = 0;
+        if (valid && t >= r.qb) {  // its sequence: the last at or after the run's whose rows begin at or before it
+          int x = r.s, y = a.S;
+          if (t < r.qe) y = x + 1;
+          while (y - x > 1) {
+            const int m = (x + y) >> 1;
+            if (a.qoff[m] <= t) x = m; else y = m;
+          }
+          seq = x, lim = own_limit(t, a.qoff[x + 1], a.lens[x]);
+        }
+      }
+      const int rlim = !valid ? 0 : r.seg < 0 ? r.kend : seq == r.seg ? lim : 0;
+      for (int b = 0; b < r.nb; b++, g++) {
+        const int sbuf = g & 1;
+        if (!(ok = wait_warp(C::B_SF + sbuf, g >> 1))) break;
+        had = true;
+        const int nv = min(max(rlim - (r.kb + b) * 64, 0), 64);
+        const uint32_t scol = tmem + lrow + (uint32_t)(C::S_COL + sbuf * KB);
+        if (__any_sync(0xffffffffu, nv > 0)) {
+          tc_fence_after();
+          uint32_t x[32];
+          __syncwarp();
+          tmem_ld32(scol + 32 * hf, x);
+          tmem_ld_wait(x);
+          const int nh = min(max(nv - 32 * hf, 0), 32);
+          const uint32_t vis = nh >= 32 ? ~0u : (1u << nh) - 1u;
+          float m4[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX};
+#pragma unroll
+          for (int e = 0; e < 32; e++) {
+            const float v = __uint_as_float(x[e]) * a.scale_log2;
+            x[e] = __float_as_uint(v);
+            m4[e & 3] = fmaxf(m4[e & 3], ((vis >> e) & 1u) ? v : -FLT_MAX);
+          }
+          const float pmx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          const int par = meets & 1;
+          xch[(par * 2 + hf) * 128 + row] = pmx;
+          if (!(ok = meet())) break;
+          const float mx = fmaxf(pmx, xch[(par * 2 + (hf ^ 1)) * 128 + row]);
+          const bool grow = mx > m_ref + 8.0f;
+          const bool resc = grow && m_ref > -FLT_MAX;
+          if (__any_sync(0xffffffffu, resc)) {
+            if (!(ok = wait_warp(C::B_OR, g - 1))) break;  // the products so far
+            tc_fence_after();
+            const float f = resc ? ex2_approx(m_ref - mx) : 1.0f;
+            l *= f;
+            const uint32_t ocol = tmem + lrow + (uint32_t)(C::O_COL + hf * (D / 2));
+#pragma unroll 1
+            for (int c = 0; c < D / 2; c += 16) {
+              uint32_t o[16];
+              __syncwarp();
+              tmem_ld16(ocol + c, o);
+              tmem_ld_wait(o);
+#pragma unroll
+              for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              __syncwarp();
+              tmem_st16(ocol + c, o);
+            }
+            tmem_st_wait();
+          }
+          if (grow) m_ref = mx;
+          const float ref = m_ref - 7.0f;
+          float r4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float p0 = ((vis >> e) & 1u) ? ex2_approx(__uint_as_float(x[e]) - ref) : 0.f;
+            const float p1 = ((vis >> (e + 1)) & 1u) ? ex2_approx(__uint_as_float(x[e + 1]) - ref) : 0.f;
+            const __half2 hp = __floats2half2_rn(p0, p1);
+            const float2 back = __half22float2(hp);
+            r4[(e >> 1) & 3] += back.x + back.y;
+            x[e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
+          }
+          l += (r4[0] + r4[1]) + (r4[2] + r4[3]);
+          __syncwarp();
+          tmem_st16(scol + 16 * hf, *reinterpret_cast<const uint32_t (*)[16]>(&x[0]));
+          tmem_st_wait();
+        } else if (anyv) {  // none of these rows sees the block: zero weights (both warps of the quadrant agree)
+          const uint32_t z[16] = {};
+          tc_fence_after();
+          __syncwarp();
+          tmem_st16(scol + 16 * hf, z);
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::B_PF + sbuf));
+      }
+      if (!ok) break;
+      if (r.flags & RUN_LAST) {
+        if (!(ok = wait_warp(C::B_OD, r.item))) break;
+        tc_fence_after();
+        const bool tlast = (r.flags & RUN_TLAST) != 0, direct = tfirst && tlast;
+        if (anyv) {
+          const int par = meets & 1;
+          xch[(par * 2 + hf) * 128 + row] = l;
+          if (!(ok = meet())) break;
+          float lt = l + xch[(par * 2 + (hf ^ 1)) * 128 + row];
+          if (had && valid && ((poison[4 * (r.item & 3) + (irow >> 5)] >> (irow & 31)) & 1u))
+            lt = __int_as_float(0x7fc00000);
+          const int h = r.kvh * a.r + jrow;
+          const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
+          if (valid && jrow == 0 && hf == 0) {
+            if (tfirst) a.recF[(long)r.kvh * a.T + t] = direct ? -1 : (int)blockIdx.x;
+            if (tlast) a.recL[(long)r.kvh * a.T + t] = (int)blockIdx.x;
+          }
+          if (!direct && valid && hf == 0) a.ml[prow] = make_float2(m_ref, lt);
+          const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+          const uint32_t ocol = tmem + lrow + (uint32_t)(C::O_COL + hf * (D / 2));
+          __half *y = a.Y + (long)t * a.ystride + (long)h * D + hf * (D / 2);
+          float *po = a.O + prow * D + hf * (D / 2);
+#pragma unroll 1
+          for (int c = 0; c < D / 2; c += 16) {
+            uint32_t o[16];
+            __syncwarp();
+            tmem_ld16(ocol + c, o);
+            tmem_ld_wait(o);
+            if (!valid) continue;
+            if (direct) {
+              uint32_t w[8];
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                const __half2 hv = __floats2half2_rn(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+                w[e] = lt == 0.f ? 0u : *reinterpret_cast<const uint32_t *>(&hv);
+              }
+              *reinterpret_cast<uint4 *>(y + c) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4 *>(y + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            } else if (lt != 0.f) {
+              st_global_v8(po + c, o), st_global_v8(po + c + 8, o + 8);
+            }
+          }
+          __syncwarp();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::B_OE));
+      }
+      done_run(n);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == PA_WM) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TCOLS);
+  }
+}
+
+// Joins the parts of the rows whose tiles were cut: y = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over the CTAs c
+// from the tile's first to its last, in that order. W warps to a row, each every W-th part.
+template <int D, int W>
+__global__ void __launch_bounds__(128) attention_join_kernel(const PArgs a) {
+  dc_pdl_begin();
+  constexpr int N = D / 32;  // a lane's values
+  __shared__ float s_o[W > 1 ? W : 1][W > 1 ? D : 1];
+  __shared__ float s_m[4], s_l[4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (a.hdr[0]) return;
+  const long idx = W > 1 ? (long)blockIdx.x : (long)blockIdx.x * 4 + warp;
+  const long t = idx / a.heads;
+  if (t >= a.T || t < a.qoff[0] || t >= a.qoff[a.S]) return;
+  const int h = (int)(idx - t * a.heads), kvh = h / a.r, j = h - kvh * a.r;
+  const int c0 = a.recF[(long)kvh * a.T + t];
+  if (c0 < 0) return;
+  const int c1 = a.recL[(long)kvh * a.T + t];
+  // part c of this row: row base + 128 c
+  const long base = ((long)kvh * a.T + t) * a.r + j;
+  const int first = W > 1 ? c0 + warp : c0;
+  float M = -FLT_MAX;
+  for (int c = first + W * lane; c <= c1; c += W * 32) {
+    const float2 x = a.ml[base + 128L * c];
+    if (x.y != 0.f) M = fmaxf(M, x.x);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float L = 0.f, o[N] = {};
+  for (int cb = first; cb <= c1; cb += W * 32) {
+    const int c = cb + W * lane;
+    float w = 0.f;
+    if (c <= c1) {
+      const float2 x = a.ml[base + 128L * c];
+      if (x.y != 0.f) w = ex2_approx(x.x - M), L += w * x.y;
+      if (x.y == 0.f) w = -1.f;  // nothing stored
+    } else {
+      w = -1.f;
+    }
+    const int cnt = min(32, (c1 - cb) / W + 1);
+#pragma unroll 4
+    for (int i = 0; i < cnt; i++) {
+      const float wi = __shfl_sync(0xffffffffu, w, i);
+      if (wi < 0.f) continue;
+      const float *p = a.O + (base + 128L * (cb + W * i)) * D + N * lane;
+#pragma unroll
+      for (int e = 0; e < N; e++) o[e] = fmaf(wi, p[e], o[e]);
+    }
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+  if (W > 1) {
+    if (lane == 0) s_m[warp] = M, s_l[warp] = L;
+    __syncthreads();
+    const float all = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    const float f = s_l[warp] == 0.f ? 0.f : ex2_approx(M - all);
+#pragma unroll
+    for (int e = 0; e < N; e++) s_o[warp][N * lane + e] = o[e] * f;
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; w++)
+      if (s_l[w] != 0.f) L += s_l[w] * ex2_approx(s_m[w] - all);
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      o[e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; w++) o[e] += s_o[w][N * lane + e];
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.0f / L;
+  __half *y = a.Y + t * a.ystride + (long)h * D + N * lane;
+#pragma unroll
+  for (int e = 0; e < N; e += 2)
+    *reinterpret_cast<__half2 *>(y + e) = __floats2half2_rn(o[e] * inv, o[e + 1] * inv);
+}
+
+typedef CUresult (*EncodeTiledP)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int encode(CUtensorMap *m, const void *p, int rank, const cuuint64_t *dims, const cuuint64_t *strides,
+           const cuuint32_t *box) {
+  static EncodeTiledP enc = nullptr;
+  if (!enc) {
+    void *f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      enc = reinterpret_cast<EncodeTiledP>(f);
+  }
+  DC_CHECK(enc, DC_ECUDA, "decision.js: cuTensorMapEncodeTiled is unavailable");
+  const cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void *>(p), dims, strides, box, es,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  DC_CHECK(r == CUDA_SUCCESS, DC_ECUDA, "decision.js: attention_paged: tensor map encode failed (%d)", (int)r);
+  return DC_OK;
+}
+
+size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// The workspace: a status word, each tile's first and last CTA by (kv head, row), parts' maxima and sums, parts' sums
+// of values. Part c of a tile starts at row (kvh T + tile) r + 128 c: along the line either the tile moves on, by at
+// least its rows, or c does, so no two parts meet.
+struct Ws {
+  size_t recF, recL, ml, O, bytes;
+};
+Ws ws_layout(int T, int heads, int kv, int D, int ctas) {
+  Ws w;
+  const size_t rows = (size_t)T * heads + 128 * (size_t)(ctas + 1);
+  w.recF = 256;
+  w.recL = w.recF + up((size_t)T * kv * 4);
+  w.ml = w.recL + up((size_t)T * kv * 4);
+  w.O = w.ml + up(rows * 8);
+  w.bytes = w.O + up(rows * (size_t)D * 4);
+  return w;
+}
+
+int ctas_of(int D) { return D == 64 ? PCfg<64>::CTAS : D == 128 ? PCfg<128>::CTAS : PCfg<256>::CTAS; }
+
+template <int D>
+int launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, const PArgs &a) {
+  using C = PCfg<D>;
+  CUtensorMap tq;
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)a.heads, (cuuint64_t)a.T};
+  const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)qs * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)a.r, (cuuint32_t)a.tpt};
+  int rc = encode(&tq, Q, 3, dims, strides, box);
+  if (rc) return rc;
+  static uint64_t attr_done = 0;
+  if (!(attr_done & (1ull << ctx->device))) {
+    DC_CUDA(cudaFuncSetAttribute(attention_paged_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    attr_done |= 1ull << ctx->device;
+  }
+  DC_CUDA(dc_launch_pdl(ctx->stream, attention_paged_kernel<D>, dim3(ctx->sms * C::CTAS), dim3(PA_THREADS), C::SMEM, tq,
+                        c->mapK, c->mapV, a));
+  rc = dc_launch_check("attention_paged");
+  if (rc) return rc;
+  const long rows = (long)a.T * a.heads;
+  if (rows <= 8192)
+    DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D, 4>, dim3((unsigned)rows), dim3(128), 0, a));
+  else
+    DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D, 1>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, a));
+  return dc_launch_check("attention_paged (join)");
+}
+
+}  // namespace
+
+int attn_cache_maps(dc_kv_cache *c) {
+  const cuuint64_t dims[2] = {(cuuint64_t)c->D, (cuuint64_t)c->pages * c->kv * c->page};
+  const cuuint64_t strides[1] = {(cuuint64_t)c->D * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)std::min(c->page, 64)};
+  int rc = encode(&c->mapK, c->K, 2, dims, strides, box);
+  return rc ? rc : encode(&c->mapV, c->V, 2, dims, strides, box);
+}
+
+size_t attn_paged_ws(dc_ctx *ctx, const dc_kv_cache *c, int T, int heads) {
+  return ws_layout(T, heads, c->kv, c->D, ctx->sms * ctas_of(c->D)).bytes;
+}
+
+int attn_paged_launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, const int *table, int tstride,
+                      const int *lens, const int *qoff, int S, const int *ptable, int pstride, const int *plens,
+                      const int *goff, int G, void *Y, long ys, int T, int heads, float scale, void *ws) {
+  const Ws w = ws_layout(T, heads, c->kv, c->D, ctx->sms * ctas_of(c->D));
+  char *p = static_cast<char *>(ws);
+  PArgs a;
+  a.Y = static_cast<__half *>(Y), a.ystride = ys;
+  a.table = table, a.lens = lens, a.qoff = qoff, a.ptable = ptable, a.plens = plens, a.goff = goff;
+  a.hdr = reinterpret_cast<int *>(p), a.recF = reinterpret_cast<int *>(p + w.recF);
+  a.recL = reinterpret_cast<int *>(p + w.recL), a.ml = reinterpret_cast<float2 *>(p + w.ml);
+  a.O = reinterpret_cast<float *>(p + w.O);
+  a.err = ctx->d_err;
+  a.tstride = tstride, a.pstride = pstride, a.S = S, a.G = G, a.T = T, a.heads = heads, a.kv = c->kv;
+  a.r = heads / c->kv, a.tpt = 128 / a.r, a.page = c->page, a.pages = c->pages;
+  a.chunk_min = 4;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  if (c->D == 64) return launch<64>(ctx, c, Q, qs, a);
+  if (c->D == 128) return launch<128>(ctx, c, Q, qs, a);
+  return launch<256>(ctx, c, Q, qs, a);
+}

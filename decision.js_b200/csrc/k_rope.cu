@@ -1,0 +1,252 @@
+// Rotary positions with any frequencies, and appending keys and values to a paged cache with the rotation on the way.
+//
+// Rotation: pair i of a head (dims i and i + rot/2, or 2i and 2i + 1) at position p turns by the angle p w_i:
+//   (a, b) -> f (a cos - b sin, b cos + a sin).
+// The angle is kept as a fraction of a turn in 64-bit fixed point: a plan holds w_i / 2 pi as a 64-bit fraction, and
+// p times it modulo 2^64 is the fraction of a turn left after the whole ones, with no rounding at all. A 32-bit
+// product p w_i would be off by 2^-24 of itself: 0.06 rad at a million radians. What is left is a number in [-1, 1)
+// half turns, which sincospif takes as it is.
+//
+// Both kernels read and write each row once and are bound by memory (many tokens) or by the launch (few).
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "dc_internal.h"
+
+namespace {
+
+__device__ __forceinline__ uint4 ld16(const __half *p) { return *reinterpret_cast<const uint4 *>(p); }
+__device__ __forceinline__ void st16(__half *p, const uint4 &u) { *reinterpret_cast<uint4 *>(p) = u; }
+
+__device__ __forceinline__ void unpack8(const uint4 &u, float (&f)[8]) {
+  const __half2 *h = reinterpret_cast<const __half2 *>(&u);
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const float2 v = __half22float2(h[j]);
+    f[2 * j] = v.x, f[2 * j + 1] = v.y;
+  }
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  uint4 u;
+  __half2 *h = reinterpret_cast<__half2 *>(&u);
+#pragma unroll
+  for (int j = 0; j < 4; j++) h[j] = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+  return u;
+}
+
+// factor * cos and factor * sin of eight consecutive pairs at position p
+__device__ __forceinline__ void angles8(const uint64_t *freq, int p, float factor, float (&cs)[8], float (&sn)[8]) {
+  uint64_t f[8];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const ulonglong2 v = reinterpret_cast<const ulonglong2 *>(freq)[j];
+    f[2 * j] = v.x, f[2 * j + 1] = v.y;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const uint64_t turn = (uint64_t)(int64_t)p * f[e];  // modulo one turn
+    const float half_turns = (float)(int)(turn >> 32) * 0x1p-31f;
+    float s, c;
+    sincospif(half_turns, &s, &c);
+    cs[e] = c * factor, sn[e] = s * factor;
+  }
+}
+
+// The eight pairs of a unit, two 16-byte chunks: dims 8c.. and 8c + rot/2.. (half layout), or 16 dims in a row.
+template <bool INTER>
+__device__ __forceinline__ void rotate(float (&a)[8], float (&b)[8], const float (&cs)[8], const float (&sn)[8]) {
+  if (INTER) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], w = b[2 * i + 1];
+      a[2 * i] = x * cs[i] - y * sn[i], a[2 * i + 1] = y * cs[i] + x * sn[i];
+      b[2 * i] = z * cs[4 + i] - w * sn[4 + i], b[2 * i + 1] = w * cs[4 + i] + z * sn[4 + i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float x = a[i], y = b[i];
+      a[i] = x * cs[i] - y * sn[i], b[i] = y * cs[i] + x * sn[i];
+    }
+  }
+}
+
+// The two 16-byte chunks of unit u of a head (D / 16 units): the first rot / 16 units hold the pairs, the others what
+// is not rotated.
+template <bool INTER>
+__device__ __forceinline__ int2 unit_chunks(int u, int rot) {
+  const int nr = rot / 16;
+  if (INTER || u >= nr) return make_int2(2 * u, 2 * u + 1);
+  return make_int2(u, u + nr);
+}
+
+// A thread takes one unit of one token for every HS-th head, so that its angles serve all of them; consecutive
+// threads take the units of a head, then HS heads, then the next token.
+template <bool INTER>
+__global__ void __launch_bounds__(256) rope_kernel(const __half *X, long xs, const int *pos, __half *Y, long ys, int T,
+                                                   int heads, int D, int rot, const uint64_t *freq, float factor,
+                                                   int HS, int tpb) {
+  dc_pdl_begin();
+  const int U = D / 16;
+  const int u = threadIdx.x % U, rest = threadIdx.x / U, hs = rest % HS, tok = rest / HS;
+  const long t = (long)blockIdx.x * tpb + tok;
+  if (tok >= tpb || t >= T) return;
+  const int2 ch = unit_chunks<INTER>(u, rot);
+  const __half *x = X + t * xs;
+  __half *y = Y + t * ys;
+  const bool turn = u < rot / 16;
+  if (!turn && X == Y) return;
+  float cs[8], sn[8];
+  if (turn) angles8(freq + 8 * u, pos[t], factor, cs, sn);
+  constexpr int NB = 4;  // heads in flight
+  for (int h0 = hs; h0 < heads; h0 += NB * HS) {
+    uint4 ra[NB], rb[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+      const int h = h0 + i * HS;
+      if (h < heads) ra[i] = ld16(x + (long)h * D + 8 * ch.x), rb[i] = ld16(x + (long)h * D + 8 * ch.y);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+      const int h = h0 + i * HS;
+      if (h >= heads) continue;
+      if (turn) {
+        float a[8], b[8];
+        unpack8(ra[i], a), unpack8(rb[i], b);
+        rotate<INTER>(a, b, cs, sn);
+        ra[i] = pack8(a), rb[i] = pack8(b);
+      }
+      st16(y + (long)h * D + 8 * ch.x, ra[i]);
+      st16(y + (long)h * D + 8 * ch.y, rb[i]);
+    }
+  }
+}
+
+struct AppendArgs {
+  const __half *Z, *qn, *kn;
+  const int *pos, *slots;
+  __half *Q, *K, *V;
+  const uint64_t *freq;
+  uint32_t *err;
+  long zs, qs;
+  int T, heads, kv, rot, page, nslots, vnorm, W;
+  float eps, factor;
+};
+
+// W warps per token; a pass of a warp covers 32 / (D/16) of the token's q, k and v heads, U = D/16 lanes to a head
+// (one unit each), NP passes with their loads in flight.
+template <int D, bool INTER>
+__global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
+  dc_pdl_begin();
+  constexpr int U = D / 16, HPP = 32 / U, NP = 4;
+  const long wid = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const long t = wid / a.W;
+  if (t >= a.T) return;  // the whole warp
+  const int wsub = (int)(wid % a.W);
+  const int lane = threadIdx.x & 31, u = lane % U, sub = lane / U;
+  const int per = a.heads + 2 * a.kv, npass = (per + HPP - 1) / HPP;
+  const int2 ch = unit_chunks<INTER>(u, a.rot);
+  const bool turn = u < a.rot / 16;
+  const __half *z = a.Z + t * a.zs;
+  const int slot = a.slots[t];
+  const bool stored = slot >= 0 && slot < a.nslots;
+  if (slot >= a.nslots && lane == 0) atomicOr(a.err, (uint32_t)DC_DEVERR_BOUNDS);
+  const int pg = slot / a.page, off = slot % a.page;
+  float cs[8], sn[8];
+  uint4 wq[2] = {}, wk[2] = {};
+  if (a.qn) wq[0] = ld16(a.qn + 8 * ch.x), wq[1] = ld16(a.qn + 8 * ch.y);
+  if (a.kn) wk[0] = ld16(a.kn + 8 * ch.x), wk[1] = ld16(a.kn + 8 * ch.y);
+  if (turn) angles8(a.freq + 8 * u, a.pos[t], a.factor, cs, sn);
+  for (int p0 = wsub; p0 < npass; p0 += NP * a.W) {
+    uint4 ra[NP], rb[NP];
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      const int h = (p0 + i * a.W) * HPP + sub;
+      const bool live = h < a.heads || (h < per && stored);
+      ra[i] = live ? ld16(z + (long)h * D + 8 * ch.x) : make_uint4(0, 0, 0, 0);
+      rb[i] = live ? ld16(z + (long)h * D + 8 * ch.y) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      const int h = (p0 + i * a.W) * HPP + sub;
+      const bool isq = h < a.heads, isk = !isq && h < a.heads + a.kv;
+      const bool normed = isq ? a.qn != nullptr : isk ? a.kn != nullptr : a.vnorm != 0;
+      float x[8], y[8];
+      unpack8(ra[i], x), unpack8(rb[i], y);
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; e++) ss += x[e] * x[e] + y[e] * y[e];
+#pragma unroll
+      for (int o = U / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);  // every lane of the warp
+      if (h >= per) continue;
+      if (normed) {
+        const float inv = rsqrtf(ss * (1.0f / D) + a.eps);
+        float wx[8], wy[8];
+        unpack8(isq ? wq[0] : wk[0], wx), unpack8(isq ? wq[1] : wk[1], wy);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          x[e] *= inv, y[e] *= inv;
+          if (isq || isk) x[e] *= wx[e], y[e] *= wy[e];
+        }
+      }
+      if (turn && (isq || isk)) rotate<INTER>(x, y, cs, sn);
+      __half *dst;
+      if (isq) {
+        dst = a.Q + t * a.qs + (long)h * D;
+      } else {
+        if (!stored) continue;
+        const int hk = h - a.heads - (isk ? 0 : a.kv);
+        dst = (isk ? a.K : a.V) + (((long)pg * a.kv + hk) * a.page + off) * D;
+      }
+      st16(dst + 8 * ch.x, pack8(x));
+      st16(dst + 8 * ch.y, pack8(y));
+    }
+  }
+}
+
+}  // namespace
+
+int ops_rope(dc_ctx *ctx, const dc_rope_plan *p, const void *X, long xs, const int *pos, void *Y, long ys, int T,
+             int heads, int D) {
+  const int U = D / 16;
+  // heads apart: 4 (a warp's threads cover 64 U halves in a row) unless that leaves the card without threads
+  const long want = (148L * 2048 / 2 + (long)T * U - 1) / ((long)T * U);
+  const int most = std::max(1, std::min(heads, 256 / U));
+  const int HS = (int)std::min<long>(most, std::max<long>(want, std::min(4, most)));
+  const int tpb = std::max(1, 256 / (U * HS));
+  const dim3 grid((unsigned)((T + (long)tpb - 1) / tpb));
+  DC_CUDA(dc_launch_pdl(ctx->stream, p->layout == DC_ROPE_INTERLEAVED ? rope_kernel<true> : rope_kernel<false>, grid,
+                        dim3(256), 0, (const __half *)X, xs, pos, (__half *)Y, ys, T, heads, D, p->rot, p->d_freq,
+                        p->factor, HS, tpb));
+  return dc_launch_check("rope");
+}
+
+int ops_kv_append(dc_ctx *ctx, const dc_kv_cache *c, const dc_rope_plan *p, const void *Z, long zs, const void *qn,
+                  const void *kn, float eps, int vnorm, const int *pos, const int *slots, void *Q, long qs, int T,
+                  int heads) {
+  AppendArgs a;
+  a.Z = (const __half *)Z, a.qn = (const __half *)qn, a.kn = (const __half *)kn;
+  a.pos = pos, a.slots = slots;
+  a.Q = (__half *)Q, a.K = (__half *)c->K, a.V = (__half *)c->V;
+  a.freq = p ? p->d_freq : nullptr, a.factor = p ? p->factor : 1.0f, a.rot = p ? p->rot : 0;
+  a.err = ctx->d_err;
+  a.zs = zs, a.qs = qs;
+  a.T = T, a.heads = heads, a.kv = c->kv, a.page = c->page, a.nslots = c->pages * c->page;
+  a.vnorm = vnorm, a.eps = eps;
+  const int npass = (heads + 2 * c->kv + 512 / c->D - 1) / (512 / c->D);
+  // warps per token: one, which works the angles out once for all heads, unless that leaves the card without warps
+  a.W = (int)std::max<long>(1, std::min<long>(npass, (148L * 32 + T - 1) / T));
+  const dim3 grid((unsigned)(((long)T * a.W + 7) / 8));
+  const bool inter = p && p->layout == DC_ROPE_INTERLEAVED;
+#define APPEND(DD)                                                                                               \
+  if (c->D == DD)                                                                                                \
+    DC_CUDA(dc_launch_pdl(ctx->stream, inter ? kv_append_kernel<DD, true> : kv_append_kernel<DD, false>, grid,   \
+                          dim3(256), 0, a));
+  APPEND(64) APPEND(128) APPEND(256)
+#undef APPEND
+  return dc_launch_check("kv_append");
+}

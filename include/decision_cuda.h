@@ -61,8 +61,23 @@ enum {
   DC_ACT_GELU_ERF = 2   /* GELU_MUL with erf (Laya), src/encoder-kernels.ts:26-44; dc_glu only */
 };
 
+/* Which dims make a rotary pair: (i, i + rot/2), as every model of the reference, or (2i, 2i + 1). */
+enum { DC_ROPE_HALF = 0, DC_ROPE_INTERLEAVED = 1 };
+
+/* How dc_rope_frequencies stretches the frequencies theta^(-2i/rot) for a context `factor` times the trained one. */
+enum {
+  DC_ROPE_PLAIN = 0,
+  DC_ROPE_LINEAR = 1, /* every position divided by factor */
+  DC_ROPE_NTK = 2,    /* theta * factor^(rot / (rot - 2)) */
+  DC_ROPE_YARN = 3,   /* plain above `a` turns in the trained context, divided below `b`, a ramp between over the pair
+                       * index; cos and sin times 0.1 ln(factor) + 1 (usual: a = 32, b = 1) */
+  DC_ROPE_BANDS = 4   /* plain above `a` turns, divided below `b`, a ramp between over the turns (usual: 4, 1) */
+};
+
 typedef struct dc_ctx dc_ctx;
 typedef struct dc_model dc_model;
+typedef struct dc_rope_plan dc_rope_plan;
+typedef struct dc_kv_cache dc_kv_cache;
 
 /* ------------------------------------------------------------------ context and memory
  * Replaces requestDevice (src/gpu.ts:38-54) and the buffer helpers storage / activations / destroy
@@ -255,6 +270,75 @@ DC_API int dc_score(dc_ctx *ctx, const void *d_Y, const void *d_w, const void *d
  * 16 to min(D, 256). */
 DC_API int dc_qk_rope(dc_ctx *ctx, void *d_Z, const void *d_qn, const void *d_kn, const int32_t *d_pos, int T,
                       int heads, int kv, int D, long stride, int rot, int norm, float eps, float theta);
+
+/* ------------------------------------------------------------------ a paged key/value cache
+ * No reference counterpart: the reference packs a state and its questions into one pass and computes the state again
+ * for every call. With these a host keeps a state's keys and values on the GPU, appends each new question's, and
+ * attends from all questions at once. All asynchronous on the context's stream; none allocates, so they can be
+ * captured into CUDA graphs and replayed with other contents of the same arrays. */
+
+/* The frequencies (radians per position) of a head's rot/2 pairs for dc_rope_plan_create, on the host:
+ * h_freq [rot/2], and *h_factor, what cos and sin are multiplied by. `scaling` DC_ROPE_*; factor >= 1 and trained (the
+ * context the model was trained at, in tokens) are read by the scalings that name them, a > b > 0 by YARN and BANDS. */
+DC_API int dc_rope_frequencies(int rot, double theta, int scaling, double factor, double trained, double a, double b,
+                               double *h_freq, double *h_factor);
+/* A rotation plan on the context's device: rot (a multiple of 16, at most 512) dims of each head turn, in pairs by
+ * `layout` (DC_ROPE_*), by position * h_freq[i] radians (h_freq [rot/2], finite), with cos and sin times factor. The
+ * angles hold for any int32 position: they are worked out modulo a turn in 64-bit fixed point. Waits for its upload;
+ * free it with dc_rope_plan_free (waits for the device). */
+DC_API int dc_rope_plan_create(dc_ctx *ctx, int rot, int layout, const double *h_freq, double factor,
+                               dc_rope_plan **out);
+DC_API int dc_rope_plan_free(dc_rope_plan *plan);
+/* Rotary positions: Y[t, h, :] = X[t, h, :] with its first rot dims turned to position d_pos[t], in f32, rounded to f16
+ * once; the other dims are copied. X and Y are rows of `xstride` and `ystride` halves that start with `heads` heads of
+ * D. D a multiple of 16, at most 512, at least the plan's rot. Y may be X (in place) or rows apart from X's, among them
+ * other columns of the same rows; a partial overlap is DC_EINVAL. Strides are multiples of 8, X and Y 16-byte
+ * aligned. */
+DC_API int dc_rope(dc_ctx *ctx, const dc_rope_plan *plan, const void *d_X, long xstride, const int32_t *d_pos, void *d_Y,
+                   long ystride, int T, int heads, int D);
+
+/* A cache over the caller's buffers d_K and d_V, each f16 [pages, kv, page, D]: page 16, 32, 64 or 128 tokens, D 64,
+ * 128 or 256, pages * kv * page < 2^31. Token slot s is row s % page of page s / page. The handle holds the addresses
+ * only: the buffers must be device memory of the context's device (DC_EINVAL otherwise), stay allocated as long as the
+ * handle is used, and may be created before or after they are filled. One handle per layer. */
+DC_API int dc_kv_cache_create(dc_ctx *ctx, void *d_K, void *d_V, int pages, int page, int kv, int D, dc_kv_cache **out);
+DC_API int dc_kv_cache_free(dc_kv_cache *cache);
+/* Appends the k and v heads of T packed rows and makes their q heads ready: Z rows of zstride halves, q (heads * D)
+ * | k (kv * D) | v (kv * D). q and k: per-head RMSNorm with d_qn / d_kn (f16 [D]) where given, v a plain one with vnorm
+ * (eps added to the mean square), then q and k turn by `plan` (NULL: not at all) to position d_pos[t] (NULL without a
+ * plan). q goes to row t of Q (qstride halves), k and v to slot d_slots[t] of the cache; all in f32, rounded to f16
+ * once. A negative slot stores no k and v (its q is made); one past the cache does the same and flags the device error
+ * word (the next dc_sync returns DC_EINVAL). The slots of a call must differ: of two tokens at one slot either may
+ * stay. Q may be Z itself (same stride: q in place); another overlap of Q with Z, or of the cache with either, is
+ * DC_EINVAL. zstride and qstride are multiples of 8; pointers 16-byte aligned, d_pos and d_slots 4-byte. */
+DC_API int dc_kv_append(dc_ctx *ctx, const dc_kv_cache *cache, const dc_rope_plan *plan, const void *d_Z, long zstride,
+                        const void *d_qn, const void *d_kn, float eps, int vnorm, const int32_t *d_pos,
+                        const int32_t *d_slots, void *d_Q, long qstride, int T, int heads);
+/* Attention over the cache for a batch of sequences, a prefix that several share read and multiplied once for all of
+ * them. Sequence s holds the query rows [d_qoff[s], d_qoff[s + 1]) of Q (T rows of qstride halves, `heads` heads of D)
+ * and d_lens[s] own tokens in the pages d_table[s * table_stride + i] (token j in page j / page, row j % page).
+ * Group g holds the sequences [d_goff[g], d_goff[g + 1]) and a prefix of d_plens[g] tokens in the pages
+ * d_ptable[g * ptable_stride + i]; G = 0: no prefixes. Query row i of the n of a sequence reads its group's whole
+ * prefix and its own tokens [0, lens - n + 1 + i): its last query row sees all, as after dc_kv_append of the n rows
+ * (fewer own tokens than rows leave the first rows none). Y (ystride halves a row) gets softmax(scale q . k) v, heads
+ * by GQA as in dc_attention; a row with no key gets zeros. Rows outside [d_qoff[0], d_qoff[S]) are neither read nor
+ * written, nor is anything of the cache past a length. Scores, sums and outputs are f32; the weights are rounded to
+ * f16 for the product with v. A value row that is not finite stays out of the rows that do not see it; those that do
+ * get NaN in its columns or in the whole head.
+ * Offsets must not fall, qoff must lie in [0, T], goff start at 0 and end at S, lens and plens fit their table's row;
+ * otherwise nothing is written, and the next dc_sync returns DC_EINVAL, as it does for a page id outside the cache
+ * (which reads zeros). Unused table entries are not read. Q and Y must not overlap unless Y is Q with its stride.
+ * d_ws: at least dc_attention_paged_workspace bytes, 16-byte aligned, for this call alone until it has run (calls on
+ * one stream can share it; graphs that may run at the same time cannot). heads / kv at most 64; strides are multiples
+ * of 8; Q, Y 16-byte aligned. Runs of one input give the same bits. */
+DC_API int dc_attention_paged(dc_ctx *ctx, const dc_kv_cache *cache, const void *d_Q, long qstride,
+                              const int32_t *d_table, int table_stride, const int32_t *d_lens, const int32_t *d_qoff,
+                              int S, const int32_t *d_ptable, int ptable_stride, const int32_t *d_plens,
+                              const int32_t *d_goff, int G, void *d_Y, long ystride, int T, int heads, float scale,
+                              void *d_ws, size_t ws_bytes);
+/* The bytes dc_attention_paged needs for T rows, S sequences and G groups. */
+DC_API int dc_attention_paged_workspace(dc_ctx *ctx, const dc_kv_cache *cache, int T, int heads, int S, int G,
+                                        size_t *out);
 
 /* ------------------------------------------------------------------ models (manifest.json + weights.bin)
  * Replaces loadWeights (src/gpu.ts:57-88) and the engine graphs (src/eg2-engine.ts, src/d1-3b-engine.ts). */
