@@ -17,8 +17,7 @@
 // Within a CTA:
 //   warps 0-7  softmax, as in the attention over packed rows: two warps per TMEM lane quadrant, thread = row, each
 //              half of a block's keys; the exp2 weights are scaled by 2^7 (the row reference moves when the maximum
-//              grows past 2^8, so they stay under 2^15) to keep small ones out of f16's subnormals, and the sum adds
-//              the rounded weights that the product uses
+//              grows past 2^8, so they stay under 2^15) to keep small ones out of f16's subnormals
 //   warp 8     walks the line, hands runs of blocks to the others through a ring of descriptors, loads Q and K
 //   warp 9     loads V
 //   warp 10    the MMAs (and TMEM)
@@ -88,7 +87,7 @@ struct PArgs {
   float *O;
   uint32_t *err;
   long ystride;
-  int tstride, pstride, S, G, T, heads, kv, r, tpt, page, pages, chunk_min;
+  int tstride, pstride, S, G, T, heads, kv, r, tpt, page, pshift, pages, rows, chunk_min;
   float scale_log2;
 };
 
@@ -146,43 +145,58 @@ __device__ __forceinline__ long seq_cost(const PArgs &a, const Group &g, int qb,
   return c;
 }
 
-// Page ids of a run in order, 32 at a time, the next 32 on their way.
-struct Pages {
+// A run's blocks for a producer warp: page ids are read 32 at a time, the next 32 on their way, and turned into rows of
+// the cache as tensor-map coordinates before the stage is waited for.
+template <int D>
+struct Blocks {
+  static constexpr int NA = D / 64;
   const int *tab;
-  int base, count, cur, nxt;
-  __device__ __forceinline__ int ld(int i) const { return i < count ? tab[i] : -1; }
-  __device__ __forceinline__ void start(const Run &r, int page, int lane) {
-    tab = r.tab, count = (r.kend + page - 1) / page, base = r.kb * 64 / page;
-    cur = ld(base + lane), nxt = ld(base + 32 + lane);
+  int base, count, cur, nxt, kend, kvh;
+  __device__ __forceinline__ int ld(const PArgs &a, int i) const {
+    int row = a.rows;  // past the cache: zeros
+    if (i < count) {
+      const int id = tab[i];
+      if (id >= 0 && id < a.pages)
+        row = (id * a.kv + kvh) << a.pshift;
+      else
+        atomicOr(a.err, (uint32_t)DC_DEVERR_BOUNDS);
+    }
+    return row;
   }
-  __device__ __forceinline__ int get(int i, int lane, int add) {  // i: the warp's, add: the lane's
-    if (i - base >= 32) base += 32, cur = nxt, nxt = ld(base + 32 + lane);
-    return __shfl_sync(0xffffffffu, cur, (i - base + add) & 31);
+  __device__ __forceinline__ void start(const PArgs &a, const Run &r, int lane) {
+    tab = r.tab, kend = r.kend, kvh = r.kvh, count = (kend + a.page - 1) >> a.pshift, base = (r.kb * 64) >> a.pshift;
+    cur = ld(a, base + lane), nxt = ld(a, base + 32 + lane);
+  }
+  // The whole warp: block `kb`'s rows, one per box of min(page, 64) rows (pages that hold none of the run's keys are
+  // left out).
+  struct Rows {
+    int row[4], n, prow;
+  };
+  __device__ __forceinline__ Rows rows(const PArgs &a, int kb, int lane) {
+    Rows x;
+    x.prow = min(a.page, 64);
+    const int key0 = kb * 64, i = key0 >> a.pshift;
+    if (i - base >= 32) base += 32, cur = nxt, nxt = ld(a, base + 32 + lane);
+    x.n = a.page >= 64 ? 1 : min(64 >> a.pshift, (kend - key0 + a.page - 1) >> a.pshift);
+    const int in = key0 & (a.page - 1);  // the second half of a page of 128
+#pragma unroll
+    for (int p = 0; p < 4; p++) {
+      const int v = __shfl_sync(0xffffffffu, cur, (i - base + p) & 31);
+      x.row[p] = v == a.rows ? v : v + in;
+    }
+    return x;
+  }
+  // One thread.
+  __device__ __forceinline__ static void load(const CUtensorMap *map, const Rows &x, uint32_t dst, uint32_t full) {
+    mbar_expect_tx(full, (uint32_t)(x.n * NA * x.prow * 128));
+#pragma unroll
+    for (int p = 0; p < 4; p++) {
+      if (p >= x.n) break;
+#pragma unroll
+      for (int j = 0; j < NA; j++) tma_load_2d(dst + j * (64 * 128) + p * x.prow * 128, map, 64 * j, x.row[p], full);
+    }
   }
 };
-
-// The whole warp loads block `b` of the run into `dst` (64 rows; pages that hold none of the run's keys are left out):
-// one box of 64 dims x min(page, 64) rows a lane. Every lane has waited for the stage.
-template <int D>
-__device__ __forceinline__ void load_block(const PArgs &a, const CUtensorMap *map, const Run &r, Pages &pg, int b,
-                                           uint32_t dst, uint32_t full, int lane) {
-  constexpr int NA = D / 64;
-  const int prow = min(a.page, 64), ppb = 64 / prow;
-  const int key0 = (r.kb + b) * 64;
-  const int np = min(ppb, (r.kend - key0 + prow - 1) / prow);
-  const int p = lane / NA, at = lane % NA;
-  const int id = pg.get(key0 / a.page, lane, p);
-  if (lane == 0) mbar_expect_tx(full, (uint32_t)(np * NA * prow * 128));
-  __syncwarp();
-  if (p < np) {
-    int row = a.pages * a.kv * a.page;  // past the cache: zeros
-    if (id >= 0 && id < a.pages)
-      row = (id * a.kv + r.kvh) * a.page + (key0 & (a.page - 1) & ~(prow - 1));
-    else
-      atomicOr(a.err, (uint32_t)DC_DEVERR_BOUNDS);
-    tma_load_2d(dst + at * (64 * 128) + p * prow * 128, map, 64 * at, row, full);
-  }
-}
 
 template <int D>
 __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
@@ -295,7 +309,7 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
   const uint32_t tmem = *tmem_slot;
 
   auto wait = [&](int i, int parity) {
-    return mbar_wait(bar(i), (uint32_t)parity & 1u, abort, a.err, DC_DEVERR_ATTN_WAIT);
+    return mbar_wait_asleep(bar(i), (uint32_t)parity & 1u, abort, a.err, DC_DEVERR_ATTN_WAIT);
   };
   // the whole warp waits, and goes on or gives up together
   auto wait_warp = [&](int i, int parity) { return __all_sync(0xffffffffu, wait(i, parity)) != 0; };
@@ -328,7 +342,7 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
       if (r.flags & RUN_END) return true;
       if (r.flags & RUN_FIRST) {
         if (!wait_warp(C::B_QE, item + 1)) return false;
-        if (lane == 0) {
+        if (elect_one()) {
           mbar_expect_tx(bar(C::B_QF), (uint32_t)(a.r * a.tpt * 128 * NA));
           for (int j = 0; j < NA; j++)
             tma_load_3d(sbase + j * 128 * 128, &tmQ, 64 * j, r.kvh * a.r, r.tok0, bar(C::B_QF));
@@ -336,12 +350,14 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
         __syncwarp();
       }
       if (r.nb > 0) {
-        Pages pg;
-        pg.start(r, a.page, lane);
+        Blocks<D> bl;
+        bl.start(a, r, lane);
         for (int b = 0; b < r.nb; b++, g++) {
           const int st = g % NST;
+          const typename Blocks<D>::Rows x = bl.rows(a, r.kb + b, lane);
           if (!wait_warp(C::B_KE + st, g / NST + 1)) return false;
-          load_block<D>(a, &tmK, r, pg, b, sbase + C::K_OFF + st * C::KV_BYTES, bar(C::B_KF + st), lane);
+          if (elect_one()) bl.load(&tmK, x, sbase + C::K_OFF + st * C::KV_BYTES, bar(C::B_KF + st));
+          __syncwarp();
         }
       }
       return true;
@@ -399,12 +415,14 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
     bool ok = true;
     for (int n = 0; ok && next_run(n, r); n++) {
       if (r.nb > 0) {
-        Pages pg;
-        pg.start(r, a.page, lane);
+        Blocks<D> bl;
+        bl.start(a, r, lane);
         for (int b = 0; b < r.nb; b++, g++) {
           const int st = g % NST;
+          const typename Blocks<D>::Rows x = bl.rows(a, r.kb + b, lane);
           if (!(ok = wait_warp(C::B_VE + st, g / NST + 1))) break;
-          load_block<D>(a, &tmV, r, pg, b, sbase + C::V_OFF + st * C::KV_BYTES, bar(C::B_VF + st), lane);
+          if (elect_one()) bl.load(&tmV, x, sbase + C::V_OFF + st * C::KV_BYTES, bar(C::B_VF + st));
+          __syncwarp();
         }
       }
       if (ok) done_run(n);
@@ -461,50 +479,59 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
   } else if (warp == PA_WM) {
     constexpr uint32_t idesc_qk = idesc_f16_f32(128, KB);
     constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // V MN-major
+    const uint64_t q0 = desc_sw128(sbase), k0 = desc_sw128(sbase + C::K_OFF), v0 = desc_mn(sbase + C::V_OFF, KB * 128);
     Run r = {};
     int g = 0;
     bool ok = true, pend = false, fresh = true;
     auto pv = [&](int x) -> bool {
       const int st = x % NST;
-      if (!wait(C::B_PF + (x & 1), x >> 1) || !wait(C::B_VF + st, x / NST) || !wait(C::B_VS + st, x / NST)) return false;
-      if (fresh && !wait(C::B_OE, r.item + 1)) return false;
+      if (!wait_warp(C::B_PF + (x & 1), x >> 1) || !wait_warp(C::B_VF + st, x / NST) || !wait_warp(C::B_VS + st, x / NST))
+        return false;
+      if (fresh && !wait_warp(C::B_OE, r.item + 1)) return false;
       tc_fence_after();
-      const uint32_t v = sbase + C::V_OFF + st * C::KV_BYTES, p = tmem + (uint32_t)(C::S_COL + (x & 1) * KB);
+      const uint32_t p = tmem + (uint32_t)(C::S_COL + (x & 1) * KB);
+      const uint64_t v = v0 + (uint32_t)(st * C::KV_BYTES >> 4);
+      if (elect_one()) {
 #pragma unroll
-      for (int kk = 0; kk < KB / 16; kk++)
-        mma_f16_ts(tmem + C::O_COL, p + 8 * kk, desc_mn(v + kk * 2048, KB * 128), idesc_pv, !fresh || kk > 0);
+        for (int kk = 0; kk < KB / 16; kk++)
+          mma_f16_ts(tmem + C::O_COL, p + 8 * kk, v + kk * (2048 >> 4), idesc_pv, !fresh || kk > 0);
+        mma_commit(bar(C::B_VE + st));
+        mma_commit(bar(C::B_OR));
+      }
+      __syncwarp();
       fresh = false;
-      mma_commit(bar(C::B_VE + st));
-      mma_commit(bar(C::B_OR));
       return true;
     };
     for (int n = 0; ok && next_run(n, r); n++) {
-      if (lane == 0) {
-        if (r.flags & RUN_FIRST) ok = wait(C::B_QF, r.item), fresh = true;
-        for (int b = 0; ok && b < r.nb; b++, g++) {
-          const int st = g % NST;
-          if (!(ok = wait(C::B_KF + st, g / NST))) break;
-          tc_fence_after();
-          const uint32_t k = sbase + C::K_OFF + st * C::KV_BYTES;
+      if (r.flags & RUN_FIRST) ok = wait_warp(C::B_QF, r.item), fresh = true;
+      for (int b = 0; ok && b < r.nb; b++, g++) {
+        const int st = g % NST;
+        if (!(ok = wait_warp(C::B_KF + st, g / NST))) break;
+        tc_fence_after();
+        const uint32_t sc = tmem + (uint32_t)(C::S_COL + (g & 1) * KB);
+        const uint64_t k = k0 + (uint32_t)(st * C::KV_BYTES >> 4);
+        if (elect_one()) {
 #pragma unroll
           for (int kd = 0; kd < D / 16; kd++)
-            mma_f16(tmem + (uint32_t)(C::S_COL + (g & 1) * KB), desc_sw128(sbase + (kd >> 2) * 128 * 128 + (kd & 3) * 32),
-                    desc_sw128(k + (kd >> 2) * KB * 128 + (kd & 3) * 32), idesc_qk, kd > 0);
+            mma_f16(sc, q0 + (((kd >> 2) * 128 * 128 + (kd & 3) * 32) >> 4), k + (((kd >> 2) * KB * 128 + (kd & 3) * 32) >> 4),
+                    idesc_qk, kd > 0);
           mma_commit(bar(C::B_SF + (g & 1)));
           mma_commit(bar(C::B_KE + st));
-          if (pend && !(ok = pv(g - 1))) break;
-          pend = true;
         }
-        if (ok && (r.flags & RUN_LAST)) {
-          mma_commit(bar(C::B_QE));
-          if (pend) ok = pv(g - 1);
-          pend = false;
-          // the accumulator is free for the next tile's first product once this tile's was read
-          if (ok && fresh) ok = wait(C::B_OE, r.item + 1);
-          if (ok) mma_commit(bar(C::B_OD));
-        }
+        __syncwarp();
+        if (pend && !(ok = pv(g - 1))) break;
+        pend = true;
       }
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      if (ok && (r.flags & RUN_LAST)) {
+        if (elect_one()) mma_commit(bar(C::B_QE));
+        __syncwarp();
+        if (pend) ok = pv(g - 1);
+        pend = false;
+        // a tile without keys: the last tile's end has to be past before this one's is announced
+        if (ok && fresh) ok = wait_warp(C::B_OE, r.item + 1);
+        if (ok && elect_one()) mma_commit(bar(C::B_OD));
+        __syncwarp();
+      }
       if (ok) done_run(n);
     }
   } else {
@@ -556,15 +583,24 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
           tmem_ld32(scol + 32 * hf, x);
           tmem_ld_wait(x);
           const int nh = min(max(nv - 32 * hf, 0), 32);
-          const uint32_t vis = nh >= 32 ? ~0u : (1u << nh) - 1u;
-          float m4[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX};
+          float sc = a.scale_log2;
+          if (sc <= 0.f) {  // the largest score is not the largest product: scale first
 #pragma unroll
-          for (int e = 0; e < 32; e++) {
-            const float v = __uint_as_float(x[e]) * a.scale_log2;
-            x[e] = __float_as_uint(v);
-            m4[e & 3] = fmaxf(m4[e & 3], ((vis >> e) & 1u) ? v : -FLT_MAX);
+            for (int e = 0; e < 32; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * sc);
+            sc = 1.f;
           }
-          const float pmx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          if (!__all_sync(0xffffffffu, nh == 32)) {  // keys not seen: weight 2^-inf
+            const uint32_t vis = nh >= 32 ? ~0u : (1u << nh) - 1u;
+#pragma unroll
+            for (int e = 0; e < 32; e++) x[e] = ((vis >> e) & 1u) ? x[e] : 0xff800000u;
+          }
+          float m2[2] = {__uint_as_float(x[0]), __uint_as_float(x[1])};
+#pragma unroll
+          for (int e = 2; e < 32; e += 4) {
+            m2[0] = max3(m2[0], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+            if (e + 2 < 32) m2[1] = max3(m2[1], __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+          }
+          const float pmx = fmaxf(m2[0], m2[1]) * sc;
           const int par = meets & 1;
           xch[(par * 2 + hf) * 128 + row] = pmx;
           if (!(ok = meet())) break;
@@ -591,18 +627,18 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
             tmem_st_wait();
           }
           if (grow) m_ref = mx;
-          const float ref = m_ref - 7.0f;
-          float r4[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t ref2 = f32x2(7.0f - m_ref, 7.0f - m_ref), sc2 = f32x2(sc, sc);
+          uint64_t sum[2] = {0, 0};
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float p0 = ((vis >> e) & 1u) ? ex2_approx(__uint_as_float(x[e]) - ref) : 0.f;
-            const float p1 = ((vis >> (e + 1)) & 1u) ? ex2_approx(__uint_as_float(x[e + 1]) - ref) : 0.f;
+            const float2 v = f32x2_split(fma_f32x2(f32x2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, ref2));
+            const float p0 = ex2_approx(v.x), p1 = ex2_approx(v.y);
+            sum[(e >> 1) & 1] = add_f32x2(sum[(e >> 1) & 1], f32x2(p0, p1));
             const __half2 hp = __floats2half2_rn(p0, p1);
-            const float2 back = __half22float2(hp);
-            r4[(e >> 1) & 3] += back.x + back.y;
             x[e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
           }
-          l += (r4[0] + r4[1]) + (r4[2] + r4[3]);
+          const float2 add = f32x2_split(add_f32x2(sum[0], sum[1]));
+          l += add.x + add.y;
           __syncwarp();
           tmem_st16(scol + 16 * hf, *reinterpret_cast<const uint32_t (*)[16]>(&x[0]));
           tmem_st_wait();
@@ -853,6 +889,7 @@ int attn_paged_launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs,
   a.err = ctx->d_err;
   a.tstride = tstride, a.pstride = pstride, a.S = S, a.G = G, a.T = T, a.heads = heads, a.kv = c->kv;
   a.r = heads / c->kv, a.tpt = 128 / a.r, a.page = c->page, a.pages = c->pages;
+  a.pshift = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7, a.rows = c->pages * c->kv * c->page;
   a.chunk_min = 4;
   a.scale_log2 = scale * 1.4426950408889634f;
   if (c->D == 64) return launch<64>(ctx, c, Q, qs, a);
