@@ -65,22 +65,22 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 }
 
 // mbar_wait for warps that wait long beside others that compute: the thread sleeps in the barrier unit (up to the
-// hinted time) instead of polling, whose instructions would take the others' issue slots.
-__device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity, volatile int *abort, uint32_t *err,
-                                                 uint32_t code, uint64_t limit_ns = 2000000000ull) {
-  auto nap = [&]() -> bool {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity), "r"(1000000u)
-        : "memory");
-    return ok != 0;
-  };
-  if (nap()) return true;
-  const uint64_t t0 = globaltimer();
+// hinted time) instead of polling, whose instructions would take the others' issue slots. What follows a nap that ran
+// out is kept out of line: a kernel of several roles has dozens of waits, and its code has to stay in the instruction
+// caches.
+__device__ __forceinline__ bool mbar_nap(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
+}
+static __device__ __noinline__ bool mbar_nap_on(uint32_t bar, uint32_t parity, volatile int *abort, uint32_t *err, uint32_t code) {
+  const uint64_t limit_ns = 2000000000ull, t0 = globaltimer();
   for (;;) {
-    if (nap()) return true;
+    if (mbar_nap(bar, parity)) return true;
     if (*abort) return false;
     if (globaltimer() - t0 > limit_ns) {
       *abort = 1;
@@ -88,6 +88,10 @@ __device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity, 
       return false;
     }
   }
+}
+__device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity, volatile int *abort, uint32_t *err,
+                                                 uint32_t code) {
+  return mbar_nap(bar, parity) || mbar_nap_on(bar, parity, abort, err, code);
 }
 
 // One lane of the (converged) warp: true in it alone. The compiler knows that what it guards runs in one thread, so the
@@ -344,6 +348,16 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// The same, added to D, with the rows (TMEM lanes) whose bits are set in `off` left as they are.
+__device__ __forceinline__ void mma_f16_ts_rows(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                                const uint32_t (&off)[4]) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.eq.b32 p, 0, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%4, %5, %6, %7}, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
       : "memory");
 }
 

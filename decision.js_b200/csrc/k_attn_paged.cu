@@ -43,7 +43,7 @@ constexpr int PA_SOFT = 8;
 constexpr int PA_WK = 8, PA_WV = 9, PA_WM = 10, PA_WC = 11;
 constexpr int PA_THREADS = 12 * 32;
 constexpr int PA_RING = 4;
-constexpr int PA_GOFF = 512;  // group offsets kept in shared memory when there are at most so many
+constexpr int PA_GOFF = 512;  // groups whose offsets are kept in shared memory
 
 enum { RUN_FIRST = 1, RUN_LAST = 2, RUN_TFIRST = 4, RUN_TLAST = 8, RUN_END = 16 };
 
@@ -71,7 +71,7 @@ struct PCfg {
   static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15);
   // misc: tmem slot, abort, start (s, g, off), poison [4][4], scan [12], runs, goff
   static constexpr int POISON_OFF = MISC_OFF + 64, SCAN_OFF = POISON_OFF + 64, RUN_OFF = SCAN_OFF + 128,
-                       GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run), XCH_OFF = GOFF_OFF + (PA_GOFF + 4) * 4;
+                       GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run), XCH_OFF = GOFF_OFF + 3 * (PA_GOFF + 4) * 4;
   static constexpr int SMEM = XCH_OFF + 2 * 2 * 128 * 4 + 1024;
   static constexpr int S_COL = 0, O_COL = 2 * KB;
   static constexpr int TCOLS = O_COL + D <= 256 ? 256 : 512;
@@ -107,14 +107,15 @@ __device__ __forceinline__ void st_global_v8(float *p, const uint32_t *r) {
 __device__ __forceinline__ int own_limit(int t, int qe, int len) { return max(len - (qe - 1 - t), 0); }
 __device__ __forceinline__ int own_cost(int lim) { return max(1, (lim + 63) >> 6); }
 
-struct Groups {  // the group offsets, from shared memory when they fit
-  const int *p;
+struct Groups {  // offsets, prefix lengths and first rows, from shared memory when they fit
+  const int *goff, *plens, *rows;
   int G;
+  int2 whole;  // without groups: all rows
   __device__ __forceinline__ int of(int s) const {  // the last g with goff[g] <= s
     int lo = 0, hi = G;
     while (hi - lo > 1) {
       const int m = (lo + hi) >> 1;
-      if (p[m] <= s) lo = m; else hi = m;
+      if (goff[m] <= s) lo = m; else hi = m;
     }
     return lo;
   }
@@ -124,13 +125,10 @@ struct Group {
   int tg, te, pb;  // its rows, its prefix's blocks
 };
 __device__ __forceinline__ Group group_of(const PArgs &a, const Groups &gs, int g) {
-  Group r;
-  if (a.G == 0) {
-    r.tg = a.qoff[0], r.te = a.qoff[a.S], r.pb = 0;
-  } else {
-    r.tg = a.qoff[gs.p[g]], r.te = a.qoff[gs.p[g + 1]], r.pb = (a.plens[g] + 63) >> 6;
-  }
-  return r;
+  if (gs.G == 0) return Group{gs.whole.x, gs.whole.y, 0};
+  const int pb = (gs.plens[g] + 63) >> 6;
+  if (gs.rows) return Group{gs.rows[g], gs.rows[g + 1], pb};
+  return Group{a.qoff[min(max(gs.goff[g], 0), a.S)], a.qoff[min(max(gs.goff[g + 1], 0), a.S)], pb};
 }
 
 // The units of a sequence: for each tile its rows touch, the prefix's blocks if the tile starts in it, and its own.
@@ -236,39 +234,45 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
   if (warp == PA_WM) tmem_alloc(smem_u32(tmem_slot), C::TCOLS);
 
   // ---- the line: units per sequence, their sum, this CTA's stretch
-  Groups gs{a.goff, a.G};
-  if (a.G > 0 && a.G <= PA_GOFF) {
-    for (int i = tid; i <= a.G; i += PA_THREADS) s_goff[i] = a.goff[i];
-    gs.p = s_goff;
-  }
-  __syncthreads();
-  dc_pdl_launch_dependents();
   bool bad = false;
+  Groups gs{a.goff, a.plens, nullptr, a.G};
   if (a.G > 0) {
-    for (int i = tid; i < a.G; i += PA_THREADS) {
-      const int x = gs.p[i], y = gs.p[i + 1], n = a.plens[i];
-      bad |= x < 0 || y < x || y > a.S || n < 0 || n > (long)a.pstride * a.page || n > (1 << 30);
+    if (a.G <= PA_GOFF) {  // offsets, prefix lengths and first rows into shared memory
+      for (int i = tid; i <= a.G; i += PA_THREADS) {
+        const int x = a.goff[i];
+        s_goff[i] = x;
+        s_goff[2 * (PA_GOFF + 4) + i] = a.qoff[min(max(x, 0), a.S)];
+        if (i < a.G) s_goff[PA_GOFF + 4 + i] = a.plens[i];
+      }
+      gs = Groups{s_goff, s_goff + PA_GOFF + 4, s_goff + 2 * (PA_GOFF + 4), a.G};
     }
-    if (tid == 0) bad |= gs.p[0] != 0 || gs.p[a.G] != a.S;
+  } else {
+    gs.whole = make_int2(a.qoff[0], a.qoff[a.S]);
   }
-  for (int i = tid; i < a.S; i += PA_THREADS) {
-    const int x = a.qoff[i], y = a.qoff[i + 1], n = a.lens[i];
-    bad |= x < 0 || y < x || y > a.T || n < 0 || n > (long)a.tstride * a.page || n > (1 << 30);
-  }
-  if (__syncthreads_or(bad)) {  // the same in every CTA
-    if (blockIdx.x == 0 && tid == 0) a.hdr[0] = 1, atomicOr(a.err, (uint32_t)DC_DEVERR_BOUNDS);
-    tc_fence_before();
-    __syncthreads();
-    if (warp == PA_WM) tc_fence_after(), tmem_dealloc(*tmem_slot, C::TCOLS);
-    return;
-  }
-  if (blockIdx.x == 0 && tid == 0) a.hdr[0] = 0;
   const int per = (a.S + PA_THREADS - 1) / PA_THREADS;
   const int sb = min(tid * per, a.S), se = min(sb + per, a.S);
+  int qb = 0, qe = 0, len = 0;  // the thread's (first) sequence
+  if (sb < se) qb = a.qoff[sb], qe = a.qoff[sb + 1], len = a.lens[sb];
+  __syncthreads();
+  dc_pdl_launch_dependents();
+  if (a.G > 0) {
+    for (int i = tid; i < a.G; i += PA_THREADS) {
+      const int x = gs.goff[i], y = gs.goff[i + 1], n = gs.plens[i];
+      bad |= x < 0 || y < x || y > a.S || n < 0 || n > (long)a.pstride * a.page || n > (1 << 30);
+    }
+    if (tid == 0) bad |= gs.goff[0] != 0 || gs.goff[a.G] != a.S;
+  }
+  // a sequence's units; nothing for offsets that are refused below (the sum is then not used)
+  auto units = [&](int s, int qb, int qe, int len) -> long {
+    if (qb < 0 || qe <= qb || qe > a.T || len < 0) return 0;
+    const Group g = group_of(a, gs, a.G ? gs.of(s) : 0);
+    return g.tg < 0 || g.tg > qb ? 0 : seq_cost(a, g, qb, qe, len);
+  };
   long mine = 0;
   for (int s = sb; s < se; s++) {
-    const int qb = a.qoff[s], qe = a.qoff[s + 1];
-    if (qe > qb) mine += seq_cost(a, group_of(a, gs, a.G ? gs.of(s) : 0), qb, qe, a.lens[s]);
+    const int x = s == sb ? qb : a.qoff[s], y = s == sb ? qe : a.qoff[s + 1], n = s == sb ? len : a.lens[s];
+    bad |= x < 0 || y < x || y > a.T || n < 0 || n > (long)a.tstride * a.page || n > (1 << 30);
+    mine += units(s, x, y, n);
   }
   long incl = mine;
 #pragma unroll
@@ -277,12 +281,20 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
     if (lane >= o) incl += v;
   }
   if (lane == 31) s_scan[warp] = incl;
-  __syncthreads();
+  if (__syncthreads_or(bad)) {  // the same in every CTA
+    if (blockIdx.x == 0 && tid == 0) a.hdr[0] = 1, atomicOr(a.err, (uint32_t)DC_DEVERR_BOUNDS);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == PA_WM) tc_fence_after(), tmem_dealloc(*tmem_slot, C::TCOLS);
+    return;
+  }
+  if (blockIdx.x == 0 && tid == 0) a.hdr[0] = 0;
   long before = incl - mine, line = 0;
 #pragma unroll
   for (int w = 0; w < PA_THREADS / 32; w++) {
-    if (w < warp) before += s_scan[w];
-    line += s_scan[w];
+    const long v = s_scan[w];
+    if (w < warp) before += v;
+    line += v;
   }
   const long B = line * a.kv;
   const long chunk = max((long)a.chunk_min, (B + gridDim.x - 1) / gridDim.x);
@@ -290,17 +302,15 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
   const bool work = p0 < p1;
   const int kvh0 = work ? (int)(p0 / line) : 0;
   if (work && mine > 0) {
-    long off = p0 % line - before;
+    long off = p0 - kvh0 * line - before;
     if (off >= 0 && off < mine) {
-      for (int s = sb; s < se; s++) {
-        const int qb = a.qoff[s], qe = a.qoff[s + 1];
-        const long c = qe > qb ? seq_cost(a, group_of(a, gs, a.G ? gs.of(s) : 0), qb, qe, a.lens[s]) : 0;
-        if (off < c) {
-          s_start[0] = s, s_start[1] = (int)(uint32_t)off, s_start[2] = (int)(off >> 32);
-          break;
-        }
+      int s = sb;
+      for (; s < se - 1; s++) {
+        const long c = units(s, a.qoff[s], a.qoff[s + 1], a.lens[s]);
+        if (off < c) break;
         off -= c;
       }
+      s_start[0] = s, s_start[1] = (int)(uint32_t)off, s_start[2] = (int)(off >> 32);
     }
   }
   tc_fence_before();
@@ -383,7 +393,7 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
           r.qb = qb, r.qe = qe, r.len = len;
           if (off < pc) {
             const int units = (int)min((long)(pc - off), p1 - pos);
-            r.tab = a.ptable + (long)gi * a.pstride, r.seg = -1, r.kend = a.plens[gi];
+            r.tab = a.ptable + (long)gi * a.pstride, r.seg = -1, r.kend = gs.plens[gi];
             r.kb = (int)off, r.nb = units;
             r.flags = (first ? RUN_FIRST : 0) | (off == 0 ? RUN_TFIRST : 0) | (pos + units == p1 ? RUN_LAST : 0);
             pos += units, off += units;
@@ -435,28 +445,37 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
       volatile uint32_t *mark = poison + 4 * (r.item & 3);
       if ((r.flags & RUN_FIRST) && lane < 4) mark[lane] = 0;
       __syncwarp();
-      const bool whole = r.seg < 0 || (r.qb <= r.tok0 && r.qe >= r.tok0 + r.ntok);
-      const int sure = r.seg < 0 ? r.kend : own_limit(r.tok0, r.qe, r.len);  // keys that every row sees, if `whole`
       for (int b = 0; b < r.nb; b++, g++) {
         const int st = g % NST;
         if (!(ok = wait_warp(C::B_VF + st, g / NST))) break;
-        const int key0 = (r.kb + b) * 64, valid = min(64, r.kend - key0);
-        const bool scan = !(whole && key0 + valid <= sure);
-        if (scan || valid < 64) {
-          uint8_t *v = smem + C::V_OFF + st * C::KV_BYTES;
-          int worst = 64;  // the first row with a value that is not finite
-          for (int i = 0; i < 16; i++) {
-            const int row = 4 * i + lane / 8;
-            if (row < valid && !scan) continue;
+        const int key0 = (r.kb + b) * 64, valid = min(64, r.kend - key0), pad = (valid + 15) & ~15;
+        uint8_t *v = smem + C::V_OFF + st * C::KV_BYTES + (lane & 7) * 16;
+        if (valid < pad) {  // up to 15 rows, four at a time
+          for (int row = valid + lane / 8; row < pad; row += 4)
 #pragma unroll
-            for (int at = 0; at < NA; at++) {
-              uint4 *q = reinterpret_cast<uint4 *>(v + at * (64 * 128) + row * 128 + (lane & 7) * 16);
-              if (row >= valid) {
-                *q = make_uint4(0, 0, 0, 0);
-              } else {
-                const uint4 x = *q;
+            for (int at = 0; at < NA; at++) *reinterpret_cast<uint4 *>(v + at * (64 * 128) + row * 128) = make_uint4(0, 0, 0, 0);
+        }
+        // the first row of the tile that sees the block sees the fewest of its keys
+        const int t1 = max(max(r.tok0, r.qb), key0 - r.len + r.qe);
+        const bool scan = r.seg >= 0 && own_limit(t1, r.qe, r.len) < key0 + valid;
+        if (scan) {
+          int worst = 64;  // the first row with a value that is not finite
+#pragma unroll
+          for (int at = 0; at < NA; at++) {
+#pragma unroll
+            for (int i0 = 0; i0 < 16; i0 += 8) {
+              uint4 x[8];
+#pragma unroll
+              for (int i = 0; i < 8; i++)
+                x[i] = *reinterpret_cast<uint4 *>(v + at * (64 * 128) + (4 * (i0 + i) + lane / 8) * 128);
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                const int row = 4 * (i0 + i) + lane / 8;
                 auto big = [](uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; };
-                if (big(x.x) | big(x.y) | big(x.z) | big(x.w)) *q = make_uint4(0, 0, 0, 0), worst = min(worst, row);
+                if (row < valid && (big(x[i].x) | big(x[i].y) | big(x[i].z) | big(x[i].w))) {
+                  *reinterpret_cast<uint4 *>(v + at * (64 * 128) + row * 128) = make_uint4(0, 0, 0, 0);
+                  worst = min(worst, row);
+                }
               }
             }
           }
@@ -469,9 +488,9 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
             const uint32_t upto = y >= 32 ? ~0u : (1u << y) - 1u, under = x >= 32 ? ~0u : (1u << x) - 1u;
             if (y > x) mark[lane] |= upto & ~under;
           }
-          fence_proxy_async_smem();
-          __syncwarp();
         }
+        if (scan || valid < pad) fence_proxy_async_smem();
+        __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::B_VS + st));
       }
       if (ok) done_run(n);
@@ -482,24 +501,24 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
     const uint64_t q0 = desc_sw128(sbase), k0 = desc_sw128(sbase + C::K_OFF), v0 = desc_mn(sbase + C::V_OFF, KB * 128);
     Run r = {};
     int g = 0;
-    bool ok = true, pend = false, fresh = true;
+    bool ok = true, pend = false, fresh = true;  // fresh: the tile has had no block yet
+    int steps = 0;               // of the pending product: 16 keys each,
+    uint32_t off[4] = {};        // and the rows that it leaves alone
     auto pv = [&](int x) -> bool {
       const int st = x % NST;
       if (!wait_warp(C::B_PF + (x & 1), x >> 1) || !wait_warp(C::B_VF + st, x / NST) || !wait_warp(C::B_VS + st, x / NST))
         return false;
-      if (fresh && !wait_warp(C::B_OE, r.item + 1)) return false;
       tc_fence_after();
       const uint32_t p = tmem + (uint32_t)(C::S_COL + (x & 1) * KB);
       const uint64_t v = v0 + (uint32_t)(st * C::KV_BYTES >> 4);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < KB / 16; kk++)
-          mma_f16_ts(tmem + C::O_COL, p + 8 * kk, v + kk * (2048 >> 4), idesc_pv, !fresh || kk > 0);
+          if (kk < steps) mma_f16_ts_rows(tmem + C::O_COL, p + 8 * kk, v + kk * (2048 >> 4), idesc_pv, off);
         mma_commit(bar(C::B_VE + st));
         mma_commit(bar(C::B_OR));
       }
       __syncwarp();
-      fresh = false;
       return true;
     };
     for (int n = 0; ok && next_run(n, r); n++) {
@@ -520,7 +539,18 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
         }
         __syncwarp();
         if (pend && !(ok = pv(g - 1))) break;
-        pend = true;
+        pend = true, fresh = false;
+        const int key0 = (r.kb + b) * 64;
+        steps = (min(64, r.kend - key0) + 15) >> 4;
+        // own blocks: the rows of the sequence that see a key of it
+        const int lo = r.seg < 0 ? 0 : (max(max(r.tok0, r.qb), key0 - r.len + r.qe) - r.tok0) * a.r;
+        const int hi = r.seg < 0 ? 128 : (min(r.qe, r.tok0 + r.ntok) - r.tok0) * a.r;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          const int x = min(max(lo - 32 * w, 0), 32), y = min(max(hi - 32 * w, 0), 32);
+          const uint32_t upto = y >= 32 ? ~0u : (1u << y) - 1u, under = x >= 32 ? ~0u : (1u << x) - 1u;
+          off[w] = ~(upto & ~under);
+        }
       }
       if (ok && (r.flags & RUN_LAST)) {
         if (elect_one()) mma_commit(bar(C::B_QE));
@@ -567,6 +597,14 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
             if (a.qoff[m] <= t) x = m; else y = m;
           }
           seq = x, lim = own_limit(t, a.qoff[x + 1], a.lens[x]);
+        }
+        if (anyv) {  // the last tile's accumulator was read by this very warp
+          const uint32_t z[16] = {};
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < D / 2; c += 16) tmem_st16(tmem + lrow + (uint32_t)(C::O_COL + hf * (D / 2) + c), z);
+          tmem_st_wait();
+          tc_fence_before();
         }
       }
       const int rlim = !valid ? 0 : r.seg < 0 ? r.kend : seq == r.seg ? lim : 0;
@@ -642,13 +680,7 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
           __syncwarp();
           tmem_st16(scol + 16 * hf, *reinterpret_cast<const uint32_t (*)[16]>(&x[0]));
           tmem_st_wait();
-        } else if (anyv) {  // none of these rows sees the block: zero weights (both warps of the quadrant agree)
-          const uint32_t z[16] = {};
-          tc_fence_after();
-          __syncwarp();
-          tmem_st16(scol + 16 * hf, z);
-          tmem_st_wait();
-        }
+        }  // none of these rows sees the block: the product leaves them alone
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::B_PF + sbuf));
@@ -723,43 +755,47 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PArgs a) {
   __shared__ float s_o[W > 1 ? W : 1][W > 1 ? D : 1];
   __shared__ float s_m[4], s_l[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (a.hdr[0]) return;
   const long idx = W > 1 ? (long)blockIdx.x : (long)blockIdx.x * 4 + warp;
   const long t = idx / a.heads;
-  if (t >= a.T || t < a.qoff[0] || t >= a.qoff[a.S]) return;
+  if (t >= a.T) return;
   const int h = (int)(idx - t * a.heads), kvh = h / a.r, j = h - kvh * a.r;
-  const int c0 = a.recF[(long)kvh * a.T + t];
-  if (c0 < 0) return;
-  const int c1 = a.recL[(long)kvh * a.T + t];
+  // all four loads in flight; the records of a row outside the sequences are not defined, and not used
+  const int refused = a.hdr[0], t0 = a.qoff[0], t1 = a.qoff[a.S];
+  const int c0 = a.recF[(long)kvh * a.T + t], c1 = a.recL[(long)kvh * a.T + t];
+  if (refused || t < t0 || t >= t1 || c0 < 0) return;
   // part c of this row: row base + 128 c
   const long base = ((long)kvh * a.T + t) * a.r + j;
   const int first = W > 1 ? c0 + warp : c0;
-  float M = -FLT_MAX;
-  for (int c = first + W * lane; c <= c1; c += W * 32) {
-    const float2 x = a.ml[base + 128L * c];
-    if (x.y != 0.f) M = fmaxf(M, x.x);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  float L = 0.f, o[N] = {};
-  for (int cb = first; cb <= c1; cb += W * 32) {
+  float M = -FLT_MAX, L = 0.f, o[N] = {};
+  for (int cb = first; cb <= c1; cb += W * 32) {  // 32 parts at a time, usually all
     const int c = cb + W * lane;
-    float w = 0.f;
-    if (c <= c1) {
-      const float2 x = a.ml[base + 128L * c];
-      if (x.y != 0.f) w = ex2_approx(x.x - M), L += w * x.y;
-      if (x.y == 0.f) w = -1.f;  // nothing stored
-    } else {
-      w = -1.f;
-    }
+    const float2 x = c <= c1 ? a.ml[base + 128L * c] : make_float2(-FLT_MAX, 0.f);
     const int cnt = min(32, (c1 - cb) / W + 1);
+    float m = x.y == 0.f ? -FLT_MAX : x.x;  // a part of weight 0 stored no values
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+    m = fmaxf(m, M);
+    const float f = ex2_approx(M - m);  // what is there goes to the new maximum (0 the first time)
+    M = m;
+    const float w = x.y == 0.f ? 0.f : ex2_approx(x.x - M);
+    L = L * f + (x.y == 0.f ? 0.f : w * x.y);
+#pragma unroll
+    for (int e = 0; e < N; e++) o[e] *= f;
+    const uint32_t have = __ballot_sync(0xffffffffu, x.y != 0.f);
 #pragma unroll 4
     for (int i = 0; i < cnt; i++) {
       const float wi = __shfl_sync(0xffffffffu, w, i);
-      if (wi < 0.f) continue;
       const float *p = a.O + (base + 128L * (cb + W * i)) * D + N * lane;
+      float v[N];
+      if (N == 2) {
+        *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(p);
+      } else {
 #pragma unroll
-      for (int e = 0; e < N; e++) o[e] = fmaf(wi, p[e], o[e]);
+        for (int e = 0; e < N; e += 4) *reinterpret_cast<float4 *>(v + e) = *reinterpret_cast<const float4 *>(p + e);
+      }
+      const bool use = (have >> i) & 1u;
+#pragma unroll
+      for (int e = 0; e < N; e++) o[e] = use ? fmaf(wi, v[e], o[e]) : o[e];
     }
   }
 #pragma unroll
