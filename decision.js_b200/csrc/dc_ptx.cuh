@@ -89,6 +89,22 @@ static __device__ __noinline__ bool mbar_nap_on(uint32_t bar, uint32_t parity, v
     }
   }
 }
+// For the one thread whose wake-up time everything else waits for: it polls (a sleeper is woken some hundred cycles
+// late), for 10,000 tries at most, then sleeps.
+__device__ __forceinline__ bool mbar_wait_alert(uint32_t bar, uint32_t parity, volatile int *abort, uint32_t *err,
+                                                uint32_t code) {
+#pragma unroll 1
+  for (int i = 0; i < 10000; i++) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return mbar_nap_on(bar, parity, abort, err, code);
+}
 __device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity, volatile int *abort, uint32_t *err,
                                                  uint32_t code) {
   return mbar_nap(bar, parity) || mbar_nap_on(bar, parity, abort, err, code);

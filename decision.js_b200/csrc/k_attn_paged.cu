@@ -15,8 +15,9 @@
 // do not depend on timing.
 //
 // Within a CTA:
-//   warps 0-7  softmax, as in the attention over packed rows: two warps per TMEM lane quadrant, thread = row, each
-//              half of a block's keys; the exp2 weights are scaled by 2^7 (the row reference moves when the maximum
+//   warps 0-7  softmax, two warpgroups that take the blocks in turn, thread = row. A row's reference (the maximum its
+//              weights are relative to) goes from block to block through shared memory, each warp waiting for its
+//              twin's turn only between its own maximum and its weights; the exp2 weights are scaled by 2^7 (the row reference moves when the maximum
 //              grows past 2^8, so they stay under 2^15) to keep small ones out of f16's subnormals
 //   warp 8     walks the line, hands runs of blocks to the others through a ring of descriptors, loads Q and K
 //   warp 9     loads V
@@ -65,14 +66,14 @@ struct PCfg {
   static constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = KB * D * 2;
   static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + NST * KV_BYTES;
   static constexpr int BAR_OFF = V_OFF + NST * KV_BYTES;
-  static constexpr int B_QF = 0, B_QE = 1, B_OD = 2, B_OE = 3, B_OR = 4, B_SF = 5, B_PF = 7, B_XB = 9, B_KF = 13,
+  static constexpr int B_QF = 0, B_QE = 1, B_OD = 2, B_OE = 3, B_OR = 4, B_SF = 5, B_PF = 7, B_XB = 9, B_CH = 13, B_KF = 17,
                        B_KE = B_KF + NST, B_VF = B_KE + NST, B_VE = B_VF + NST, B_VS = B_VE + NST,
                        B_IF = B_VS + NST, B_IE = B_IF + PA_RING, NBARS = B_IE + PA_RING;
   static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15);
   // misc: tmem slot, abort, start (s, g, off), poison [4][4], scan [12], runs, goff
   static constexpr int POISON_OFF = MISC_OFF + 64, SCAN_OFF = POISON_OFF + 64, RUN_OFF = SCAN_OFF + 128,
                        GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run), XCH_OFF = GOFF_OFF + 3 * (PA_GOFF + 4) * 4;
-  static constexpr int SMEM = XCH_OFF + 2 * 2 * 128 * 4 + 1024;
+  static constexpr int SMEM = XCH_OFF + 5 * 128 * 4 + 1024;
   static constexpr int S_COL = 0, O_COL = 2 * KB;
   static constexpr int TCOLS = O_COL + D <= 256 ? 256 : 512;
   static constexpr int CTAS = TCOLS == 256 ? 2 : 1;
@@ -217,10 +218,11 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
 
   if (tid == 0) {
     for (int i = 0; i < C::NBARS; i++) {
-      const int n = i == C::B_OE || i == C::B_PF || i == C::B_PF + 1 ? PA_SOFT
-                    : i >= C::B_XB && i < C::B_XB + 4                ? 2
-                    : i >= C::B_IE                                   ? PA_SOFT + 3
-                                                                     : 1;
+      const int n = i == C::B_OE                              ? PA_SOFT
+                    : i == C::B_PF || i == C::B_PF + 1      ? PA_SOFT / 2
+                    : i >= C::B_XB && i < C::B_XB + 4       ? 2
+                    : i >= C::B_IE                          ? PA_SOFT + 3
+                                                            : 1;
       mbar_init(bar(i), n);
     }
     *abort = 0;
@@ -336,22 +338,51 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
 
   if (!work) {
   } else if (warp == PA_WK) {
-    int n = 0, g = 0, item = -1;  // runs, blocks, tiles
+    int g = 0, item = -1, n = 0;  // blocks, tiles, runs
     bool ok = true, first = true;
-    long pos = p0, off = (long)(uint32_t)s_start[1] | (long)s_start[2] << 32;
-    auto emit = [&](Run &r) -> bool {
-      if (!wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1)) return false;
-      if (r.flags & RUN_FIRST) item++;
+    long pos = p0, off = (long)(uint32_t)s_start[1] | (long)s_start[2] << 32;  // on the line; in the piece
+    int s = s_start[0], kvh = kvh0, ts = -1;                                     // ts: the piece's tile, from the group's first row
+    while (pos < p1 && kvh < a.kv) {
+      Run r;
+      r.s = s, r.qb = a.qoff[s], r.qe = a.qoff[s + 1], r.len = a.lens[s];
+      const int gi = a.G ? gs.of(s) : 0;
+      const Group gr = group_of(a, gs, gi);
+      const int lo = r.qb - gr.tg, hi = r.qe - gr.tg, rows = gr.te - gr.tg;
+      if (ts < 0) ts = lo / a.tpt * a.tpt;
+      if (hi <= lo || ts >= hi) {  // the next sequence
+        ts = -1;
+        if (++s == a.S) s = 0, kvh++;
+        continue;
+      }
+      const int pe = min(hi, ts + a.tpt);
+      const bool starts = ts >= lo, ends = pe == min(rows, ts + a.tpt);
+      const int pc = starts ? gr.pb : 0, lim = own_limit(gr.tg + pe - 1, r.qe, r.len), all = pc + own_cost(lim);
+      if (off >= all) {  // the next piece of the sequence
+        off -= all, ts += a.tpt;
+        continue;
+      }
+      const bool prefix = off < pc;
+      const int units = (int)min((prefix ? pc : all) - off, p1 - pos);
+      const bool done = off + units == all && ends;
+      r.tok0 = gr.tg + ts, r.ntok = min(rows - ts, a.tpt), r.kvh = kvh;
+      r.tab = prefix ? a.ptable + (long)gi * a.pstride : a.table + (long)s * a.tstride;
+      r.seg = prefix ? -1 : s, r.kend = prefix ? gs.plens[gi] : lim;
+      r.kb = (int)(prefix ? off : off - pc), r.nb = r.kend > 0 ? units : 0;
+      r.flags = (first ? RUN_FIRST : 0) | (off == 0 && starts ? RUN_TFIRST : 0) |
+                (done || pos + units == p1 ? RUN_LAST : 0) | (done ? RUN_TLAST : 0);
+      if (first) item++;
       r.item = item;
+      if (!(ok = wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1))) break;
       if (lane == 0) {
         runs[n % PA_RING] = r;
         mbar_arrive(bar(C::B_IF + n % PA_RING));
       }
-      __syncwarp();
       n++;
-      if (r.flags & RUN_END) return true;
-      if (r.flags & RUN_FIRST) {
-        if (!wait_warp(C::B_QE, item + 1)) return false;
+      __syncwarp();
+      Blocks<D> bl;
+      bl.start(a, r, lane);
+      if (first) {
+        if (!(ok = wait_warp(C::B_QE, item + 1))) break;
         if (elect_one()) {
           mbar_expect_tx(bar(C::B_QF), (uint32_t)(a.r * a.tpt * 128 * NA));
           for (int j = 0; j < NA; j++)
@@ -359,65 +390,20 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
         }
         __syncwarp();
       }
-      if (r.nb > 0) {
-        Blocks<D> bl;
-        bl.start(a, r, lane);
-        for (int b = 0; b < r.nb; b++, g++) {
-          const int st = g % NST;
-          const typename Blocks<D>::Rows x = bl.rows(a, r.kb + b, lane);
-          if (!wait_warp(C::B_KE + st, g / NST + 1)) return false;
-          if (elect_one()) bl.load(&tmK, x, sbase + C::K_OFF + st * C::KV_BYTES, bar(C::B_KF + st));
-          __syncwarp();
-        }
+      for (int b = 0; b < r.nb; b++, g++) {
+        const int st = g % NST;
+        const typename Blocks<D>::Rows x = bl.rows(a, r.kb + b, lane);
+        if (!(ok = wait_warp(C::B_KE + st, g / NST + 1))) break;
+        if (elect_one()) bl.load(&tmK, x, sbase + C::K_OFF + st * C::KV_BYTES, bar(C::B_KF + st));
+        __syncwarp();
       }
-      return true;
-    };
-    int s = s_start[0], kvh = kvh0;
-    while (ok && pos < p1 && kvh < a.kv) {
-      const int qb = a.qoff[s], qe = a.qoff[s + 1], len = a.lens[s];
-      if (qe > qb) {
-        const int gi = a.G ? gs.of(s) : 0;
-        const Group gr = group_of(a, gs, gi);
-        const int lo = qb - gr.tg, hi = qe - gr.tg, rows = gr.te - gr.tg;
-        for (int ts = lo / a.tpt * a.tpt; ok && pos < p1 && ts < hi; ts += a.tpt) {
-          const int pe = min(hi, ts + a.tpt);
-          const bool starts = ts >= lo, ends = pe == min(rows, ts + a.tpt);
-          const int pc = starts ? gr.pb : 0;
-          const int lim = own_limit(gr.tg + pe - 1, qe, len), oc = own_cost(lim);
-          if (off >= pc + oc) {
-            off -= pc + oc;
-            continue;
-          }
-          Run r;
-          r.tok0 = gr.tg + ts, r.ntok = min(rows - ts, a.tpt), r.kvh = kvh, r.s = s;
-          r.qb = qb, r.qe = qe, r.len = len;
-          if (off < pc) {
-            const int units = (int)min((long)(pc - off), p1 - pos);
-            r.tab = a.ptable + (long)gi * a.pstride, r.seg = -1, r.kend = gs.plens[gi];
-            r.kb = (int)off, r.nb = units;
-            r.flags = (first ? RUN_FIRST : 0) | (off == 0 ? RUN_TFIRST : 0) | (pos + units == p1 ? RUN_LAST : 0);
-            pos += units, off += units;
-            first = false;
-            ok = emit(r);
-            if (!ok || pos == p1) break;
-          }
-          const int o2 = (int)(off - pc), units = (int)min((long)(oc - o2), p1 - pos);
-          const bool last = ends && o2 + units == oc;
-          r.tab = a.table + (long)s * a.tstride, r.seg = s, r.kend = lim;
-          r.kb = o2, r.nb = lim > 0 ? units : 0;
-          r.flags = (first ? RUN_FIRST : 0) | (starts && off == 0 ? RUN_TFIRST : 0) |
-                    (last || pos + units == p1 ? RUN_LAST : 0) | (last ? RUN_TLAST : 0);
-          pos += units, off = 0;
-          first = (r.flags & RUN_LAST) != 0;
-          ok = emit(r);
-        }
-      }
-      if (++s == a.S) s = 0, kvh++;
+      if (!ok) break;
+      first = (r.flags & RUN_LAST) != 0;
+      pos += units, off += units;
     }
-    if (ok) {
-      Run r = {};
-      r.flags = RUN_END;
-      emit(r);
+    if (ok && wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1) && lane == 0) {
+      runs[n % PA_RING].flags = RUN_END;
+      mbar_arrive(bar(C::B_IF + n % PA_RING));
     }
   } else if (warp == PA_WV) {
     Run r;
@@ -460,9 +446,9 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
         const bool scan = r.seg >= 0 && own_limit(t1, r.qe, r.len) < key0 + valid;
         if (scan) {
           int worst = 64;  // the first row with a value that is not finite
-#pragma unroll
+#pragma unroll 1
           for (int at = 0; at < NA; at++) {
-#pragma unroll
+#pragma unroll 1
             for (int i0 = 0; i0 < 16; i0 += 8) {
               uint4 x[8];
 #pragma unroll
@@ -498,96 +484,115 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
   } else if (warp == PA_WM) {
     constexpr uint32_t idesc_qk = idesc_f16_f32(128, KB);
     constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // V MN-major
-    const uint64_t q0 = desc_sw128(sbase), k0 = desc_sw128(sbase + C::K_OFF), v0 = desc_mn(sbase + C::V_OFF, KB * 128);
-    Run r = {};
-    int g = 0;
-    bool ok = true, pend = false, fresh = true;  // fresh: the tile has had no block yet
-    int steps = 0;               // of the pending product: 16 keys each,
-    uint32_t off[4] = {};        // and the rows that it leaves alone
-    auto pv = [&](int x) -> bool {
-      const int st = x % NST;
-      if (!wait_warp(C::B_PF + (x & 1), x >> 1) || !wait_warp(C::B_VF + st, x / NST) || !wait_warp(C::B_VS + st, x / NST))
-        return false;
-      tc_fence_after();
-      const uint32_t p = tmem + (uint32_t)(C::S_COL + (x & 1) * KB);
-      const uint64_t v = v0 + (uint32_t)(st * C::KV_BYTES >> 4);
-      if (elect_one()) {
+    // One thread. Q K^T of block g + 1 needs the scores' buffer that P V of block g - 1 frees, so the two are issued
+    // together, as soon as the weights of g - 1 are there; everything else that they need is waited for before.
+    if (elect_one()) {
+      const uint64_t q0 = desc_sw128(sbase), k0 = desc_sw128(sbase + C::K_OFF), v0 = desc_mn(sbase + C::V_OFF, KB * 128);
+      auto wait1 = [&](int i, int parity) {
+        return mbar_wait_alert(bar(i), (uint32_t)parity & 1u, abort, a.err, DC_DEVERR_ATTN_WAIT);
+      };
+      int g = 0, item = 0;
+      bool ok = true, pend = false, begins = true;  // begins: the tile has had no product yet
+      int steps = 0;                                // of the pending product (block g - 1): 16 keys each,
+      uint32_t off[4] = {};                         // and the rows that it leaves alone
+      auto qk = [&](int x) {
+        const int st = x % NST;
+        const uint32_t sc = tmem + (uint32_t)(C::S_COL + (x & 1) * KB);
+        const uint64_t k = k0 + (uint32_t)(st * C::KV_BYTES >> 4);
+        tc_fence_after();
+#pragma unroll
+        for (int kd = 0; kd < D / 16; kd++)
+          mma_f16(sc, q0 + (((kd >> 2) * 128 * 128 + (kd & 3) * 32) >> 4), k + (((kd >> 2) * KB * 128 + (kd & 3) * 32) >> 4),
+                  idesc_qk, kd > 0);
+        mma_commit(bar(C::B_SF + (x & 1)));
+        mma_commit(bar(C::B_KE + st));
+      };
+      auto pv = [&](int x) -> bool {
+        const int st = x % NST;
+        if (!wait1(C::B_VF + st, x / NST) || !wait1(C::B_VS + st, x / NST)) return false;
+        if (begins && !wait1(C::B_OE, item)) return false;  // the accumulator is zero
+        begins = false;
+        if (!wait1(C::B_PF + (x & 1), x >> 1)) return false;
+        tc_fence_after();
+        const uint32_t p = tmem + (uint32_t)(C::S_COL + (x & 1) * KB);
+        const uint64_t v = v0 + (uint32_t)(st * C::KV_BYTES >> 4);
 #pragma unroll
         for (int kk = 0; kk < KB / 16; kk++)
           if (kk < steps) mma_f16_ts_rows(tmem + C::O_COL, p + 8 * kk, v + kk * (2048 >> 4), idesc_pv, off);
         mma_commit(bar(C::B_VE + st));
         mma_commit(bar(C::B_OR));
-      }
-      __syncwarp();
-      return true;
-    };
-    for (int n = 0; ok && next_run(n, r); n++) {
-      if (r.flags & RUN_FIRST) ok = wait_warp(C::B_QF, r.item), fresh = true;
-      for (int b = 0; ok && b < r.nb; b++, g++) {
-        const int st = g % NST;
-        if (!(ok = wait_warp(C::B_KF + st, g / NST))) break;
-        tc_fence_after();
-        const uint32_t sc = tmem + (uint32_t)(C::S_COL + (g & 1) * KB);
-        const uint64_t k = k0 + (uint32_t)(st * C::KV_BYTES >> 4);
-        if (elect_one()) {
+        return true;
+      };
+      for (int n = 0; ok && wait1(C::B_IF + n % PA_RING, n / PA_RING); n++) {
+        const Run r = runs[n % PA_RING];
+        if (r.flags & RUN_END) break;
+        if (r.flags & RUN_FIRST) item = r.item, begins = true, ok = wait1(C::B_QF, item);
+#pragma unroll 1
+        for (int b = 0; ok && b < r.nb; b++, g++) {
+          if (b == 0) {
+            if (!(ok = wait1(C::B_KF + g % NST, g / NST))) break;
+            qk(g);
+          }
+          const bool next = b + 1 < r.nb;
+          if (next && !(ok = wait1(C::B_KF + (g + 1) % NST, (g + 1) / NST))) break;
+          if (pend && !(ok = pv(g - 1))) break;
+          if (next) qk(g + 1);
+          pend = true;
+          const int key0 = (r.kb + b) * 64;
+          steps = (min(64, r.kend - key0) + 15) >> 4;
+          // own blocks: the rows of the sequence that see a key of it
+          const int lo = r.seg < 0 ? 0 : (max(max(r.tok0, r.qb), key0 - r.len + r.qe) - r.tok0) * a.r;
+          const int hi = r.seg < 0 ? 128 : (min(r.qe, r.tok0 + r.ntok) - r.tok0) * a.r;
 #pragma unroll
-          for (int kd = 0; kd < D / 16; kd++)
-            mma_f16(sc, q0 + (((kd >> 2) * 128 * 128 + (kd & 3) * 32) >> 4), k + (((kd >> 2) * KB * 128 + (kd & 3) * 32) >> 4),
-                    idesc_qk, kd > 0);
-          mma_commit(bar(C::B_SF + (g & 1)));
-          mma_commit(bar(C::B_KE + st));
+          for (int w = 0; w < 4; w++) {
+            const int x = min(max(lo - 32 * w, 0), 32), y = min(max(hi - 32 * w, 0), 32);
+            const uint32_t upto = y >= 32 ? ~0u : (1u << y) - 1u, under = x >= 32 ? ~0u : (1u << x) - 1u;
+            off[w] = ~(upto & ~under);
+          }
         }
-        __syncwarp();
-        if (pend && !(ok = pv(g - 1))) break;
-        pend = true, fresh = false;
-        const int key0 = (r.kb + b) * 64;
-        steps = (min(64, r.kend - key0) + 15) >> 4;
-        // own blocks: the rows of the sequence that see a key of it
-        const int lo = r.seg < 0 ? 0 : (max(max(r.tok0, r.qb), key0 - r.len + r.qe) - r.tok0) * a.r;
-        const int hi = r.seg < 0 ? 128 : (min(r.qe, r.tok0 + r.ntok) - r.tok0) * a.r;
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-          const int x = min(max(lo - 32 * w, 0), 32), y = min(max(hi - 32 * w, 0), 32);
-          const uint32_t upto = y >= 32 ? ~0u : (1u << y) - 1u, under = x >= 32 ? ~0u : (1u << x) - 1u;
-          off[w] = ~(upto & ~under);
+        if (ok && (r.flags & RUN_LAST)) {
+          mma_commit(bar(C::B_QE));
+          if (pend) ok = pv(g - 1);
+          pend = false;
+          // a tile without keys: the last tile's end has to be past before this one's is announced
+          if (ok && begins) ok = wait1(C::B_OE, item);
+          if (ok) mma_commit(bar(C::B_OD));
         }
+        if (ok) mbar_arrive(bar(C::B_IE + n % PA_RING));
       }
-      if (ok && (r.flags & RUN_LAST)) {
-        if (elect_one()) mma_commit(bar(C::B_QE));
-        __syncwarp();
-        if (pend) ok = pv(g - 1);
-        pend = false;
-        // a tile without keys: the last tile's end has to be past before this one's is announced
-        if (ok && fresh) ok = wait_warp(C::B_OE, r.item + 1);
-        if (ok && elect_one()) mma_commit(bar(C::B_OD));
-        __syncwarp();
-      }
-      if (ok) done_run(n);
     }
+    __syncwarp();
   } else {
-    const int q = warp & 3, hf = warp >> 2;
+    const int q = warp & 3, wg = warp >> 2;
     const int row = 32 * q + lane, irow = row / a.r, jrow = row - irow * a.r;
-    const uint32_t lrow = (uint32_t)(32 * q) << 16;
-    float *xch = reinterpret_cast<float *>(smem + C::XCH_OFF);
+    const uint32_t lrow = tmem + ((uint32_t)(32 * q) << 16), ocol = lrow + (uint32_t)(C::O_COL + wg * (D / 2));
+    const uint32_t scol = lrow + (uint32_t)(C::S_COL + wg * KB);
+    float *s_ref = reinterpret_cast<float *>(smem + C::XCH_OFF), *s_sum = s_ref + 128;  // [128], [2 turns][2][128]
     Run r;
-    int g = 0, meets = 0;
+    int g = 0, chain = 0, meets = 0;
     bool ok = true;
     // the tile's state
     bool valid = false, anyv = false, had = false, tfirst = false;
     int t = 0, seq = -1, lim = 0;
-    float m_ref = -FLT_MAX, l = 0.f;
-    auto meet = [&]() -> bool {  // both warps of the quadrant have written their halves
+    float ref = -FLT_MAX, l = 0.f;  // l: the sum of this thread's weights, in units of 2^(ref - 7)
+    auto zero = [&]() {             // this warp's half of its rows' accumulators
+      const uint32_t z[16] = {};
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(C::B_XB + q));
-      return wait_warp(C::B_XB + q, meets++);
+#pragma unroll
+      for (int c = 0; c < D / 2; c += 16) tmem_st16(ocol + c, z);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::B_OE));
     };
+    zero();
     for (int n = 0; ok && next_run(n, r); n++) {
       if (r.flags & RUN_FIRST) {
         t = r.tok0 + irow;
         valid = irow < r.ntok && irow < a.tpt;
         anyv = __any_sync(0xffffffffu, valid);
         had = false, tfirst = (r.flags & RUN_TFIRST) != 0;
-        m_ref = -FLT_MAX, l = 0.f;
+        ref = -FLT_MAX, l = 0.f;
         seq = -1, lim = 0;
         if (valid && t >= r.qb) {  // its sequence: the last at or after the run's whose rows begin at or before it
           int x = r.s, y = a.S;
@@ -598,116 +603,140 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
           }
           seq = x, lim = own_limit(t, a.qoff[x + 1], a.lens[x]);
         }
-        if (anyv) {  // the last tile's accumulator was read by this very warp
-          const uint32_t z[16] = {};
-          __syncwarp();
-#pragma unroll
-          for (int c = 0; c < D / 2; c += 16) tmem_st16(tmem + lrow + (uint32_t)(C::O_COL + hf * (D / 2) + c), z);
-          tmem_st_wait();
-          tc_fence_before();
-        }
       }
       const int rlim = !valid ? 0 : r.seg < 0 ? r.kend : seq == r.seg ? lim : 0;
       for (int b = 0; b < r.nb; b++, g++) {
-        const int sbuf = g & 1;
-        if (!(ok = wait_warp(C::B_SF + sbuf, g >> 1))) break;
+        const bool opens = !had;  // the tile's first block
         had = true;
+        if (anyv) chain++;
+        if ((g & 1) != wg) continue;
+        if (!(ok = wait_warp(C::B_SF + wg, g >> 1))) break;
         const int nv = min(max(rlim - (r.kb + b) * 64, 0), 64);
-        const uint32_t scol = tmem + lrow + (uint32_t)(C::S_COL + sbuf * KB);
-        if (__any_sync(0xffffffffu, nv > 0)) {
+        // (lanes without a row do not force the masks on the others)
+        const bool sees = __any_sync(0xffffffffu, nv > 0), part = !__all_sync(0xffffffffu, nv == 64 || !valid);
+        float sc = a.scale_log2, pmx = -FLT_MAX;
+        if (sees) {
           tc_fence_after();
-          uint32_t x[32];
-          __syncwarp();
-          tmem_ld32(scol + 32 * hf, x);
-          tmem_ld_wait(x);
-          const int nh = min(max(nv - 32 * hf, 0), 32);
-          float sc = a.scale_log2;
           if (sc <= 0.f) {  // the largest score is not the largest product: scale first
+#pragma unroll 1
+            for (int c = 0; c < KB; c += 16) {
+              uint32_t x[16];
+              __syncwarp();
+              tmem_ld16(scol + c, x);
+              tmem_ld_wait(x);
 #pragma unroll
-            for (int e = 0; e < 32; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * sc);
+              for (int e = 0; e < 16; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * sc);
+              __syncwarp();
+              tmem_st16(scol + c, x);
+            }
+            tmem_st_wait();
             sc = 1.f;
           }
-          if (!__all_sync(0xffffffffu, nh == 32)) {  // keys not seen: weight 2^-inf
-            const uint32_t vis = nh >= 32 ? ~0u : (1u << nh) - 1u;
+          float m2[2] = {__uint_as_float(0xff800000u), __uint_as_float(0xff800000u)};
+#pragma unroll 1
+          for (int c = 0; c < KB; c += 32) {
+            uint32_t x[32];
+            __syncwarp();
+            tmem_ld32(scol + c, x);
+            tmem_ld_wait(x);
+            if (part)
 #pragma unroll
-            for (int e = 0; e < 32; e++) x[e] = ((vis >> e) & 1u) ? x[e] : 0xff800000u;
-          }
-          float m2[2] = {__uint_as_float(x[0]), __uint_as_float(x[1])};
+              for (int e = 0; e < 32; e++) x[e] = c + e < nv ? x[e] : 0xff800000u;
 #pragma unroll
-          for (int e = 2; e < 32; e += 4) {
-            m2[0] = max3(m2[0], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-            if (e + 2 < 32) m2[1] = max3(m2[1], __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+            for (int e = 0; e < 32; e += 4) {
+              m2[0] = max3(m2[0], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+              m2[1] = max3(m2[1], __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+            }
           }
-          const float pmx = fmaxf(m2[0], m2[1]) * sc;
-          const int par = meets & 1;
-          xch[(par * 2 + hf) * 128 + row] = pmx;
-          if (!(ok = meet())) break;
-          const float mx = fmaxf(pmx, xch[(par * 2 + (hf ^ 1)) * 128 + row]);
-          const bool grow = mx > m_ref + 8.0f;
-          const bool resc = grow && m_ref > -FLT_MAX;
+          pmx = fmaxf(m2[0], m2[1]) * sc;
+        }
+        if (anyv) {
+          // the row's reference goes from block to block through shared memory, with the turn to move it
+          if (!(ok = wait_warp(C::B_CH + q, chain))) break;
+          const float cur = opens ? -FLT_MAX : s_ref[row];
+          const bool grow = pmx > cur + 8.0f;
+          const float now = grow ? pmx : cur;
+          const bool resc = grow && cur > -FLT_MAX;
           if (__any_sync(0xffffffffu, resc)) {
             if (!(ok = wait_warp(C::B_OR, g - 1))) break;  // the products so far
             tc_fence_after();
-            const float f = resc ? ex2_approx(m_ref - mx) : 1.0f;
-            l *= f;
-            const uint32_t ocol = tmem + lrow + (uint32_t)(C::O_COL + hf * (D / 2));
+            const float f = resc ? ex2_approx(cur - now) : 1.0f;
 #pragma unroll 1
-            for (int c = 0; c < D / 2; c += 16) {
+            for (int c = 0; c < D; c += 16) {
               uint32_t o[16];
               __syncwarp();
-              tmem_ld16(ocol + c, o);
+              tmem_ld16(lrow + (uint32_t)(C::O_COL + c), o);
               tmem_ld_wait(o);
 #pragma unroll
               for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
               __syncwarp();
-              tmem_st16(ocol + c, o);
+              tmem_st16(lrow + (uint32_t)(C::O_COL + c), o);
             }
             tmem_st_wait();
           }
-          if (grow) m_ref = mx;
-          const uint64_t ref2 = f32x2(7.0f - m_ref, 7.0f - m_ref), sc2 = f32x2(sc, sc);
+          if (grow || opens) s_ref[row] = now;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::B_CH + q));
+          if (__any_sync(0xffffffffu, now != ref)) {
+            l *= ex2_approx(ref - now);  // 0 * 0 where there was none
+            ref = now;
+          }
+        }
+        if (sees) {
+          const uint64_t ref2 = f32x2(7.0f - ref, 7.0f - ref), sc2 = f32x2(sc, sc);
           uint64_t sum[2] = {0, 0};
+#pragma unroll 1
+          for (int c = 0; c < KB; c += 32) {  // 32 weights go where 16 of the scores were that are done with
+            uint32_t x[32];
+            __syncwarp();
+            tmem_ld32(scol + c, x);
+            tmem_ld_wait(x);
+            if (part)
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 v = f32x2_split(fma_f32x2(f32x2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, ref2));
-            const float p0 = ex2_approx(v.x), p1 = ex2_approx(v.y);
-            sum[(e >> 1) & 1] = add_f32x2(sum[(e >> 1) & 1], f32x2(p0, p1));
-            const __half2 hp = __floats2half2_rn(p0, p1);
-            x[e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
+              for (int e = 0; e < 32; e++) x[e] = c + e < nv ? x[e] : 0xff800000u;
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 v = f32x2_split(fma_f32x2(f32x2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, ref2));
+              const float p0 = ex2_approx(v.x), p1 = ex2_approx(v.y);
+              sum[(e >> 1) & 1] = add_f32x2(sum[(e >> 1) & 1], f32x2(p0, p1));
+              const __half2 hp = __floats2half2_rn(p0, p1);
+              x[e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
+            }
+            __syncwarp();
+            tmem_st16(scol + c / 2, *reinterpret_cast<const uint32_t (*)[16]>(&x[0]));
           }
           const float2 add = f32x2_split(add_f32x2(sum[0], sum[1]));
           l += add.x + add.y;
-          __syncwarp();
-          tmem_st16(scol + 16 * hf, *reinterpret_cast<const uint32_t (*)[16]>(&x[0]));
           tmem_st_wait();
         }  // none of these rows sees the block: the product leaves them alone
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::B_PF + sbuf));
+        if (lane == 0) mbar_arrive(bar(C::B_PF + wg));
       }
       if (!ok) break;
       if (r.flags & RUN_LAST) {
         if (!(ok = wait_warp(C::B_OD, r.item))) break;
         tc_fence_after();
-        const bool tlast = (r.flags & RUN_TLAST) != 0, direct = tfirst && tlast;
         if (anyv) {
-          const int par = meets & 1;
-          xch[(par * 2 + hf) * 128 + row] = l;
-          if (!(ok = meet())) break;
-          float lt = l + xch[(par * 2 + (hf ^ 1)) * 128 + row];
-          if (had && valid && ((poison[4 * (r.item & 3) + (irow >> 5)] >> (irow & 31)) & 1u))
-            lt = __int_as_float(0x7fc00000);
-          const int h = r.kvh * a.r + jrow;
+          const bool tlast = (r.flags & RUN_TLAST) != 0, direct = tfirst && tlast;
+          // the two warps of the quadrant add their sums at the row's last reference
+          const float fin = had ? s_ref[row] : -FLT_MAX;
+          float *sums = s_sum + (meets & 1) * 256;
+          sums[wg * 128 + row] = l * ex2_approx(ref - fin);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::B_XB + q));
+          if (!(ok = wait_warp(C::B_XB + q, meets++))) break;
+          float lt = sums[row] + sums[128 + row];
+          if (had && valid && ((poison[4 * (r.item & 3) + (irow >> 5)] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
           const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
-          if (valid && jrow == 0 && hf == 0) {
+          if (valid && jrow == 0 && wg == 0) {
             if (tfirst) a.recF[(long)r.kvh * a.T + t] = direct ? -1 : (int)blockIdx.x;
             if (tlast) a.recL[(long)r.kvh * a.T + t] = (int)blockIdx.x;
           }
-          if (!direct && valid && hf == 0) a.ml[prow] = make_float2(m_ref, lt);
+          if (!direct && valid && wg == 0) a.ml[prow] = make_float2(fin, lt);
           const float inv = lt == 0.f ? 0.f : 1.0f / lt;
-          const uint32_t ocol = tmem + lrow + (uint32_t)(C::O_COL + hf * (D / 2));
-          __half *y = a.Y + (long)t * a.ystride + (long)h * D + hf * (D / 2);
-          float *po = a.O + prow * D + hf * (D / 2);
+          __half *y = a.Y + (long)t * a.ystride + (long)(r.kvh * a.r + jrow) * D + wg * (D / 2);
+          float *po = a.O + prow * D + wg * (D / 2);
 #pragma unroll 1
           for (int c = 0; c < D / 2; c += 16) {
             uint32_t o[16];
@@ -720,7 +749,7 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
 #pragma unroll
               for (int e = 0; e < 8; e++) {
                 const __half2 hv = __floats2half2_rn(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-                w[e] = lt == 0.f ? 0u : *reinterpret_cast<const uint32_t *>(&hv);
+                w[e] = *reinterpret_cast<const uint32_t *>(&hv);
               }
               *reinterpret_cast<uint4 *>(y + c) = make_uint4(w[0], w[1], w[2], w[3]);
               *reinterpret_cast<uint4 *>(y + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
@@ -728,11 +757,8 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
               st_global_v8(po + c, o), st_global_v8(po + c + 8, o + 8);
             }
           }
-          __syncwarp();
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::B_OE));
+        zero();
       }
       done_run(n);
     }
