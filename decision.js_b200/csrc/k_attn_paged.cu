@@ -19,10 +19,10 @@
 //              weights are relative to) goes from block to block through shared memory, each warp waiting for its
 //              twin's turn only between its own maximum and its weights; the exp2 weights are scaled by 2^7 (the row reference moves when the maximum
 //              grows past 2^8, so they stay under 2^15) to keep small ones out of f16's subnormals
-//   warp 8     walks the line, hands runs of blocks to the others through a ring of descriptors, loads Q and K
-//   warp 9     loads V
-//   warp 10    the MMAs (and TMEM)
-//   warp 11    looks over V blocks that some row of the tile does not see: rows past the last key are zeroed, and
+//   warp 16    walks the line, hands runs of blocks to the others through a ring of descriptors, loads Q and K
+//   warp 13    loads V
+//   warp 14    Q K^T (and TMEM), warp 15 P V: two threads, as one would be busy issuing for longer than the products take
+//   warp 12    looks over V blocks that some row of the tile does not see: rows past the last key are zeroed, and
 //              values that are not finite too (a weight of 0 times them would be NaN in every row), with a mark on
 //              the rows that see them
 // All roles run ahead across tiles: only Q (single buffer) and the accumulator wait for a tile's end.
@@ -40,9 +40,9 @@ using namespace dcx;
 
 namespace {
 
-constexpr int PA_SOFT = 8;
-constexpr int PA_WK = 8, PA_WV = 9, PA_WM = 10, PA_WC = 11;
-constexpr int PA_THREADS = 12 * 32;
+constexpr int PA_WG = 3, PA_SOFT = 4 * PA_WG;  // softmax warpgroups, warps
+constexpr int PA_WC = PA_SOFT, PA_WV = PA_SOFT + 1, PA_WM = PA_SOFT + 2, PA_WP = PA_SOFT + 3, PA_WK = PA_SOFT + 4;
+constexpr int PA_THREADS = (PA_SOFT + 5) * 32;
 constexpr int PA_RING = 4;
 constexpr int PA_GOFF = 512;  // groups whose offsets are kept in shared memory
 
@@ -61,23 +61,26 @@ struct Run {
 
 template <int D>
 struct PCfg {
-  static constexpr int KB = 64, NA = D / 64;
-  static constexpr int NST = D == 64 ? 4 : 2;  // stages of the K and of the V ring
+  // keys per block; 64 at D = 256, whose tiles and accumulator leave room for no more
+  static constexpr int KB = D == 256 ? 64 : 128, NA = D / 64;
+  static constexpr int KST = D == 64 ? 4 : D == 128 ? 3 : 2, VST = D == 64 ? 4 : 2;  // stages of the K and of the V ring
   static constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = KB * D * 2;
-  static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + NST * KV_BYTES;
-  static constexpr int BAR_OFF = V_OFF + NST * KV_BYTES;
-  static constexpr int B_QF = 0, B_QE = 1, B_OD = 2, B_OE = 3, B_OR = 4, B_SF = 5, B_PF = 7, B_XB = 9, B_CH = 13, B_KF = 17,
-                       B_KE = B_KF + NST, B_VF = B_KE + NST, B_VE = B_VF + NST, B_VS = B_VE + NST,
-                       B_IF = B_VS + NST, B_IE = B_IF + PA_RING, NBARS = B_IE + PA_RING;
+  static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + KST * KV_BYTES;
+  static constexpr int BAR_OFF = V_OFF + VST * KV_BYTES;
+  static constexpr int B_QF = 0, B_QE = 1, B_OD = 2, B_OE = 3, B_XB = 4, B_SF = 8, B_PF = B_SF + PA_WG,
+                       B_SE = B_PF + PA_WG, B_CH = B_SE + PA_WG, B_KF = B_CH + 4 * PA_WG, B_KE = B_KF + KST, B_VF = B_KE + KST,
+                       B_VE = B_VF + VST, B_VS = B_VE + VST, B_IF = B_VS + VST, B_IE = B_IF + PA_RING,
+                       NBARS = B_IE + PA_RING;
   static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15);
-  // misc: tmem slot, abort, start (s, g, off), poison [4][4], scan [12], runs, goff
-  static constexpr int POISON_OFF = MISC_OFF + 64, SCAN_OFF = POISON_OFF + 64, RUN_OFF = SCAN_OFF + 128,
-                       GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run), XCH_OFF = GOFF_OFF + 3 * (PA_GOFF + 4) * 4;
-  static constexpr int SMEM = XCH_OFF + 5 * 128 * 4 + 1024;
-  static constexpr int S_COL = 0, O_COL = 2 * KB;
-  static constexpr int TCOLS = O_COL + D <= 256 ? 256 : 512;
-  static constexpr int CTAS = TCOLS == 256 ? 2 : 1;
-  static_assert(SMEM * CTAS <= 227 * 1024, "shared memory");
+  // misc: tmem slot, abort, start (s, offset); poison; scan; runs; groups; references and sums
+  static constexpr int POISON_OFF = MISC_OFF + 32, SCAN_OFF = POISON_OFF + 64,
+                       RUN_OFF = SCAN_OFF + ((PA_THREADS / 32 * 8 + 15) & ~15), GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run),
+                       XCH_OFF = GOFF_OFF + 3 * (PA_GOFF + 4) * 4;
+  static constexpr int SMEM = XCH_OFF + (1 + 2 * PA_WG) * 128 * 4 + 1024;
+  static constexpr int S_COL = 0, O_COL = PA_WG * KB;  // tensor memory: a scores' buffer per warpgroup, the accumulator
+  static constexpr int TCOLS = 512;
+  static_assert(O_COL + D <= TCOLS, "tensor memory");
+  static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 struct PArgs {
@@ -106,7 +109,8 @@ __device__ __forceinline__ void st_global_v8(float *p, const uint32_t *r) {
 
 // own keys that query row `t` of a sequence [.., qe) with `len` own tokens sees
 __device__ __forceinline__ int own_limit(int t, int qe, int len) { return max(len - (qe - 1 - t), 0); }
-__device__ __forceinline__ int own_cost(int lim) { return max(1, (lim + 63) >> 6); }
+template <int KB>
+__device__ __forceinline__ int blocks_of(int keys) { return (keys + KB - 1) / KB; }
 
 struct Groups {  // offsets, prefix lengths and first rows, from shared memory when they fit
   const int *goff, *plens, *rows;
@@ -125,21 +129,23 @@ struct Groups {  // offsets, prefix lengths and first rows, from shared memory w
 struct Group {
   int tg, te, pb;  // its rows, its prefix's blocks
 };
+template <int KB>
 __device__ __forceinline__ Group group_of(const PArgs &a, const Groups &gs, int g) {
   if (gs.G == 0) return Group{gs.whole.x, gs.whole.y, 0};
-  const int pb = (gs.plens[g] + 63) >> 6;
+  const int pb = blocks_of<KB>(gs.plens[g]);
   if (gs.rows) return Group{gs.rows[g], gs.rows[g + 1], pb};
   return Group{a.qoff[min(max(gs.goff[g], 0), a.S)], a.qoff[min(max(gs.goff[g + 1], 0), a.S)], pb};
 }
 
 // The units of a sequence: for each tile its rows touch, the prefix's blocks if the tile starts in it, and its own.
-__device__ __forceinline__ long seq_cost(const PArgs &a, const Group &g, int qb, int qe, int len) {
+template <int KB>
+__device__ __noinline__ long seq_cost(int tpt, Group g, int qb, int qe, int len) {
   long c = 0;
   const int lo = qb - g.tg, hi = qe - g.tg;
   if (hi <= lo) return 0;
-  for (int ts = lo / a.tpt * a.tpt; ts < hi; ts += a.tpt) {
+  for (int ts = lo / tpt * tpt; ts < hi; ts += tpt) {
     if (ts >= lo) c += g.pb;
-    c += own_cost(own_limit(g.tg + min(hi, ts + a.tpt) - 1, qe, len));
+    c += max(1, blocks_of<KB>(own_limit(g.tg + min(hi, ts + tpt) - 1, qe, len)));
   }
   return c;
 }
@@ -148,7 +154,7 @@ __device__ __forceinline__ long seq_cost(const PArgs &a, const Group &g, int qb,
 // the cache as tensor-map coordinates before the stage is waited for.
 template <int D>
 struct Blocks {
-  static constexpr int NA = D / 64;
+  static constexpr int NA = D / 64, KB = PCfg<D>::KB, NB = KB / 16;
   const int *tab;
   int base, count, cur, nxt, kend, kvh;
   __device__ __forceinline__ int ld(const PArgs &a, int i) const {
@@ -163,25 +169,25 @@ struct Blocks {
     return row;
   }
   __device__ __forceinline__ void start(const PArgs &a, const Run &r, int lane) {
-    tab = r.tab, kend = r.kend, kvh = r.kvh, count = (kend + a.page - 1) >> a.pshift, base = (r.kb * 64) >> a.pshift;
+    tab = r.tab, kend = r.kend, kvh = r.kvh, count = (kend + a.page - 1) >> a.pshift, base = (r.kb * KB) >> a.pshift;
     cur = ld(a, base + lane), nxt = ld(a, base + 32 + lane);
   }
-  // The whole warp: block `kb`'s rows, one per box of min(page, 64) rows (pages that hold none of the run's keys are
+  // The whole warp: block `kb`'s rows, one per box of min(page, 64) rows (boxes that hold none of the run's keys are
   // left out).
   struct Rows {
-    int row[4], n, prow;
+    int row[NB], n, prow;
   };
   __device__ __forceinline__ Rows rows(const PArgs &a, int kb, int lane) {
     Rows x;
-    x.prow = min(a.page, 64);
-    const int key0 = kb * 64, i = key0 >> a.pshift;
+    const int pr = min(a.pshift, 6), key0 = kb * KB, i = key0 >> a.pshift, sub = a.pshift - pr;
+    x.prow = 1 << pr;
     if (i - base >= 32) base += 32, cur = nxt, nxt = ld(a, base + 32 + lane);
-    x.n = a.page >= 64 ? 1 : min(64 >> a.pshift, (kend - key0 + a.page - 1) >> a.pshift);
-    const int in = key0 & (a.page - 1);  // the second half of a page of 128
+    x.n = min(KB >> pr, (kend - key0 + x.prow - 1) >> pr);
+    const int first = (key0 & (a.page - 1)) >> pr;  // the first box within its page
 #pragma unroll
-    for (int p = 0; p < 4; p++) {
-      const int v = __shfl_sync(0xffffffffu, cur, (i - base + p) & 31);
-      x.row[p] = v == a.rows ? v : v + in;
+    for (int p = 0; p < NB; p++) {
+      const int at = first + p, v = __shfl_sync(0xffffffffu, cur, (i - base + (at >> sub)) & 31);
+      x.row[p] = v == a.rows ? v : v + ((at & ((1 << sub) - 1)) << pr);
     }
     return x;
   }
@@ -189,20 +195,20 @@ struct Blocks {
   __device__ __forceinline__ static void load(const CUtensorMap *map, const Rows &x, uint32_t dst, uint32_t full) {
     mbar_expect_tx(full, (uint32_t)(x.n * NA * x.prow * 128));
 #pragma unroll
-    for (int p = 0; p < 4; p++) {
+    for (int p = 0; p < NB; p++) {
       if (p >= x.n) break;
 #pragma unroll
-      for (int j = 0; j < NA; j++) tma_load_2d(dst + j * (64 * 128) + p * x.prow * 128, map, 64 * j, x.row[p], full);
+      for (int j = 0; j < NA; j++) tma_load_2d(dst + j * (KB * 128) + p * x.prow * 128, map, 64 * j, x.row[p], full);
     }
   }
 };
 
 template <int D>
-__global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
+__global__ void __launch_bounds__(PA_THREADS, 1)
     attention_paged_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                            const __grid_constant__ CUtensorMap tmV, const PArgs a) {
   using C = PCfg<D>;
-  constexpr int KB = C::KB, NST = C::NST, NA = C::NA;
+  constexpr int KB = C::KB, KST = C::KST, VST = C::VST, NA = C::NA;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
@@ -219,9 +225,9 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
   if (tid == 0) {
     for (int i = 0; i < C::NBARS; i++) {
       const int n = i == C::B_OE                              ? PA_SOFT
-                    : i == C::B_PF || i == C::B_PF + 1      ? PA_SOFT / 2
-                    : i >= C::B_XB && i < C::B_XB + 4       ? 2
-                    : i >= C::B_IE                          ? PA_SOFT + 3
+                    : i >= C::B_PF && i < C::B_PF + PA_WG   ? 4
+                    : i >= C::B_XB && i < C::B_XB + 4       ? PA_WG
+                    : i >= C::B_IE                          ? PA_SOFT + 4
                                                             : 1;
       mbar_init(bar(i), n);
     }
@@ -267,8 +273,8 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
   // a sequence's units; nothing for offsets that are refused below (the sum is then not used)
   auto units = [&](int s, int qb, int qe, int len) -> long {
     if (qb < 0 || qe <= qb || qe > a.T || len < 0) return 0;
-    const Group g = group_of(a, gs, a.G ? gs.of(s) : 0);
-    return g.tg < 0 || g.tg > qb ? 0 : seq_cost(a, g, qb, qe, len);
+    const Group g = group_of<KB>(a, gs, a.G ? gs.of(s) : 0);
+    return g.tg < 0 || g.tg > qb ? 0 : seq_cost<KB>(a.tpt, g, qb, qe, len);
   };
   long mine = 0;
   for (int s = sb; s < se; s++) {
@@ -325,6 +331,9 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
   };
   // the whole warp waits, and goes on or gives up together
   auto wait_warp = [&](int i, int parity) { return __all_sync(0xffffffffu, wait(i, parity)) != 0; };
+  auto wait1 = [&](int i, int parity) {  // one thread that issues products
+    return mbar_wait_alert(bar(i), (uint32_t)parity & 1u, abort, a.err, DC_DEVERR_ATTN_WAIT);
+  };
   // a consumer's next run: false at the end (or on abort)
   auto next_run = [&](int n, Run &r) -> bool {
     if (!wait_warp(C::B_IF + n % PA_RING, n / PA_RING)) return false;
@@ -346,7 +355,7 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
       Run r;
       r.s = s, r.qb = a.qoff[s], r.qe = a.qoff[s + 1], r.len = a.lens[s];
       const int gi = a.G ? gs.of(s) : 0;
-      const Group gr = group_of(a, gs, gi);
+      const Group gr = group_of<KB>(a, gs, gi);
       const int lo = r.qb - gr.tg, hi = r.qe - gr.tg, rows = gr.te - gr.tg;
       if (ts < 0) ts = lo / a.tpt * a.tpt;
       if (hi <= lo || ts >= hi) {  // the next sequence
@@ -356,7 +365,7 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
       }
       const int pe = min(hi, ts + a.tpt);
       const bool starts = ts >= lo, ends = pe == min(rows, ts + a.tpt);
-      const int pc = starts ? gr.pb : 0, lim = own_limit(gr.tg + pe - 1, r.qe, r.len), all = pc + own_cost(lim);
+      const int pc = starts ? gr.pb : 0, lim = own_limit(gr.tg + pe - 1, r.qe, r.len), all = pc + max(1, blocks_of<KB>(lim));
       if (off >= all) {  // the next piece of the sequence
         off -= all, ts += a.tpt;
         continue;
@@ -370,6 +379,8 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
       r.kb = (int)(prefix ? off : off - pc), r.nb = r.kend > 0 ? units : 0;
       r.flags = (first ? RUN_FIRST : 0) | (off == 0 && starts ? RUN_TFIRST : 0) |
                 (done || pos + units == p1 ? RUN_LAST : 0) | (done ? RUN_TLAST : 0);
+      pos += units, off += units;
+      if (r.nb == 0 && !(r.flags & (RUN_FIRST | RUN_LAST))) continue;  // (a run in a tile's midst always has blocks)
       if (first) item++;
       r.item = item;
       if (!(ok = wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1))) break;
@@ -391,15 +402,14 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
         __syncwarp();
       }
       for (int b = 0; b < r.nb; b++, g++) {
-        const int st = g % NST;
+        const int st = g % KST;
         const typename Blocks<D>::Rows x = bl.rows(a, r.kb + b, lane);
-        if (!(ok = wait_warp(C::B_KE + st, g / NST + 1))) break;
+        if (!(ok = wait_warp(C::B_KE + st, g / KST + 1))) break;
         if (elect_one()) bl.load(&tmK, x, sbase + C::K_OFF + st * C::KV_BYTES, bar(C::B_KF + st));
         __syncwarp();
       }
       if (!ok) break;
       first = (r.flags & RUN_LAST) != 0;
-      pos += units, off += units;
     }
     if (ok && wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1) && lane == 0) {
       runs[n % PA_RING].flags = RUN_END;
@@ -414,9 +424,9 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
         Blocks<D> bl;
         bl.start(a, r, lane);
         for (int b = 0; b < r.nb; b++, g++) {
-          const int st = g % NST;
+          const int st = g % VST;
           const typename Blocks<D>::Rows x = bl.rows(a, r.kb + b, lane);
-          if (!(ok = wait_warp(C::B_VE + st, g / NST + 1))) break;
+          if (!(ok = wait_warp(C::B_VE + st, g / VST + 1))) break;
           if (elect_one()) bl.load(&tmV, x, sbase + C::V_OFF + st * C::KV_BYTES, bar(C::B_VF + st));
           __syncwarp();
         }
@@ -432,41 +442,41 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
       if ((r.flags & RUN_FIRST) && lane < 4) mark[lane] = 0;
       __syncwarp();
       for (int b = 0; b < r.nb; b++, g++) {
-        const int st = g % NST;
-        if (!(ok = wait_warp(C::B_VF + st, g / NST))) break;
-        const int key0 = (r.kb + b) * 64, valid = min(64, r.kend - key0), pad = (valid + 15) & ~15;
+        const int st = g % VST;
+        if (!(ok = wait_warp(C::B_VF + st, g / VST))) break;
+        const int key0 = (r.kb + b) * KB, valid = min(KB, r.kend - key0), pad = (valid + 15) & ~15;
         uint8_t *v = smem + C::V_OFF + st * C::KV_BYTES + (lane & 7) * 16;
         if (valid < pad) {  // up to 15 rows, four at a time
           for (int row = valid + lane / 8; row < pad; row += 4)
 #pragma unroll
-            for (int at = 0; at < NA; at++) *reinterpret_cast<uint4 *>(v + at * (64 * 128) + row * 128) = make_uint4(0, 0, 0, 0);
+            for (int at = 0; at < NA; at++) *reinterpret_cast<uint4 *>(v + at * (KB * 128) + row * 128) = make_uint4(0, 0, 0, 0);
         }
         // the first row of the tile that sees the block sees the fewest of its keys
         const int t1 = max(max(r.tok0, r.qb), key0 - r.len + r.qe);
         const bool scan = r.seg >= 0 && own_limit(t1, r.qe, r.len) < key0 + valid;
         if (scan) {
-          int worst = 64;  // the first row with a value that is not finite
+          int worst = KB;  // the first row with a value that is not finite
 #pragma unroll 1
           for (int at = 0; at < NA; at++) {
 #pragma unroll 1
-            for (int i0 = 0; i0 < 16; i0 += 8) {
+            for (int i0 = 0; 4 * i0 < valid; i0 += 8) {
               uint4 x[8];
 #pragma unroll
               for (int i = 0; i < 8; i++)
-                x[i] = *reinterpret_cast<uint4 *>(v + at * (64 * 128) + (4 * (i0 + i) + lane / 8) * 128);
+                x[i] = *reinterpret_cast<uint4 *>(v + at * (KB * 128) + (4 * (i0 + i) + lane / 8) * 128);
 #pragma unroll
               for (int i = 0; i < 8; i++) {
                 const int row = 4 * (i0 + i) + lane / 8;
                 auto big = [](uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; };
                 if (row < valid && (big(x[i].x) | big(x[i].y) | big(x[i].z) | big(x[i].w))) {
-                  *reinterpret_cast<uint4 *>(v + at * (64 * 128) + row * 128) = make_uint4(0, 0, 0, 0);
+                  *reinterpret_cast<uint4 *>(v + at * (KB * 128) + row * 128) = make_uint4(0, 0, 0, 0);
                   worst = min(worst, row);
                 }
               }
             }
           }
           worst = __reduce_min_sync(0xffffffffu, worst);
-          if (worst < 64 && lane < 4) {
+          if (worst < KB && lane < 4) {
             // rows of the sequence in this tile that see key key0 + worst
             const int from = max(max(r.tok0, r.qb), key0 + worst - r.len + r.qe) - r.tok0;
             const int to = min(r.qe, r.tok0 + r.ntok) - r.tok0;
@@ -482,82 +492,73 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
       if (ok) done_run(n);
     }
   } else if (warp == PA_WM) {
+    // Q K^T, one thread: a block's scores go to the buffer of the warpgroup that takes it, free since the P V of the
+    // block PA_WG before
     constexpr uint32_t idesc_qk = idesc_f16_f32(128, KB);
-    constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // V MN-major
-    // One thread. Q K^T of block g + 1 needs the scores' buffer that P V of block g - 1 frees, so the two are issued
-    // together, as soon as the weights of g - 1 are there; everything else that they need is waited for before.
     if (elect_one()) {
-      const uint64_t q0 = desc_sw128(sbase), k0 = desc_sw128(sbase + C::K_OFF), v0 = desc_mn(sbase + C::V_OFF, KB * 128);
-      auto wait1 = [&](int i, int parity) {
-        return mbar_wait_alert(bar(i), (uint32_t)parity & 1u, abort, a.err, DC_DEVERR_ATTN_WAIT);
-      };
-      int g = 0, item = 0;
-      bool ok = true, pend = false, begins = true;  // begins: the tile has had no product yet
-      int steps = 0;                                // of the pending product (block g - 1): 16 keys each,
-      uint32_t off[4] = {};                         // and the rows that it leaves alone
-      auto qk = [&](int x) {
-        const int st = x % NST;
-        const uint32_t sc = tmem + (uint32_t)(C::S_COL + (x & 1) * KB);
-        const uint64_t k = k0 + (uint32_t)(st * C::KV_BYTES >> 4);
-        tc_fence_after();
+      const uint64_t q0 = desc_sw128(sbase), k0 = desc_sw128(sbase + C::K_OFF);
+      int g = 0;
+      bool ok = true;
+      for (int n = 0; ok && wait1(C::B_IF + n % PA_RING, n / PA_RING); n++) {
+        const int flags = runs[n % PA_RING].flags, nb = runs[n % PA_RING].nb, item = runs[n % PA_RING].item;
+        if (flags & RUN_END) break;
+        if (flags & RUN_FIRST) ok = wait1(C::B_QF, item);
+#pragma unroll 1
+        for (int b = 0; ok && b < nb; b++, g++) {
+          const int st = g % KST, sb = g % PA_WG;
+          if (!(ok = wait1(C::B_KF + st, g / KST) && wait1(C::B_SE + sb, g / PA_WG + 1))) break;
+          tc_fence_after();
+          const uint32_t sc = tmem + (uint32_t)(C::S_COL + sb * KB);
+          const uint64_t k = k0 + (uint32_t)(st * C::KV_BYTES >> 4);
 #pragma unroll
-        for (int kd = 0; kd < D / 16; kd++)
-          mma_f16(sc, q0 + (((kd >> 2) * 128 * 128 + (kd & 3) * 32) >> 4), k + (((kd >> 2) * KB * 128 + (kd & 3) * 32) >> 4),
-                  idesc_qk, kd > 0);
-        mma_commit(bar(C::B_SF + (x & 1)));
-        mma_commit(bar(C::B_KE + st));
-      };
-      auto pv = [&](int x) -> bool {
-        const int st = x % NST;
-        if (!wait1(C::B_VF + st, x / NST) || !wait1(C::B_VS + st, x / NST)) return false;
-        if (begins && !wait1(C::B_OE, item)) return false;  // the accumulator is zero
-        begins = false;
-        if (!wait1(C::B_PF + (x & 1), x >> 1)) return false;
-        tc_fence_after();
-        const uint32_t p = tmem + (uint32_t)(C::S_COL + (x & 1) * KB);
-        const uint64_t v = v0 + (uint32_t)(st * C::KV_BYTES >> 4);
-#pragma unroll
-        for (int kk = 0; kk < KB / 16; kk++)
-          if (kk < steps) mma_f16_ts_rows(tmem + C::O_COL, p + 8 * kk, v + kk * (2048 >> 4), idesc_pv, off);
-        mma_commit(bar(C::B_VE + st));
-        mma_commit(bar(C::B_OR));
-        return true;
-      };
+          for (int kd = 0; kd < D / 16; kd++)
+            mma_f16(sc, q0 + (((kd >> 2) * 128 * 128 + (kd & 3) * 32) >> 4), k + (((kd >> 2) * KB * 128 + (kd & 3) * 32) >> 4),
+                    idesc_qk, kd > 0);
+          mma_commit(bar(C::B_SF + sb));
+          mma_commit(bar(C::B_KE + st));
+        }
+        if (ok && (flags & RUN_LAST)) mma_commit(bar(C::B_QE));
+        if (ok) mbar_arrive(bar(C::B_IE + n % PA_RING));
+      }
+    }
+    __syncwarp();
+  } else if (warp == PA_WP) {
+    // P V, one thread
+    constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // V MN-major
+    if (elect_one()) {
+      const uint64_t v0 = desc_mn(sbase + C::V_OFF, KB * 128);
+      int g = 0;
+      bool ok = true;
       for (int n = 0; ok && wait1(C::B_IF + n % PA_RING, n / PA_RING); n++) {
         const Run r = runs[n % PA_RING];
         if (r.flags & RUN_END) break;
-        if (r.flags & RUN_FIRST) item = r.item, begins = true, ok = wait1(C::B_QF, item);
+        if (r.flags & RUN_FIRST) ok = wait1(C::B_OE, r.item);  // the accumulator is zero
 #pragma unroll 1
         for (int b = 0; ok && b < r.nb; b++, g++) {
-          if (b == 0) {
-            if (!(ok = wait1(C::B_KF + g % NST, g / NST))) break;
-            qk(g);
-          }
-          const bool next = b + 1 < r.nb;
-          if (next && !(ok = wait1(C::B_KF + (g + 1) % NST, (g + 1) / NST))) break;
-          if (pend && !(ok = pv(g - 1))) break;
-          if (next) qk(g + 1);
-          pend = true;
-          const int key0 = (r.kb + b) * 64;
-          steps = (min(64, r.kend - key0) + 15) >> 4;
-          // own blocks: the rows of the sequence that see a key of it
-          const int lo = r.seg < 0 ? 0 : (max(max(r.tok0, r.qb), key0 - r.len + r.qe) - r.tok0) * a.r;
-          const int hi = r.seg < 0 ? 128 : (min(r.qe, r.tok0 + r.ntok) - r.tok0) * a.r;
+          const int st = g % VST, sb = g % PA_WG, key0 = (r.kb + b) * KB;
+          const int steps = (min(KB, r.kend - key0) + 15) >> 4;  // of 16 keys
+          uint32_t off[4] = {0, 0, 0, 0};                        // rows that it leaves alone
+          if (r.seg >= 0) {                                      // own blocks: but the sequence's that see a key of it
+            const int lo = (max(max(r.tok0, r.qb), key0 - r.len + r.qe) - r.tok0) * a.r;
+            const int hi = (min(r.qe, r.tok0 + r.ntok) - r.tok0) * a.r;
 #pragma unroll
-          for (int w = 0; w < 4; w++) {
-            const int x = min(max(lo - 32 * w, 0), 32), y = min(max(hi - 32 * w, 0), 32);
-            const uint32_t upto = y >= 32 ? ~0u : (1u << y) - 1u, under = x >= 32 ? ~0u : (1u << x) - 1u;
-            off[w] = ~(upto & ~under);
+            for (int w = 0; w < 4; w++) {
+              const int x = min(max(lo - 32 * w, 0), 32), y = min(max(hi - 32 * w, 0), 32);
+              const uint32_t upto = y >= 32 ? ~0u : (1u << y) - 1u, under = x >= 32 ? ~0u : (1u << x) - 1u;
+              off[w] = ~(upto & ~under);
+            }
           }
+          if (!(ok = wait1(C::B_VS + st, g / VST) && wait1(C::B_PF + sb, g / PA_WG))) break;  // (VS: after VF)
+          tc_fence_after();
+          const uint32_t p = tmem + (uint32_t)(C::S_COL + sb * KB);
+          const uint64_t v = v0 + (uint32_t)(st * C::KV_BYTES >> 4);
+#pragma unroll
+          for (int kk = 0; kk < KB / 16; kk++)
+            if (kk < steps) mma_f16_ts_rows(tmem + C::O_COL, p + 8 * kk, v + kk * (2048 >> 4), idesc_pv, off);
+          mma_commit(bar(C::B_SE + sb));
+          mma_commit(bar(C::B_VE + st));
         }
-        if (ok && (r.flags & RUN_LAST)) {
-          mma_commit(bar(C::B_QE));
-          if (pend) ok = pv(g - 1);
-          pend = false;
-          // a tile without keys: the last tile's end has to be past before this one's is announced
-          if (ok && begins) ok = wait1(C::B_OE, item);
-          if (ok) mma_commit(bar(C::B_OD));
-        }
+        if (ok && (r.flags & RUN_LAST)) mma_commit(bar(C::B_OD));
         if (ok) mbar_arrive(bar(C::B_IE + n % PA_RING));
       }
     }
@@ -565,21 +566,21 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
   } else {
     const int q = warp & 3, wg = warp >> 2;
     const int row = 32 * q + lane, irow = row / a.r, jrow = row - irow * a.r;
-    const uint32_t lrow = tmem + ((uint32_t)(32 * q) << 16), ocol = lrow + (uint32_t)(C::O_COL + wg * (D / 2));
+    const uint32_t lrow = tmem + ((uint32_t)(32 * q) << 16), ocol = lrow + (uint32_t)C::O_COL;
     const uint32_t scol = lrow + (uint32_t)(C::S_COL + wg * KB);
-    float *s_ref = reinterpret_cast<float *>(smem + C::XCH_OFF), *s_sum = s_ref + 128;  // [128], [2 turns][2][128]
+    float *s_ref = reinterpret_cast<float *>(smem + C::XCH_OFF), *s_sum = s_ref + 128;  // [128], [2 turns][PA_WG][128]
     Run r;
-    int g = 0, chain = 0, meets = 0;
+    int g = 0, mine = wg, meets = 0;  // blocks: the line's, this warpgroup's next
     bool ok = true;
     // the tile's state
     bool valid = false, anyv = false, had = false, tfirst = false;
     int t = 0, seq = -1, lim = 0;
     float ref = -FLT_MAX, l = 0.f;  // l: the sum of this thread's weights, in units of 2^(ref - 7)
-    auto zero = [&]() {             // this warp's half of its rows' accumulators
+    auto zero = [&]() {             // this warp's share of its rows' accumulators: every third 16 columns
       const uint32_t z[16] = {};
       __syncwarp();
-#pragma unroll
-      for (int c = 0; c < D / 2; c += 16) tmem_st16(ocol + c, z);
+#pragma unroll 1
+      for (int c = 16 * wg; c < D; c += 16 * PA_WG) tmem_st16(ocol + c, z);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -608,18 +609,20 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
       for (int b = 0; b < r.nb; b++, g++) {
         const bool opens = !had;  // the tile's first block
         had = true;
-        if (anyv) chain++;
-        if ((g & 1) != wg) continue;
-        if (!(ok = wait_warp(C::B_SF + wg, g >> 1))) break;
-        const int nv = min(max(rlim - (r.kb + b) * 64, 0), 64);
+        if (g != mine) continue;
+        mine += PA_WG;
+        const int turn = g / PA_WG;
+        if (!(ok = wait_warp(C::B_SF + wg, turn))) break;
+        const int nv = min(max(rlim - (r.kb + b) * KB, 0), KB);
+        const int cols = min(KB, (r.kend - (r.kb + b) * KB + 31) & ~31);  // the others' weights are not read
         // (lanes without a row do not force the masks on the others)
-        const bool sees = __any_sync(0xffffffffu, nv > 0), part = !__all_sync(0xffffffffu, nv == 64 || !valid);
+        const bool sees = __any_sync(0xffffffffu, nv > 0), part = !__all_sync(0xffffffffu, nv >= cols || !valid);
         float sc = a.scale_log2, pmx = -FLT_MAX;
         if (sees) {
           tc_fence_after();
           if (sc <= 0.f) {  // the largest score is not the largest product: scale first
 #pragma unroll 1
-            for (int c = 0; c < KB; c += 16) {
+            for (int c = 0; c < cols; c += 16) {
               uint32_t x[16];
               __syncwarp();
               tmem_ld16(scol + c, x);
@@ -634,7 +637,7 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
           }
           float m2[2] = {__uint_as_float(0xff800000u), __uint_as_float(0xff800000u)};
 #pragma unroll 1
-          for (int c = 0; c < KB; c += 32) {
+          for (int c = 0; c < cols; c += 32) {
             uint32_t x[32];
             __syncwarp();
             tmem_ld32(scol + c, x);
@@ -650,15 +653,16 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
           }
           pmx = fmaxf(m2[0], m2[1]) * sc;
         }
+        // the row's reference goes from block to block through shared memory, with the turn to move it
+        const int prev = wg == 0 ? PA_WG - 1 : wg - 1;
+        if (g > 0 && !(ok = wait_warp(C::B_CH + PA_WG * q + prev, (g - 1) / PA_WG))) break;
         if (anyv) {
-          // the row's reference goes from block to block through shared memory, with the turn to move it
-          if (!(ok = wait_warp(C::B_CH + q, chain))) break;
           const float cur = opens ? -FLT_MAX : s_ref[row];
           const bool grow = pmx > cur + 8.0f;
           const float now = grow ? pmx : cur;
           const bool resc = grow && cur > -FLT_MAX;
           if (__any_sync(0xffffffffu, resc)) {
-            if (!(ok = wait_warp(C::B_OR, g - 1))) break;  // the products so far
+            if (!(ok = wait_warp(C::B_SE + prev, (g - 1) / PA_WG))) break;  // the products so far
             tc_fence_after();
             const float f = resc ? ex2_approx(cur - now) : 1.0f;
 #pragma unroll 1
@@ -675,18 +679,18 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
             tmem_st_wait();
           }
           if (grow || opens) s_ref[row] = now;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(C::B_CH + q));
           if (__any_sync(0xffffffffu, now != ref)) {
             l *= ex2_approx(ref - now);  // 0 * 0 where there was none
             ref = now;
           }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::B_CH + PA_WG * q + wg));
         if (sees) {
           const uint64_t ref2 = f32x2(7.0f - ref, 7.0f - ref), sc2 = f32x2(sc, sc);
           uint64_t sum[2] = {0, 0};
 #pragma unroll 1
-          for (int c = 0; c < KB; c += 32) {  // 32 weights go where 16 of the scores were that are done with
+          for (int c = 0; c < cols; c += 32) {  // 32 weights go where 16 of the scores were that are done with
             uint32_t x[32];
             __syncwarp();
             tmem_ld32(scol + c, x);
@@ -719,14 +723,16 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
         tc_fence_after();
         if (anyv) {
           const bool tlast = (r.flags & RUN_TLAST) != 0, direct = tfirst && tlast;
-          // the two warps of the quadrant add their sums at the row's last reference
+          // the quadrant's warps add their sums at the row's last reference
           const float fin = had ? s_ref[row] : -FLT_MAX;
-          float *sums = s_sum + (meets & 1) * 256;
+          float *sums = s_sum + (meets & 1) * (PA_WG * 128);
           sums[wg * 128 + row] = l * ex2_approx(ref - fin);
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(C::B_XB + q));
           if (!(ok = wait_warp(C::B_XB + q, meets++))) break;
-          float lt = sums[row] + sums[128 + row];
+          float lt = 0.f;
+#pragma unroll
+          for (int w = 0; w < PA_WG; w++) lt += sums[w * 128 + row];
           if (had && valid && ((poison[4 * (r.item & 3) + (irow >> 5)] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
           const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
           if (valid && jrow == 0 && wg == 0) {
@@ -735,10 +741,10 @@ __global__ void __launch_bounds__(PA_THREADS, PCfg<D>::CTAS)
           }
           if (!direct && valid && wg == 0) a.ml[prow] = make_float2(fin, lt);
           const float inv = lt == 0.f ? 0.f : 1.0f / lt;
-          __half *y = a.Y + (long)t * a.ystride + (long)(r.kvh * a.r + jrow) * D + wg * (D / 2);
-          float *po = a.O + prow * D + wg * (D / 2);
+          __half *y = a.Y + (long)t * a.ystride + (long)(r.kvh * a.r + jrow) * D;
+          float *po = a.O + prow * D;
 #pragma unroll 1
-          for (int c = 0; c < D / 2; c += 16) {
+          for (int c = 16 * wg; c < D; c += 16 * PA_WG) {
             uint32_t o[16];
             __syncwarp();
             tmem_ld16(ocol + c, o);
@@ -895,8 +901,6 @@ Ws ws_layout(int T, int heads, int kv, int D, int ctas) {
   return w;
 }
 
-int ctas_of(int D) { return D == 64 ? PCfg<64>::CTAS : D == 128 ? PCfg<128>::CTAS : PCfg<256>::CTAS; }
-
 template <int D>
 int launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, const PArgs &a) {
   using C = PCfg<D>;
@@ -911,7 +915,7 @@ int launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, const PArg
     DC_CUDA(cudaFuncSetAttribute(attention_paged_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     attr_done |= 1ull << ctx->device;
   }
-  DC_CUDA(dc_launch_pdl(ctx->stream, attention_paged_kernel<D>, dim3(ctx->sms * C::CTAS), dim3(PA_THREADS), C::SMEM, tq,
+  DC_CUDA(dc_launch_pdl(ctx->stream, attention_paged_kernel<D>, dim3(ctx->sms), dim3(PA_THREADS), C::SMEM, tq,
                         c->mapK, c->mapV, a));
   rc = dc_launch_check("attention_paged");
   if (rc) return rc;
@@ -934,13 +938,13 @@ int attn_cache_maps(dc_kv_cache *c) {
 }
 
 size_t attn_paged_ws(dc_ctx *ctx, const dc_kv_cache *c, int T, int heads) {
-  return ws_layout(T, heads, c->kv, c->D, ctx->sms * ctas_of(c->D)).bytes;
+  return ws_layout(T, heads, c->kv, c->D, ctx->sms).bytes;
 }
 
 int attn_paged_launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, const int *table, int tstride,
                       const int *lens, const int *qoff, int S, const int *ptable, int pstride, const int *plens,
                       const int *goff, int G, void *Y, long ys, int T, int heads, float scale, void *ws) {
-  const Ws w = ws_layout(T, heads, c->kv, c->D, ctx->sms * ctas_of(c->D));
+  const Ws w = ws_layout(T, heads, c->kv, c->D, ctx->sms);
   char *p = static_cast<char *>(ws);
   PArgs a;
   a.Y = static_cast<__half *>(Y), a.ystride = ys;
@@ -952,7 +956,7 @@ int attn_paged_launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs,
   a.tstride = tstride, a.pstride = pstride, a.S = S, a.G = G, a.T = T, a.heads = heads, a.kv = c->kv;
   a.r = heads / c->kv, a.tpt = 128 / a.r, a.page = c->page, a.pages = c->pages;
   a.pshift = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7, a.rows = c->pages * c->kv * c->page;
-  a.chunk_min = 4;
+  a.chunk_min = 2;
   a.scale_log2 = scale * 1.4426950408889634f;
   if (c->D == 64) return launch<64>(ctx, c, Q, qs, a);
   if (c->D == 128) return launch<128>(ctx, c, Q, qs, a);
