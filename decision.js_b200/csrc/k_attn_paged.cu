@@ -86,7 +86,9 @@ struct PCfg {
 struct PArgs {
   __half *Y;
   const int *table, *lens, *qoff, *ptable, *plens, *goff;
-  int *hdr, *recF, *recL;
+  int *hdr;
+  int4 *head;  // by CTA: the tile that it ends and did not begin (first row, rows, kv head), or no rows
+  int *tail;   // by CTA: whether it begins a tile that it does not end
   float2 *ml;
   float *O;
   uint32_t *err;
@@ -296,7 +298,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     if (warp == PA_WM) tc_fence_after(), tmem_dealloc(*tmem_slot, C::TCOLS);
     return;
   }
-  if (blockIdx.x == 0 && tid == 0) a.hdr[0] = 0;
+  if (tid == 0) {
+    if (blockIdx.x == 0) a.hdr[0] = 0;
+    a.head[blockIdx.x] = make_int4(0, 0, 0, 0), a.tail[blockIdx.x] = 0;
+  }
   long before = incl - mine, line = 0;
 #pragma unroll
   for (int w = 0; w < PA_THREADS / 32; w++) {
@@ -305,10 +310,18 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     line += v;
   }
   const long B = line * a.kv;
-  const long chunk = max((long)a.chunk_min, (B + gridDim.x - 1) / gridDim.x);
-  const long p0 = chunk * blockIdx.x, p1 = min(p0 + chunk, B);
+  long chunk, p0;
+  int kvh0 = 0;
+  if (B < 0x7fff0000) {  // (64-bit divisions take a microsecond)
+    chunk = max((unsigned)a.chunk_min, ((unsigned)B + gridDim.x - 1) / gridDim.x);
+    p0 = chunk * blockIdx.x;
+    if (p0 < B) kvh0 = (unsigned)p0 / (unsigned)line;
+  } else {
+    chunk = (B + gridDim.x - 1) / gridDim.x, p0 = chunk * blockIdx.x;
+    if (p0 < B) kvh0 = (int)(p0 / line);
+  }
+  const long p1 = min(p0 + chunk, B);
   const bool work = p0 < p1;
-  const int kvh0 = work ? (int)(p0 / line) : 0;
   if (work && mine > 0) {
     long off = p0 - kvh0 * line - before;
     if (off >= 0 && off < mine) {
@@ -569,8 +582,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const uint32_t lrow = tmem + ((uint32_t)(32 * q) << 16), ocol = lrow + (uint32_t)C::O_COL;
     const uint32_t scol = lrow + (uint32_t)(C::S_COL + wg * KB);
     float *s_ref = reinterpret_cast<float *>(smem + C::XCH_OFF), *s_sum = s_ref + 128;  // [128], [2 turns][PA_WG][128]
-    Run r;
-    int g = 0, mine = wg, meets = 0;  // blocks: the line's, this warpgroup's next
+    int g = 0, turn = 0, meets = 0;  // blocks before the run, this warpgroup's blocks before this one
+    const int prev = wg == 0 ? PA_WG - 1 : wg - 1;
     bool ok = true;
     // the tile's state
     bool valid = false, anyv = false, had = false, tfirst = false;
@@ -587,7 +600,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       if (lane == 0) mbar_arrive(bar(C::B_OE));
     };
     zero();
-    for (int n = 0; ok && next_run(n, r); n++) {
+    for (int n = 0; ok && wait_warp(C::B_IF + n % PA_RING, n / PA_RING); n++) {
+      const Run &r = runs[n % PA_RING];  // (stays as it is until done_run)
+      if (r.flags & RUN_END) break;
       if (r.flags & RUN_FIRST) {
         t = r.tok0 + irow;
         valid = irow < r.ntok && irow < a.tpt;
@@ -606,17 +621,16 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
       }
       const int rlim = !valid ? 0 : r.seg < 0 ? r.kend : seq == r.seg ? lim : 0;
-      for (int b = 0; b < r.nb; b++, g++) {
-        const bool opens = !had;  // the tile's first block
-        had = true;
-        if (g != mine) continue;
-        mine += PA_WG;
-        const int turn = g / PA_WG;
+      const int nb = r.nb, kb = r.kb, kend = r.kend;
+      // the run's first blocks that every row here sees whole (lanes without a row have no say)
+      const int full = __reduce_min_sync(0xffffffffu, valid ? rlim : 0x7fffffff) / KB - kb;
+      for (int b = (wg + PA_WG - g % PA_WG) % PA_WG; b < nb; b += PA_WG, turn++) {
+        const bool opens = b == 0 && !had;  // the tile's first block
         if (!(ok = wait_warp(C::B_SF + wg, turn))) break;
-        const int nv = min(max(rlim - (r.kb + b) * KB, 0), KB);
-        const int cols = min(KB, (r.kend - (r.kb + b) * KB + 31) & ~31);  // the others' weights are not read
-        // (lanes without a row do not force the masks on the others)
-        const bool sees = __any_sync(0xffffffffu, nv > 0), part = !__all_sync(0xffffffffu, nv >= cols || !valid);
+        const int nv = rlim - (kb + b) * KB;  // its keys that the row sees (or fewer than none, or more than there are)
+        const bool part = b >= full;
+        const bool sees = part ? __any_sync(0xffffffffu, nv > 0) : anyv;
+        const int cols = part ? min(KB, (kend - (kb + b) * KB + 31) & ~31) : KB;  // the others' weights are not read
         float sc = a.scale_log2, pmx = -FLT_MAX;
         if (sees) {
           tc_fence_after();
@@ -654,15 +668,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           pmx = fmaxf(m2[0], m2[1]) * sc;
         }
         // the row's reference goes from block to block through shared memory, with the turn to move it
-        const int prev = wg == 0 ? PA_WG - 1 : wg - 1;
-        if (g > 0 && !(ok = wait_warp(C::B_CH + PA_WG * q + prev, (g - 1) / PA_WG))) break;
+        if (g + b > 0 && !(ok = wait_warp(C::B_CH + PA_WG * q + prev, wg == 0 ? turn - 1 : turn))) break;
         if (anyv) {
           const float cur = opens ? -FLT_MAX : s_ref[row];
           const bool grow = pmx > cur + 8.0f;
           const float now = grow ? pmx : cur;
           const bool resc = grow && cur > -FLT_MAX;
           if (__any_sync(0xffffffffu, resc)) {
-            if (!(ok = wait_warp(C::B_SE + prev, (g - 1) / PA_WG))) break;  // the products so far
+            if (!(ok = wait_warp(C::B_SE + prev, wg == 0 ? turn - 1 : turn))) break;  // the products so far
             tc_fence_after();
             const float f = resc ? ex2_approx(cur - now) : 1.0f;
 #pragma unroll 1
@@ -718,11 +731,16 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         if (lane == 0) mbar_arrive(bar(C::B_PF + wg));
       }
       if (!ok) break;
+      g += nb, had = had || nb > 0;
       if (r.flags & RUN_LAST) {
         if (!(ok = wait_warp(C::B_OD, r.item))) break;
         tc_fence_after();
+        const bool tlast = (r.flags & RUN_TLAST) != 0, direct = tfirst && tlast;
+        if (!direct && warp == 0 && lane == 0) {
+          if (tlast) a.head[blockIdx.x] = make_int4(r.tok0, r.ntok, r.kvh, 0);
+          if (tfirst) a.tail[blockIdx.x] = 1;
+        }
         if (anyv) {
-          const bool tlast = (r.flags & RUN_TLAST) != 0, direct = tfirst && tlast;
           // the quadrant's warps add their sums at the row's last reference
           const float fin = had ? s_ref[row] : -FLT_MAX;
           float *sums = s_sum + (meets & 1) * (PA_WG * 128);
@@ -735,10 +753,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           for (int w = 0; w < PA_WG; w++) lt += sums[w * 128 + row];
           if (had && valid && ((poison[4 * (r.item & 3) + (irow >> 5)] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
           const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
-          if (valid && jrow == 0 && wg == 0) {
-            if (tfirst) a.recF[(long)r.kvh * a.T + t] = direct ? -1 : (int)blockIdx.x;
-            if (tlast) a.recL[(long)r.kvh * a.T + t] = (int)blockIdx.x;
-          }
           if (!direct && valid && wg == 0) a.ml[prow] = make_float2(fin, lt);
           const float inv = lt == 0.f ? 0.f : 1.0f / lt;
           __half *y = a.Y + (long)t * a.ystride + (long)(r.kvh * a.r + jrow) * D;
@@ -772,88 +786,73 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 
   tc_fence_before();
   __syncthreads();
+  if (tid == 0 && *abort) a.hdr[0] = 1;  // a wait ran out: the records may be missing
   if (warp == PA_WM) {
     tc_fence_after();
     tmem_dealloc(tmem, C::TCOLS);
   }
 }
 
-// Joins the parts of the rows whose tiles were cut: y = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over the CTAs c
-// from the tile's first to its last, in that order. W warps to a row, each every W-th part.
-template <int D, int W>
+// Joins the parts of the tiles that were cut: y = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over the CTAs c from the
+// tile's first to its last, in that order. A block takes four rows of the tile that CTA blockIdx.y ends, a warp each.
+template <int D>
 __global__ void __launch_bounds__(128) attention_join_kernel(const PArgs a) {
   dc_pdl_begin();
   constexpr int N = D / 32;  // a lane's values
-  __shared__ float s_o[W > 1 ? W : 1][W > 1 ? D : 1];
-  __shared__ float s_m[4], s_l[4];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long idx = W > 1 ? (long)blockIdx.x : (long)blockIdx.x * 4 + warp;
-  const long t = idx / a.heads;
-  if (t >= a.T) return;
-  const int h = (int)(idx - t * a.heads), kvh = h / a.r, j = h - kvh * a.r;
-  // all four loads in flight; the records of a row outside the sequences are not defined, and not used
-  const int refused = a.hdr[0], t0 = a.qoff[0], t1 = a.qoff[a.S];
-  const int c0 = a.recF[(long)kvh * a.T + t], c1 = a.recL[(long)kvh * a.T + t];
-  if (refused || t < t0 || t >= t1 || c0 < 0) return;
-  // part c of this row: row base + 128 c
-  const long base = ((long)kvh * a.T + t) * a.r + j;
-  const int first = W > 1 ? c0 + warp : c0;
+  const int lane = threadIdx.x & 31, row = blockIdx.x * 4 + (threadIdx.x >> 5), c1 = blockIdx.y;
+  const int refused = a.hdr[0];  // (a refused call, or one whose waits ran out, has no records)
+  const int4 tile = a.head[c1];
+  if (refused || row >= tile.y * a.r) return;
+  int c0 = -1;  // the last CTA before that begins a tile and does not end it
+  for (int e = c1; e > 0 && c0 < 0; e -= 32) {
+    const int c = e - 1 - lane;
+    const uint32_t at = __ballot_sync(0xffffffffu, c >= 0 && a.tail[c] != 0);
+    if (at) c0 = e - __ffs(at);
+  }
+  if (c0 < 0) return;
+  const int i = row / a.r, j = row - i * a.r;
+  const long base = ((long)tile.z * a.T + tile.x) * a.r + row;  // part c of this row: row base + 128 c
   float M = -FLT_MAX, L = 0.f, o[N] = {};
-  for (int cb = first; cb <= c1; cb += W * 32) {  // 32 parts at a time, usually all
-    const int c = cb + W * lane;
+  for (int cb = c0; cb <= c1; cb += 32) {  // 32 parts at a time, usually all
+    const int c = cb + lane;
     const float2 x = c <= c1 ? a.ml[base + 128L * c] : make_float2(-FLT_MAX, 0.f);
-    const int cnt = min(32, (c1 - cb) / W + 1);
+    const int cnt = min(32, c1 - cb + 1);
     float m = x.y == 0.f ? -FLT_MAX : x.x;  // a part of weight 0 stored no values
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
     m = fmaxf(m, M);
-    const float f = ex2_approx(M - m);  // what is there goes to the new maximum (0 the first time)
+    const float f = ex2_approx(M - m);  // what is there goes to the new maximum
     M = m;
     const float w = x.y == 0.f ? 0.f : ex2_approx(x.x - M);
     L = L * f + (x.y == 0.f ? 0.f : w * x.y);
 #pragma unroll
     for (int e = 0; e < N; e++) o[e] *= f;
     const uint32_t have = __ballot_sync(0xffffffffu, x.y != 0.f);
-#pragma unroll 4
-    for (int i = 0; i < cnt; i++) {
-      const float wi = __shfl_sync(0xffffffffu, w, i);
-      const float *p = a.O + (base + 128L * (cb + W * i)) * D + N * lane;
-      float v[N];
-      if (N == 2) {
-        *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(p);
-      } else {
+    for (int k0 = 0; k0 < cnt; k0 += 8) {  // eight parts' values on their way
+      float v[8][N];
 #pragma unroll
-        for (int e = 0; e < N; e += 4) *reinterpret_cast<float4 *>(v + e) = *reinterpret_cast<const float4 *>(p + e);
+      for (int k = 0; k < 8; k++) {
+        const float *p = a.O + (base + 128L * (cb + min(k0 + k, cnt - 1))) * D + N * lane;
+        if (N == 2) {
+          *reinterpret_cast<float2 *>(v[k]) = *reinterpret_cast<const float2 *>(p);
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; e += 4) *reinterpret_cast<float4 *>(v[k] + e) = *reinterpret_cast<const float4 *>(p + e);
+        }
       }
-      const bool use = (have >> i) & 1u;
 #pragma unroll
-      for (int e = 0; e < N; e++) o[e] = use ? fmaf(wi, v[e], o[e]) : o[e];
+      for (int k = 0; k < 8; k++) {
+        const float wk = __shfl_sync(0xffffffffu, w, (k0 + k) & 31);
+        const bool use = k0 + k < cnt && ((have >> (k0 + k)) & 1u);
+#pragma unroll
+        for (int e = 0; e < N; e++) o[e] = use ? fmaf(wk, v[k][e], o[e]) : o[e];
+      }
     }
   }
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
-  if (W > 1) {
-    if (lane == 0) s_m[warp] = M, s_l[warp] = L;
-    __syncthreads();
-    const float all = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    const float f = s_l[warp] == 0.f ? 0.f : ex2_approx(M - all);
-#pragma unroll
-    for (int e = 0; e < N; e++) s_o[warp][N * lane + e] = o[e] * f;
-    L = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; w++)
-      if (s_l[w] != 0.f) L += s_l[w] * ex2_approx(s_m[w] - all);
-    __syncthreads();
-    if (warp) return;
-#pragma unroll
-    for (int e = 0; e < N; e++) {
-      o[e] = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; w++) o[e] += s_o[w][N * lane + e];
-    }
-  }
+  for (int s = 16; s > 0; s >>= 1) L += __shfl_xor_sync(0xffffffffu, L, s);
   const float inv = L == 0.f ? 0.f : 1.0f / L;
-  __half *y = a.Y + t * a.ystride + (long)h * D + N * lane;
+  __half *y = a.Y + (long)(tile.x + i) * a.ystride + (long)(tile.z * a.r + j) * D + N * lane;
 #pragma unroll
   for (int e = 0; e < N; e += 2)
     *reinterpret_cast<__half2 *>(y + e) = __floats2half2_rn(o[e] * inv, o[e + 1] * inv);
@@ -884,18 +883,18 @@ int encode(CUtensorMap *m, const void *p, int rank, const cuuint64_t *dims, cons
 
 size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// The workspace: a status word, each tile's first and last CTA by (kv head, row), parts' maxima and sums, parts' sums
-// of values. Part c of a tile starts at row (kvh T + tile) r + 128 c: along the line either the tile moves on, by at
-// least its rows, or c does, so no two parts meet.
+// The workspace: a status word, the CTAs' records, parts' maxima and sums, parts' sums of values. Part c of a tile
+// starts at row (kvh T + first row) r + 128 c: along the line either the tile moves on, by at least its rows, or c does,
+// so no two parts meet.
 struct Ws {
-  size_t recF, recL, ml, O, bytes;
+  size_t head, tail, ml, O, bytes;
 };
-Ws ws_layout(int T, int heads, int kv, int D, int ctas) {
+Ws ws_layout(int T, int heads, int D, int ctas) {
   Ws w;
   const size_t rows = (size_t)T * heads + 128 * (size_t)(ctas + 1);
-  w.recF = 256;
-  w.recL = w.recF + up((size_t)T * kv * 4);
-  w.ml = w.recL + up((size_t)T * kv * 4);
+  w.head = 256;
+  w.tail = w.head + up((size_t)ctas * 16);
+  w.ml = w.tail + up((size_t)ctas * 4);
   w.O = w.ml + up(rows * 8);
   w.bytes = w.O + up(rows * (size_t)D * 4);
   return w;
@@ -919,11 +918,8 @@ int launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, const PArg
                         c->mapK, c->mapV, a));
   rc = dc_launch_check("attention_paged");
   if (rc) return rc;
-  const long rows = (long)a.T * a.heads;
-  if (rows <= 8192)
-    DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D, 4>, dim3((unsigned)rows), dim3(128), 0, a));
-  else
-    DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D, 1>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, a));
+  const dim3 grid((std::min((long)a.T * a.r, 128L) + 3) / 4, ctx->sms);
+  DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D>, grid, dim3(128), 0, a));
   return dc_launch_check("attention_paged (join)");
 }
 
@@ -938,19 +934,19 @@ int attn_cache_maps(dc_kv_cache *c) {
 }
 
 size_t attn_paged_ws(dc_ctx *ctx, const dc_kv_cache *c, int T, int heads) {
-  return ws_layout(T, heads, c->kv, c->D, ctx->sms).bytes;
+  return ws_layout(T, heads, c->D, ctx->sms).bytes;
 }
 
 int attn_paged_launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, const int *table, int tstride,
                       const int *lens, const int *qoff, int S, const int *ptable, int pstride, const int *plens,
                       const int *goff, int G, void *Y, long ys, int T, int heads, float scale, void *ws) {
-  const Ws w = ws_layout(T, heads, c->kv, c->D, ctx->sms);
+  const Ws w = ws_layout(T, heads, c->D, ctx->sms);
   char *p = static_cast<char *>(ws);
   PArgs a;
   a.Y = static_cast<__half *>(Y), a.ystride = ys;
   a.table = table, a.lens = lens, a.qoff = qoff, a.ptable = ptable, a.plens = plens, a.goff = goff;
-  a.hdr = reinterpret_cast<int *>(p), a.recF = reinterpret_cast<int *>(p + w.recF);
-  a.recL = reinterpret_cast<int *>(p + w.recL), a.ml = reinterpret_cast<float2 *>(p + w.ml);
+  a.hdr = reinterpret_cast<int *>(p), a.head = reinterpret_cast<int4 *>(p + w.head);
+  a.tail = reinterpret_cast<int *>(p + w.tail), a.ml = reinterpret_cast<float2 *>(p + w.ml);
   a.O = reinterpret_cast<float *>(p + w.O);
   a.err = ctx->d_err;
   a.tstride = tstride, a.pstride = pstride, a.S = S, a.G = G, a.T = T, a.heads = heads, a.kv = c->kv;
