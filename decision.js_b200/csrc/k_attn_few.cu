@@ -1,0 +1,370 @@
+// The attention over the paged cache for groups of few rows (a decode step: some sequences at one token each). The line
+// of blocks, its cutting and the join are those of the wide kernel (k_attn_paged.cu), as are the tiles of 128 rows; here
+// most rows of a tile are empty and what has to flow is the cache. What a block costs then is the latency of its chain
+// (scores, maximum, weights, product), so two CTAs share an SM and within each two warps share a row:
+//   warps 0-7  softmax: two warps per TMEM lane quadrant, thread = row, each half of a block's keys; the halves' maxima
+//              meet in shared memory. Quadrants without rows only keep step.
+//   warp 8     walks the line, loads Q and K; warp 9 loads V; warp 10 Q K^T and P V (and TMEM); warp 11 looks values over
+// Blocks are 64 keys with two scores' buffers at D = 128, 128 keys with one at D = 64: 256 columns of tensor memory either
+// way, and about the same bytes a block. The weights are scaled by 2^7 as in the wide kernel.
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <float.h>
+
+#include "dc_internal.h"
+#include "dc_paged.cuh"
+#include "dc_ptx.cuh"
+
+using namespace dcx;
+
+namespace {
+
+constexpr int FS = 8;  // softmax warps
+constexpr int FW_K = FS, FW_V = FS + 1, FW_M = FS + 2, FW_C = FS + 3;
+constexpr int F_THREADS = (FS + 4) * 32;
+
+template <int D>
+struct FewCfg {
+  static constexpr int KB = 64, SB = 2;  // keys of a block; scores' buffers
+  static constexpr int NA = D / 64, Q_ROWS = 128, THREADS = F_THREADS;
+  static constexpr int KST = D == 64 ? 4 : 2, VST = KST;
+  static constexpr int Q_BYTES = Q_ROWS * D * 2, KV_BYTES = KB * D * 2;
+  static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + KST * KV_BYTES;
+  static constexpr int BAR_OFF = V_OFF + VST * KV_BYTES;
+  static constexpr int B_QF = 0, B_QE = 1, B_OD = 2, B_OE = 3, B_OR = 4, B_XB = 5, B_SF = 9, B_PF = B_SF + SB,
+                       B_KF = B_PF + SB, B_KE = B_KF + KST, B_VF = B_KE + KST, B_VE = B_VF + VST, B_VS = B_VE + VST,
+                       B_IF = B_VS + VST, B_IE = B_IF + PA_RING, NBARS = B_IE + PA_RING;
+  static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15);
+  static constexpr int POISON_OFF = MISC_OFF + 32, SCAN_OFF = POISON_OFF + 64,
+                       RUN_OFF = SCAN_OFF + ((F_THREADS / 32 * 8 + 15) & ~15), GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run),
+                       XCH_OFF = GOFF_OFF + 3 * (PA_GOFF + 4) * 4;  // floats [2 turns][2 halves][128 rows]
+  static constexpr int SMEM = XCH_OFF + 2 * 2 * 128 * 4 + 1024;
+  static constexpr int S_COL = 0, O_COL = SB * KB, TCOLS = 256;
+  static_assert(O_COL + D <= TCOLS, "tensor memory");
+  static_assert(2 * SMEM <= 227 * 1024, "shared memory");
+};
+
+template <int D>
+__global__ void __launch_bounds__(F_THREADS, 2)
+    attention_paged_few_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                               const __grid_constant__ CUtensorMap tmV, const PArgs a) {
+  using C = FewCfg<D>;
+  constexpr int KB = C::KB, SB = C::SB, KST = C::KST, VST = C::VST, COLS = KB / 2;
+  extern __shared__ uint8_t smem_raw[];
+  const Cta<C> k(a, smem_raw);
+  const int tid = k.tid, warp = k.warp, lane = k.lane;
+  if (tid == 0) {
+    for (int i = 0; i < C::NBARS; i++) {
+      const int n = i == C::B_OE || (i >= C::B_PF && i < C::B_PF + SB) ? FS
+                    : i >= C::B_XB && i < C::B_XB + 4                  ? 2
+                    : i >= C::B_IE                                     ? FS + 3
+                                                                       : 1;
+      mbar_init(k.bar(i), n);
+    }
+    *k.abort() = 0;
+    mbar_init_fence();
+  }
+  if (warp == FW_K && lane == 0) tma_prefetch_desc(&tmQ), tma_prefetch_desc(&tmK);
+  if (warp == FW_V && lane == 0) tma_prefetch_desc(&tmV);
+  // (tensor memory after the kernels before, and before the next is let in: see the wide kernel)
+  dc_pdl_wait();
+  if (warp == FW_M) tmem_alloc(smem_u32(k.tmem_slot()), C::TCOLS);
+  Groups gs;
+  Stretch st;
+  const bool fine = line_start(k, gs, st);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *k.tmem_slot();
+
+  if (!fine || st.p0 >= st.p1) {
+  } else if (warp == FW_K) {
+    walk_line(k, gs, st, &tmQ, &tmK);
+  } else if (warp == FW_V) {
+    load_values(k, &tmV);
+  } else if (warp == FW_C) {
+    look_over(k);
+  } else if (warp == FW_M) {
+    constexpr uint32_t idesc_qk = idesc_f16_f32(128, KB);
+    constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // V MN-major
+    const uint64_t q0 = desc_sw128(k.base), k0 = desc_sw128(k.base + C::K_OFF), v0 = desc_mn(k.base + C::V_OFF, KB * 128);
+    Run r = {};
+    int g = 0;
+    bool ok = true, pend = false, begins = true;  // begins: the tile has had no block yet
+    int steps = 0;                                // of the pending product (block g - 1): 16 keys each,
+    uint32_t off[4] = {};                         // and the rows that it leaves alone
+    auto pv = [&](int x) -> bool {
+      const int vs = x % VST;
+      if (!k.wait_warp(C::B_VS + vs, x / VST) || !k.wait_warp(C::B_PF + x % SB, x / SB)) return false;  // (VS: after VF)
+      tc_fence_after();
+      // the weights of keys [0, COLS) begin the scores' buffer, those of [COLS, KB) its second half
+      const uint32_t p = tmem + (uint32_t)(C::S_COL + x % SB * KB);
+      const uint64_t v = v0 + (uint32_t)(vs * C::KV_BYTES >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < KB / 16; kk++)
+          if (kk < steps)
+            mma_f16_ts_rows(tmem + C::O_COL, p + (kk * 16 < COLS ? 8 * kk : COLS + 8 * kk - COLS / 2), v + kk * (2048 >> 4),
+                            idesc_pv, off);
+        mma_commit(k.bar(C::B_VE + vs));
+        mma_commit(k.bar(C::B_OR));
+      }
+      __syncwarp();
+      return true;
+    };
+    for (int n = 0; ok && k.next_run(n, r); n++) {
+      if (r.flags & RUN_FIRST) ok = k.wait_warp(C::B_QF, r.item), begins = true;
+      for (int b = 0; ok && b < r.nb; b++, g++) {
+        const int ks = g % KST, key0 = (r.kb + b) * KB;
+        if (!(ok = k.wait_warp(C::B_KF + ks, g / KST))) break;
+        if (SB == 1 && pend && !(ok = pv(g - 1))) break;  // the one buffer holds its weights
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t sc = tmem + (uint32_t)(C::S_COL + g % SB * KB);
+          const uint64_t kd0 = k0 + (uint32_t)(ks * C::KV_BYTES >> 4);
+#pragma unroll
+          for (int kd = 0; kd < D / 16; kd++)
+            mma_f16(sc, q0 + (((kd >> 2) * 128 * 128 + (kd & 3) * 32) >> 4), kd0 + (((kd >> 2) * KB * 128 + (kd & 3) * 32) >> 4),
+                    idesc_qk, kd > 0);
+          mma_commit(k.bar(C::B_SF + g % SB));
+          mma_commit(k.bar(C::B_KE + ks));
+        }
+        __syncwarp();
+        if (SB > 1 && pend && !(ok = pv(g - 1))) break;
+        pend = true, begins = false;
+        steps = (min(KB, r.kend - key0) + 15) >> 4;
+        // own blocks: the rows of the sequence that see a key of it
+        const int lo = r.seg < 0 ? 0 : (max(max(r.tok0, r.qb), key0 - r.len + r.qe) - r.tok0) * a.r;
+        const int hi = r.seg < 0 ? 128 : (min(r.qe, r.tok0 + r.ntok) - r.tok0) * a.r;
+#pragma unroll
+        for (int w = 0; w < 4; w++) off[w] = ~mask_word(lo, hi, w);
+      }
+      if (ok && (r.flags & RUN_LAST)) {
+        if (elect_one()) mma_commit(k.bar(C::B_QE));
+        __syncwarp();
+        if (pend) ok = pv(g - 1);
+        pend = false;
+        // a tile without keys: the last tile's end has to be past before this one's is announced
+        if (ok && begins) ok = k.wait_warp(C::B_OE, r.item + 1);
+        if (ok && elect_one()) mma_commit(k.bar(C::B_OD));
+        __syncwarp();
+      }
+      if (ok) k.done_run(n);
+    }
+  } else {
+    const int q = warp & 3, hf = warp >> 2;
+    const int row = 32 * q + lane, irow = row / a.r, jrow = row - irow * a.r;
+    const uint32_t lrow = tmem + ((uint32_t)(32 * q) << 16), ocol = lrow + (uint32_t)(C::O_COL + hf * (D / 2));
+    float *xch = reinterpret_cast<float *>(k.smem + C::XCH_OFF);
+    int g = 0, meets = 0;
+    bool ok = true;
+    // the tile's state
+    bool valid = false, anyv = false, had = false, tfirst = false;
+    int t = 0, seq = -1, lim = 0;
+    float ref = -FLT_MAX, l = 0.f;
+    auto meet = [&]() -> bool {  // both warps of the quadrant have written their halves
+      __syncwarp();
+      if (lane == 0) mbar_arrive(k.bar(C::B_XB + q));
+      return k.wait_warp(C::B_XB + q, meets++);
+    };
+    for (int n = 0; ok && k.wait_warp(C::B_IF + n % PA_RING, n / PA_RING); n++) {
+      const Run &r = k.runs()[n % PA_RING];  // (stays as it is until done_run)
+      if (r.flags & RUN_END) break;
+      if (r.flags & RUN_FIRST) {
+        t = r.tok0 + irow;
+        valid = irow < r.ntok && irow < a.tpt;
+        anyv = __any_sync(0xffffffffu, valid);
+        had = false, tfirst = (r.flags & RUN_TFIRST) != 0;
+        ref = -FLT_MAX, l = 0.f;
+        seq = -1, lim = 0;
+        if (valid && t >= r.qb) {  // its sequence: the last at or after the run's whose rows begin at or before it
+          int x = r.s, y = a.S;
+          if (t < r.qe) y = x + 1;
+          while (y - x > 1) {
+            const int m = (x + y) >> 1;
+            if (a.qoff[m] <= t) x = m; else y = m;
+          }
+          seq = x, lim = own_limit(t, a.qoff[x + 1], a.lens[x]);
+        }
+        if (anyv) {  // the accumulator to zero; the last tile's was read by this very warp
+          const uint32_t z[16] = {};
+          __syncwarp();
+#pragma unroll 1
+          for (int c = 0; c < D / 2; c += 16) tmem_st16(ocol + c, z);
+          tmem_st_wait();
+          tc_fence_before();
+        }
+      }
+      const int rlim = !valid ? 0 : r.seg < 0 ? r.kend : seq == r.seg ? lim : 0;
+      const int nb = r.nb, kb = r.kb;
+      // the run's first blocks that every row here sees whole (lanes without a row have no say)
+      const int full = __reduce_min_sync(0xffffffffu, valid ? rlim : 0x7fffffff) / KB - kb;
+      for (int b = 0; b < nb; b++, g++) {
+        const int sb = g % SB;
+        if (!(ok = k.wait_warp(C::B_SF + sb, g / SB))) break;
+        const int nv = rlim - (kb + b) * KB;  // its keys that the row sees (or fewer than none, or more than there are)
+        const bool part = b >= full;
+        if (part ? __any_sync(0xffffffffu, nv > 0) : anyv) {
+          tc_fence_after();
+          const uint32_t scol = lrow + (uint32_t)(C::S_COL + sb * KB + hf * COLS);
+          float sc = a.scale_log2;
+          uint32_t x[32];
+          auto load = [&](int c) {  // 32 scores; minus infinity where the row does not see the key
+            __syncwarp();
+            tmem_ld32(scol + c, x);
+            tmem_ld_wait(x);
+            if (a.scale_log2 <= 0.f)  // the largest score is not the largest product: scale first
+#pragma unroll
+              for (int e = 0; e < 32; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * a.scale_log2);
+            if (part)
+#pragma unroll
+              for (int e = 0; e < 32; e++) x[e] = hf * COLS + c + e < nv ? x[e] : 0xff800000u;
+          };
+          if (sc <= 0.f) sc = 1.f;
+          float m2[2] = {__uint_as_float(0xff800000u), __uint_as_float(0xff800000u)};
+#pragma unroll 1
+          for (int c = 0; c < COLS; c += 32) {
+            load(c);
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              m2[0] = max3(m2[0], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+              m2[1] = max3(m2[1], __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+            }
+          }
+          const float pmx = fmaxf(m2[0], m2[1]) * sc;
+          const int par = meets & 1;
+          xch[(par * 2 + hf) * 128 + row] = pmx;
+          if (!(ok = meet())) break;
+          const float mx = fmaxf(pmx, xch[(par * 2 + (hf ^ 1)) * 128 + row]);
+          const bool grow = mx > ref + 8.0f;
+          const bool resc = grow && ref > -FLT_MAX;
+          if (__any_sync(0xffffffffu, resc)) {
+            // the products so far (with one scores' buffer they were done before this block's scores)
+            if (SB > 1 && !(ok = k.wait_warp(C::B_OR, g - 1))) break;
+            tc_fence_after();
+            const float f = resc ? ex2_approx(ref - mx) : 1.0f;
+            l *= f;
+#pragma unroll 1
+            for (int c = 0; c < D / 2; c += 16) {
+              uint32_t o[16];
+              __syncwarp();
+              tmem_ld16(ocol + c, o);
+              tmem_ld_wait(o);
+#pragma unroll
+              for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              __syncwarp();
+              tmem_st16(ocol + c, o);
+            }
+            tmem_st_wait();
+          }
+          if (grow) ref = mx;
+          const uint64_t ref2 = f32x2(7.0f - ref, 7.0f - ref), sc2 = f32x2(sc, sc);
+          uint64_t sum[2] = {0, 0};
+#pragma unroll 1
+          for (int c = 0; c < COLS; c += 32) {
+            if (COLS > 32) load(c);  // (one chunk of 32 is still in registers)
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 v = f32x2_split(fma_f32x2(f32x2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, ref2));
+              const float p0 = ex2_approx(v.x), p1 = ex2_approx(v.y);
+              sum[(e >> 1) & 1] = add_f32x2(sum[(e >> 1) & 1], f32x2(p0, p1));
+              const __half2 hp = __floats2half2_rn(p0, p1);
+              w[e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
+            }
+            // 32 weights over 16 of this warp's own scores, all done with
+            __syncwarp();
+            tmem_st16(scol + c / 2, w);
+          }
+          const float2 add = f32x2_split(add_f32x2(sum[0], sum[1]));
+          l += add.x + add.y;
+          tmem_st_wait();
+        }  // none of these rows sees the block: the product leaves them alone
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(k.bar(C::B_PF + sb));
+      }
+      if (!ok) break;
+      had = had || nb > 0;
+      if (r.flags & RUN_LAST) {
+        if (!(ok = k.wait_warp(C::B_OD, r.item))) break;
+        tc_fence_after();
+        const bool tlast = (r.flags & RUN_TLAST) != 0, direct = tfirst && tlast;
+        if (!direct && !a.by_row && tid == 0) {
+          if (tlast) a.head[blockIdx.x] = make_int4(r.tok0, r.ntok, r.kvh, 0);
+          if (tfirst) a.tail[blockIdx.x] = 1;
+        }
+        if (anyv) {
+          const int par = meets & 1;
+          xch[(par * 2 + hf) * 128 + row] = l;
+          if (!(ok = meet())) break;
+          float lt = l + xch[(par * 2 + (hf ^ 1)) * 128 + row];
+          if (had && valid && ((k.poison(r.item)[irow >> 5] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
+          const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
+          if (a.by_row && valid && jrow == 0 && hf == 0) {
+            if (tfirst) a.first[(long)r.kvh * a.T + t] = direct ? -1 : (int)blockIdx.x;
+            if (tlast) a.last[(long)r.kvh * a.T + t] = (int)blockIdx.x;
+          }
+          if (!direct && valid && hf == 0) a.ml[prow] = make_float2(ref, lt);
+          const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+          __half *y = a.Y + (long)t * a.ystride + (long)(r.kvh * a.r + jrow) * D + hf * (D / 2);
+          float *po = a.O + prow * D + hf * (D / 2);
+#pragma unroll 1
+          for (int c = 0; c < D / 2; c += 16) {
+            uint32_t o[16];
+            __syncwarp();
+            tmem_ld16(ocol + c, o);
+            tmem_ld_wait(o);
+            if (!valid) continue;
+            if (direct) {
+              uint32_t w[8];
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                const __half2 hv = __floats2half2_rn(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+                w[e] = *reinterpret_cast<const uint32_t *>(&hv);
+              }
+              *reinterpret_cast<uint4 *>(y + c) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4 *>(y + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            } else if (lt != 0.f) {
+              st_global_v8(po + c, o), st_global_v8(po + c + 8, o + 8);
+            }
+          }
+          __syncwarp();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(k.bar(C::B_OE));
+      }
+      k.done_run(n);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *k.abort()) a.hdr[0] = 1;  // a wait ran out: the records may be missing
+  if (warp == FW_M) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TCOLS);
+  }
+}
+
+template <int D>
+int launch(dc_ctx *ctx, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const PArgs &a) {
+  using C = FewCfg<D>;
+  static uint64_t attr_done = 0;
+  if (!(attr_done & (1ull << ctx->device))) {
+    DC_CUDA(cudaFuncSetAttribute(attention_paged_few_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    attr_done |= 1ull << ctx->device;
+  }
+  DC_CUDA(dc_launch_pdl(ctx->stream, attention_paged_few_kernel<D>, dim3(2 * ctx->sms), dim3(F_THREADS), C::SMEM, tq, tk, tv,
+                        a));
+  return dc_launch_check("attention_paged (few rows)");
+}
+
+}  // namespace
+
+// D = 64 or 128; two CTAs an SM. The caller launches the join.
+int attn_few_launch(dc_ctx *ctx, int D, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const PArgs &a) {
+  return D == 64 ? launch<64>(ctx, tq, tk, tv, a) : launch<128>(ctx, tq, tk, tv, a);
+}

@@ -34,35 +34,23 @@
 #include <algorithm>
 
 #include "dc_internal.h"
+#include "dc_paged.cuh"
 #include "dc_ptx.cuh"
 
 using namespace dcx;
+
+int attn_few_launch(dc_ctx *, int, const CUtensorMap &, const CUtensorMap &, const CUtensorMap &, const PArgs &);
 
 namespace {
 
 constexpr int PA_WG = 3, PA_SOFT = 4 * PA_WG;  // softmax warpgroups, warps
 constexpr int PA_WC = PA_SOFT, PA_WV = PA_SOFT + 1, PA_WM = PA_SOFT + 2, PA_WP = PA_SOFT + 3, PA_WK = PA_SOFT + 4;
 constexpr int PA_THREADS = (PA_SOFT + 5) * 32;
-constexpr int PA_RING = 4;
-constexpr int PA_GOFF = 512;  // groups whose offsets are kept in shared memory
-
-enum { RUN_FIRST = 1, RUN_LAST = 2, RUN_TFIRST = 4, RUN_TLAST = 8, RUN_END = 16 };
-
-// A run of blocks of one segment (the prefix or one sequence's own keys) for one tile.
-struct Run {
-  const int *tab;          // its page row
-  int tok0, ntok, kvh;     // the tile
-  int flags, item;
-  int seg;                 // sequence, or -1: the prefix
-  int s;                   // the sequence the run was found at
-  int kb, nb, kend;        // first block, blocks, keys of the segment that the tile's last row in it sees
-  int qb, qe, len;         // own runs: the sequence's rows and own keys
-};
 
 template <int D>
-struct PCfg {
+struct WideCfg {
   // keys per block; 64 at D = 256, whose tiles and accumulator leave room for no more
-  static constexpr int KB = D == 256 ? 64 : 128, NA = D / 64;
+  static constexpr int KB = D == 256 ? 64 : 128, NA = D / 64, Q_ROWS = 128, THREADS = PA_THREADS;
   static constexpr int KST = D == 64 ? 4 : D == 128 ? 3 : 2, VST = D == 64 ? 4 : 2;  // stages of the K and of the V ring
   static constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = KB * D * 2;
   static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + KST * KV_BYTES;
@@ -83,146 +71,19 @@ struct PCfg {
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
-struct PArgs {
-  __half *Y;
-  const int *table, *lens, *qoff, *ptable, *plens, *goff;
-  int *hdr;
-  int4 *head;  // by CTA: the tile that it ends and did not begin (first row, rows, kv head), or no rows
-  int *tail;   // by CTA: whether it begins a tile that it does not end
-  float2 *ml;
-  float *O;
-  uint32_t *err;
-  long ystride;
-  int tstride, pstride, S, G, T, heads, kv, r, tpt, page, pshift, pages, rows, chunk_min;
-  float scale_log2;
-};
-
-__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t lbo) {
-  // MN-major operand in 128-byte-swizzled {64, rows} boxes: 8-row groups 1024 bytes apart, 64-wide chunks `lbo` apart
-  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 | (uint64_t)(1024 >> 4) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-
-__device__ __forceinline__ void st_global_v8(float *p, const uint32_t *r) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
-
-// own keys that query row `t` of a sequence [.., qe) with `len` own tokens sees
-__device__ __forceinline__ int own_limit(int t, int qe, int len) { return max(len - (qe - 1 - t), 0); }
-template <int KB>
-__device__ __forceinline__ int blocks_of(int keys) { return (keys + KB - 1) / KB; }
-
-struct Groups {  // offsets, prefix lengths and first rows, from shared memory when they fit
-  const int *goff, *plens, *rows;
-  int G;
-  int2 whole;  // without groups: all rows
-  __device__ __forceinline__ int of(int s) const {  // the last g with goff[g] <= s
-    int lo = 0, hi = G;
-    while (hi - lo > 1) {
-      const int m = (lo + hi) >> 1;
-      if (goff[m] <= s) lo = m; else hi = m;
-    }
-    return lo;
-  }
-};
-
-struct Group {
-  int tg, te, pb;  // its rows, its prefix's blocks
-};
-template <int KB>
-__device__ __forceinline__ Group group_of(const PArgs &a, const Groups &gs, int g) {
-  if (gs.G == 0) return Group{gs.whole.x, gs.whole.y, 0};
-  const int pb = blocks_of<KB>(gs.plens[g]);
-  if (gs.rows) return Group{gs.rows[g], gs.rows[g + 1], pb};
-  return Group{a.qoff[min(max(gs.goff[g], 0), a.S)], a.qoff[min(max(gs.goff[g + 1], 0), a.S)], pb};
-}
-
-// The units of a sequence: for each tile its rows touch, the prefix's blocks if the tile starts in it, and its own.
-template <int KB>
-__device__ __noinline__ long seq_cost(int tpt, Group g, int qb, int qe, int len) {
-  long c = 0;
-  const int lo = qb - g.tg, hi = qe - g.tg;
-  if (hi <= lo) return 0;
-  for (int ts = lo / tpt * tpt; ts < hi; ts += tpt) {
-    if (ts >= lo) c += g.pb;
-    c += max(1, blocks_of<KB>(own_limit(g.tg + min(hi, ts + tpt) - 1, qe, len)));
-  }
-  return c;
-}
-
-// A run's blocks for a producer warp: page ids are read 32 at a time, the next 32 on their way, and turned into rows of
-// the cache as tensor-map coordinates before the stage is waited for.
-template <int D>
-struct Blocks {
-  static constexpr int NA = D / 64, KB = PCfg<D>::KB, NB = KB / 16;
-  const int *tab;
-  int base, count, cur, nxt, kend, kvh;
-  __device__ __forceinline__ int ld(const PArgs &a, int i) const {
-    int row = a.rows;  // past the cache: zeros
-    if (i < count) {
-      const int id = tab[i];
-      if (id >= 0 && id < a.pages)
-        row = (id * a.kv + kvh) << a.pshift;
-      else
-        atomicOr(a.err, (uint32_t)DC_DEVERR_BOUNDS);
-    }
-    return row;
-  }
-  __device__ __forceinline__ void start(const PArgs &a, const Run &r, int lane) {
-    tab = r.tab, kend = r.kend, kvh = r.kvh, count = (kend + a.page - 1) >> a.pshift, base = (r.kb * KB) >> a.pshift;
-    cur = ld(a, base + lane), nxt = ld(a, base + 32 + lane);
-  }
-  // The whole warp: block `kb`'s rows, one per box of min(page, 64) rows (boxes that hold none of the run's keys are
-  // left out).
-  struct Rows {
-    int row[NB], n, prow;
-  };
-  __device__ __forceinline__ Rows rows(const PArgs &a, int kb, int lane) {
-    Rows x;
-    const int pr = min(a.pshift, 6), key0 = kb * KB, i = key0 >> a.pshift, sub = a.pshift - pr;
-    x.prow = 1 << pr;
-    if (i - base >= 32) base += 32, cur = nxt, nxt = ld(a, base + 32 + lane);
-    x.n = min(KB >> pr, (kend - key0 + x.prow - 1) >> pr);
-    const int first = (key0 & (a.page - 1)) >> pr;  // the first box within its page
-#pragma unroll
-    for (int p = 0; p < NB; p++) {
-      const int at = first + p, v = __shfl_sync(0xffffffffu, cur, (i - base + (at >> sub)) & 31);
-      x.row[p] = v == a.rows ? v : v + ((at & ((1 << sub) - 1)) << pr);
-    }
-    return x;
-  }
-  // One thread.
-  __device__ __forceinline__ static void load(const CUtensorMap *map, const Rows &x, uint32_t dst, uint32_t full) {
-    mbar_expect_tx(full, (uint32_t)(x.n * NA * x.prow * 128));
-#pragma unroll
-    for (int p = 0; p < NB; p++) {
-      if (p >= x.n) break;
-#pragma unroll
-      for (int j = 0; j < NA; j++) tma_load_2d(dst + j * (KB * 128) + p * x.prow * 128, map, 64 * j, x.row[p], full);
-    }
-  }
-};
-
 template <int D>
 __global__ void __launch_bounds__(PA_THREADS, 1)
     attention_paged_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                            const __grid_constant__ CUtensorMap tmV, const PArgs a) {
-  using C = PCfg<D>;
-  constexpr int KB = C::KB, KST = C::KST, VST = C::VST, NA = C::NA;
+  using C = WideCfg<D>;
+  constexpr int KB = C::KB, KST = C::KST, VST = C::VST;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t sbase = smem_u32(smem);
-  auto bar = [&](int i) { return sbase + C::BAR_OFF + 8u * (uint32_t)i; };
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::MISC_OFF);
-  volatile int *abort = reinterpret_cast<volatile int *>(smem + C::MISC_OFF + 4);
-  int *s_start = reinterpret_cast<int *>(smem + C::MISC_OFF + 8);          // s, offset (low, high)
-  volatile uint32_t *poison = reinterpret_cast<volatile uint32_t *>(smem + C::POISON_OFF);  // [item % 4][4 words]
-  long *s_scan = reinterpret_cast<long *>(smem + C::SCAN_OFF);
-  Run *runs = reinterpret_cast<Run *>(smem + C::RUN_OFF);
-  int *s_goff = reinterpret_cast<int *>(smem + C::GOFF_OFF);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Cta<C> k(a, smem_raw);
+  uint8_t *smem = k.smem;
+  const uint32_t sbase = k.base;
+  auto bar = [&](int i) { return k.bar(i); };
+  const int tid = k.tid, warp = k.warp, lane = k.lane;
+  const Run *runs = k.runs();
 
   if (tid == 0) {
     for (int i = 0; i < C::NBARS; i++) {
@@ -233,7 +94,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                                                             : 1;
       mbar_init(bar(i), n);
     }
-    *abort = 0;
+    *k.abort() = 0;
     mbar_init_fence();
   }
   if (warp == PA_WK && lane == 0) tma_prefetch_desc(&tmQ), tma_prefetch_desc(&tmK);
@@ -241,269 +102,25 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   // Tensor memory is taken only when the kernels before are done, and the next kernel is let in only when every CTA
   // here has its own: of two kernels on an SM, neither can hold columns while it waits for the other.
   dc_pdl_wait();
-  if (warp == PA_WM) tmem_alloc(smem_u32(tmem_slot), C::TCOLS);
+  if (warp == PA_WM) tmem_alloc(smem_u32(k.tmem_slot()), C::TCOLS);
 
-  // ---- the line: units per sequence, their sum, this CTA's stretch
-  bool bad = false;
-  Groups gs{a.goff, a.plens, nullptr, a.G};
-  if (a.G > 0) {
-    if (a.G <= PA_GOFF) {  // offsets, prefix lengths and first rows into shared memory
-      for (int i = tid; i <= a.G; i += PA_THREADS) {
-        const int x = a.goff[i];
-        s_goff[i] = x;
-        s_goff[2 * (PA_GOFF + 4) + i] = a.qoff[min(max(x, 0), a.S)];
-        if (i < a.G) s_goff[PA_GOFF + 4 + i] = a.plens[i];
-      }
-      gs = Groups{s_goff, s_goff + PA_GOFF + 4, s_goff + 2 * (PA_GOFF + 4), a.G};
-    }
-  } else {
-    gs.whole = make_int2(a.qoff[0], a.qoff[a.S]);
-  }
-  const int per = (a.S + PA_THREADS - 1) / PA_THREADS;
-  const int sb = min(tid * per, a.S), se = min(sb + per, a.S);
-  int qb = 0, qe = 0, len = 0;  // the thread's (first) sequence
-  if (sb < se) qb = a.qoff[sb], qe = a.qoff[sb + 1], len = a.lens[sb];
-  __syncthreads();
-  dc_pdl_launch_dependents();
-  if (a.G > 0) {
-    for (int i = tid; i < a.G; i += PA_THREADS) {
-      const int x = gs.goff[i], y = gs.goff[i + 1], n = gs.plens[i];
-      bad |= x < 0 || y < x || y > a.S || n < 0 || n > (long)a.pstride * a.page || n > (1 << 30);
-    }
-    if (tid == 0) bad |= gs.goff[0] != 0 || gs.goff[a.G] != a.S;
-  }
-  // a sequence's units; nothing for offsets that are refused below (the sum is then not used)
-  auto units = [&](int s, int qb, int qe, int len) -> long {
-    if (qb < 0 || qe <= qb || qe > a.T || len < 0) return 0;
-    const Group g = group_of<KB>(a, gs, a.G ? gs.of(s) : 0);
-    return g.tg < 0 || g.tg > qb ? 0 : seq_cost<KB>(a.tpt, g, qb, qe, len);
-  };
-  long mine = 0;
-  for (int s = sb; s < se; s++) {
-    const int x = s == sb ? qb : a.qoff[s], y = s == sb ? qe : a.qoff[s + 1], n = s == sb ? len : a.lens[s];
-    bad |= x < 0 || y < x || y > a.T || n < 0 || n > (long)a.tstride * a.page || n > (1 << 30);
-    mine += units(s, x, y, n);
-  }
-  long incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) s_scan[warp] = incl;
-  if (__syncthreads_or(bad)) {  // the same in every CTA
-    if (blockIdx.x == 0 && tid == 0) a.hdr[0] = 1, atomicOr(a.err, (uint32_t)DC_DEVERR_BOUNDS);
-    tc_fence_before();
-    __syncthreads();
-    if (warp == PA_WM) tc_fence_after(), tmem_dealloc(*tmem_slot, C::TCOLS);
-    return;
-  }
-  if (tid == 0) {
-    if (blockIdx.x == 0) a.hdr[0] = 0;
-    a.head[blockIdx.x] = make_int4(0, 0, 0, 0), a.tail[blockIdx.x] = 0;
-  }
-  long before = incl - mine, line = 0;
-#pragma unroll
-  for (int w = 0; w < PA_THREADS / 32; w++) {
-    const long v = s_scan[w];
-    if (w < warp) before += v;
-    line += v;
-  }
-  const long B = line * a.kv;
-  long chunk, p0;
-  int kvh0 = 0;
-  if (B < 0x7fff0000) {  // (64-bit divisions take a microsecond)
-    chunk = max((unsigned)a.chunk_min, ((unsigned)B + gridDim.x - 1) / gridDim.x);
-    p0 = chunk * blockIdx.x;
-    if (p0 < B) kvh0 = (unsigned)p0 / (unsigned)line;
-  } else {
-    chunk = (B + gridDim.x - 1) / gridDim.x, p0 = chunk * blockIdx.x;
-    if (p0 < B) kvh0 = (int)(p0 / line);
-  }
-  const long p1 = min(p0 + chunk, B);
-  const bool work = p0 < p1;
-  if (work && mine > 0) {
-    long off = p0 - kvh0 * line - before;
-    if (off >= 0 && off < mine) {
-      int s = sb;
-      for (; s < se - 1; s++) {
-        const long c = units(s, a.qoff[s], a.qoff[s + 1], a.lens[s]);
-        if (off < c) break;
-        off -= c;
-      }
-      s_start[0] = s, s_start[1] = (int)(uint32_t)off, s_start[2] = (int)(off >> 32);
-    }
-  }
+  Groups gs;
+  Stretch st;
+  const bool fine = line_start(k, gs, st);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = *k.tmem_slot();
 
-  auto wait = [&](int i, int parity) {
-    return mbar_wait_asleep(bar(i), (uint32_t)parity & 1u, abort, a.err, DC_DEVERR_ATTN_WAIT);
-  };
-  // the whole warp waits, and goes on or gives up together
-  auto wait_warp = [&](int i, int parity) { return __all_sync(0xffffffffu, wait(i, parity)) != 0; };
-  auto wait1 = [&](int i, int parity) {  // one thread that issues products
-    return mbar_wait_alert(bar(i), (uint32_t)parity & 1u, abort, a.err, DC_DEVERR_ATTN_WAIT);
-  };
-  // a consumer's next run: false at the end (or on abort)
-  auto next_run = [&](int n, Run &r) -> bool {
-    if (!wait_warp(C::B_IF + n % PA_RING, n / PA_RING)) return false;
-    r = runs[n % PA_RING];
-    return !(r.flags & RUN_END);
-  };
-  auto done_run = [&](int n) {
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar(C::B_IE + n % PA_RING));
-  };
-
-  if (!work) {
+  auto wait_warp = [&](int i, int parity) { return k.wait_warp(i, parity); };
+  auto wait1 = [&](int i, int parity) { return k.wait1(i, parity); };
+  if (!fine || st.p0 >= st.p1) {
   } else if (warp == PA_WK) {
-    int g = 0, item = -1, n = 0;  // blocks, tiles, runs
-    bool ok = true, first = true;
-    long pos = p0, off = (long)(uint32_t)s_start[1] | (long)s_start[2] << 32;  // on the line; in the piece
-    int s = s_start[0], kvh = kvh0, ts = -1;                                     // ts: the piece's tile, from the group's first row
-    while (pos < p1 && kvh < a.kv) {
-      Run r;
-      r.s = s, r.qb = a.qoff[s], r.qe = a.qoff[s + 1], r.len = a.lens[s];
-      const int gi = a.G ? gs.of(s) : 0;
-      const Group gr = group_of<KB>(a, gs, gi);
-      const int lo = r.qb - gr.tg, hi = r.qe - gr.tg, rows = gr.te - gr.tg;
-      if (ts < 0) ts = lo / a.tpt * a.tpt;
-      if (hi <= lo || ts >= hi) {  // the next sequence
-        ts = -1;
-        if (++s == a.S) s = 0, kvh++;
-        continue;
-      }
-      const int pe = min(hi, ts + a.tpt);
-      const bool starts = ts >= lo, ends = pe == min(rows, ts + a.tpt);
-      const int pc = starts ? gr.pb : 0, lim = own_limit(gr.tg + pe - 1, r.qe, r.len), all = pc + max(1, blocks_of<KB>(lim));
-      if (off >= all) {  // the next piece of the sequence
-        off -= all, ts += a.tpt;
-        continue;
-      }
-      const bool prefix = off < pc;
-      const int units = (int)min((prefix ? pc : all) - off, p1 - pos);
-      const bool done = off + units == all && ends;
-      r.tok0 = gr.tg + ts, r.ntok = min(rows - ts, a.tpt), r.kvh = kvh;
-      r.tab = prefix ? a.ptable + (long)gi * a.pstride : a.table + (long)s * a.tstride;
-      r.seg = prefix ? -1 : s, r.kend = prefix ? gs.plens[gi] : lim;
-      r.kb = (int)(prefix ? off : off - pc), r.nb = r.kend > 0 ? units : 0;
-      r.flags = (first ? RUN_FIRST : 0) | (off == 0 && starts ? RUN_TFIRST : 0) |
-                (done || pos + units == p1 ? RUN_LAST : 0) | (done ? RUN_TLAST : 0);
-      pos += units, off += units;
-      if (r.nb == 0 && !(r.flags & (RUN_FIRST | RUN_LAST))) continue;  // (a run in a tile's midst always has blocks)
-      if (first) item++;
-      r.item = item;
-      if (!(ok = wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1))) break;
-      if (lane == 0) {
-        runs[n % PA_RING] = r;
-        mbar_arrive(bar(C::B_IF + n % PA_RING));
-      }
-      n++;
-      __syncwarp();
-      Blocks<D> bl;
-      bl.start(a, r, lane);
-      if (first) {
-        if (!(ok = wait_warp(C::B_QE, item + 1))) break;
-        if (elect_one()) {
-          mbar_expect_tx(bar(C::B_QF), (uint32_t)(a.r * a.tpt * 128 * NA));
-          for (int j = 0; j < NA; j++)
-            tma_load_3d(sbase + j * 128 * 128, &tmQ, 64 * j, r.kvh * a.r, r.tok0, bar(C::B_QF));
-        }
-        __syncwarp();
-      }
-      for (int b = 0; b < r.nb; b++, g++) {
-        const int st = g % KST;
-        const typename Blocks<D>::Rows x = bl.rows(a, r.kb + b, lane);
-        if (!(ok = wait_warp(C::B_KE + st, g / KST + 1))) break;
-        if (elect_one()) bl.load(&tmK, x, sbase + C::K_OFF + st * C::KV_BYTES, bar(C::B_KF + st));
-        __syncwarp();
-      }
-      if (!ok) break;
-      first = (r.flags & RUN_LAST) != 0;
-    }
-    if (ok && wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1) && lane == 0) {
-      runs[n % PA_RING].flags = RUN_END;
-      mbar_arrive(bar(C::B_IF + n % PA_RING));
-    }
+    walk_line(k, gs, st, &tmQ, &tmK);
   } else if (warp == PA_WV) {
-    Run r;
-    int g = 0;
-    bool ok = true;
-    for (int n = 0; ok && next_run(n, r); n++) {
-      if (r.nb > 0) {
-        Blocks<D> bl;
-        bl.start(a, r, lane);
-        for (int b = 0; b < r.nb; b++, g++) {
-          const int st = g % VST;
-          const typename Blocks<D>::Rows x = bl.rows(a, r.kb + b, lane);
-          if (!(ok = wait_warp(C::B_VE + st, g / VST + 1))) break;
-          if (elect_one()) bl.load(&tmV, x, sbase + C::V_OFF + st * C::KV_BYTES, bar(C::B_VF + st));
-          __syncwarp();
-        }
-      }
-      if (ok) done_run(n);
-    }
+    load_values(k, &tmV);
   } else if (warp == PA_WC) {
-    Run r;
-    int g = 0;
-    bool ok = true;
-    for (int n = 0; ok && next_run(n, r); n++) {
-      volatile uint32_t *mark = poison + 4 * (r.item & 3);
-      if ((r.flags & RUN_FIRST) && lane < 4) mark[lane] = 0;
-      __syncwarp();
-      for (int b = 0; b < r.nb; b++, g++) {
-        const int st = g % VST;
-        if (!(ok = wait_warp(C::B_VF + st, g / VST))) break;
-        const int key0 = (r.kb + b) * KB, valid = min(KB, r.kend - key0), pad = (valid + 15) & ~15;
-        uint8_t *v = smem + C::V_OFF + st * C::KV_BYTES + (lane & 7) * 16;
-        if (valid < pad) {  // up to 15 rows, four at a time
-          for (int row = valid + lane / 8; row < pad; row += 4)
-#pragma unroll
-            for (int at = 0; at < NA; at++) *reinterpret_cast<uint4 *>(v + at * (KB * 128) + row * 128) = make_uint4(0, 0, 0, 0);
-        }
-        // the first row of the tile that sees the block sees the fewest of its keys
-        const int t1 = max(max(r.tok0, r.qb), key0 - r.len + r.qe);
-        const bool scan = r.seg >= 0 && own_limit(t1, r.qe, r.len) < key0 + valid;
-        if (scan) {
-          int worst = KB;  // the first row with a value that is not finite
-#pragma unroll 1
-          for (int at = 0; at < NA; at++) {
-#pragma unroll 1
-            for (int i0 = 0; 4 * i0 < valid; i0 += 8) {
-              uint4 x[8];
-#pragma unroll
-              for (int i = 0; i < 8; i++)
-                x[i] = *reinterpret_cast<uint4 *>(v + at * (KB * 128) + (4 * (i0 + i) + lane / 8) * 128);
-#pragma unroll
-              for (int i = 0; i < 8; i++) {
-                const int row = 4 * (i0 + i) + lane / 8;
-                auto big = [](uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; };
-                if (row < valid && (big(x[i].x) | big(x[i].y) | big(x[i].z) | big(x[i].w))) {
-                  *reinterpret_cast<uint4 *>(v + at * (KB * 128) + row * 128) = make_uint4(0, 0, 0, 0);
-                  worst = min(worst, row);
-                }
-              }
-            }
-          }
-          worst = __reduce_min_sync(0xffffffffu, worst);
-          if (worst < KB && lane < 4) {
-            // rows of the sequence in this tile that see key key0 + worst
-            const int from = max(max(r.tok0, r.qb), key0 + worst - r.len + r.qe) - r.tok0;
-            const int to = min(r.qe, r.tok0 + r.ntok) - r.tok0;
-            const int x = min(max(from - 32 * lane, 0), 32), y = min(max(to - 32 * lane, 0), 32);
-            const uint32_t upto = y >= 32 ? ~0u : (1u << y) - 1u, under = x >= 32 ? ~0u : (1u << x) - 1u;
-            if (y > x) mark[lane] |= upto & ~under;
-          }
-        }
-        if (scan || valid < pad) fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::B_VS + st));
-      }
-      if (ok) done_run(n);
-    }
+    look_over(k);
   } else if (warp == PA_WM) {
     // Q K^T, one thread: a block's scores go to the buffer of the warpgroup that takes it, free since the P V of the
     // block PA_WG before
@@ -555,11 +172,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             const int lo = (max(max(r.tok0, r.qb), key0 - r.len + r.qe) - r.tok0) * a.r;
             const int hi = (min(r.qe, r.tok0 + r.ntok) - r.tok0) * a.r;
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
-              const int x = min(max(lo - 32 * w, 0), 32), y = min(max(hi - 32 * w, 0), 32);
-              const uint32_t upto = y >= 32 ? ~0u : (1u << y) - 1u, under = x >= 32 ? ~0u : (1u << x) - 1u;
-              off[w] = ~(upto & ~under);
-            }
+            for (int w = 0; w < 4; w++) off[w] = ~mask_word(lo, hi, w);
           }
           if (!(ok = wait1(C::B_VS + st, g / VST) && wait1(C::B_PF + sb, g / PA_WG))) break;  // (VS: after VF)
           tc_fence_after();
@@ -736,7 +349,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         if (!(ok = wait_warp(C::B_OD, r.item))) break;
         tc_fence_after();
         const bool tlast = (r.flags & RUN_TLAST) != 0, direct = tfirst && tlast;
-        if (!direct && warp == 0 && lane == 0) {
+        if (!direct && !a.by_row && tid == 0) {
           if (tlast) a.head[blockIdx.x] = make_int4(r.tok0, r.ntok, r.kvh, 0);
           if (tfirst) a.tail[blockIdx.x] = 1;
         }
@@ -751,8 +364,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           float lt = 0.f;
 #pragma unroll
           for (int w = 0; w < PA_WG; w++) lt += sums[w * 128 + row];
-          if (had && valid && ((poison[4 * (r.item & 3) + (irow >> 5)] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
+          if (had && valid && ((k.poison(r.item)[irow >> 5] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
           const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
+          if (a.by_row && valid && jrow == 0 && wg == 0) {
+            if (tfirst) a.first[(long)r.kvh * a.T + t] = direct ? -1 : (int)blockIdx.x;
+            if (tlast) a.last[(long)r.kvh * a.T + t] = (int)blockIdx.x;
+          }
           if (!direct && valid && wg == 0) a.ml[prow] = make_float2(fin, lt);
           const float inv = lt == 0.f ? 0.f : 1.0f / lt;
           __half *y = a.Y + (long)t * a.ystride + (long)(r.kvh * a.r + jrow) * D;
@@ -780,13 +397,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
         zero();
       }
-      done_run(n);
+      k.done_run(n);
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *abort) a.hdr[0] = 1;  // a wait ran out: the records may be missing
+  if (tid == 0 && *k.abort()) a.hdr[0] = 1;  // a wait ran out: the records may be missing
   if (warp == PA_WM) {
     tc_fence_after();
     tmem_dealloc(tmem, C::TCOLS);
@@ -794,29 +411,45 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 }
 
 // Joins the parts of the tiles that were cut: y = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over the CTAs c from the
-// tile's first to its last, in that order. A block takes four rows of the tile that CTA blockIdx.y ends, a warp each.
-template <int D>
+// tile's first to its last. W = 4, for few rows in many parts: a block to a (row, head), each warp every fourth part,
+// joined in order of the warps. W = 1, for many rows, most of them whole or cut once: blockIdx.y is the CTA that ends a
+// cut tile, a block takes four rows of it.
+template <int D, int W>
 __global__ void __launch_bounds__(128) attention_join_kernel(const PArgs a) {
   dc_pdl_begin();
   constexpr int N = D / 32;  // a lane's values
-  const int lane = threadIdx.x & 31, row = blockIdx.x * 4 + (threadIdx.x >> 5), c1 = blockIdx.y;
+  __shared__ float s_o[W][W > 1 ? D : 1], s_m[W], s_l[W];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = W > 1 ? warp : 0;
   const int refused = a.hdr[0];  // (a refused call, or one whose waits ran out, has no records)
-  const int4 tile = a.head[c1];
-  if (refused || row >= tile.y * a.r) return;
-  int c0 = -1;  // the last CTA before that begins a tile and does not end it
-  for (int e = c1; e > 0 && c0 < 0; e -= 32) {
-    const int c = e - 1 - lane;
-    const uint32_t at = __ballot_sync(0xffffffffu, c >= 0 && a.tail[c] != 0);
-    if (at) c0 = e - __ffs(at);
+  int c0 = -1, c1;
+  long t, base;  // part c of the row: row base + 128 c
+  int h;
+  if (W > 1) {
+    t = blockIdx.x / a.heads, h = blockIdx.x - (int)t * a.heads;
+    const int kvh = h / a.r;
+    const int t0 = a.qoff[0], t1 = a.qoff[a.S];
+    c0 = a.first[(long)kvh * a.T + t], c1 = a.last[(long)kvh * a.T + t];
+    if (refused || t < t0 || t >= t1 || c0 < 0 || c1 < c0 || c1 >= a.ctas) return;
+    base = ((long)kvh * a.T + t) * a.r + h - kvh * a.r;
+  } else {
+    const int row = blockIdx.x * 4 + warp;
+    c1 = blockIdx.y;
+    const int4 tile = a.head[c1];
+    if (refused || row >= tile.y * a.r) return;
+    for (int e = c1; e > 0 && c0 < 0; e -= 32) {  // the last CTA before that begins a tile and does not end it
+      const int c = e - 1 - lane;
+      const uint32_t at = __ballot_sync(0xffffffffu, c >= 0 && a.tail[c] != 0);
+      if (at) c0 = e - __ffs(at);
+    }
+    if (c0 < 0) return;
+    const int i = row / a.r;
+    t = tile.x + i, h = tile.z * a.r + row - i * a.r;
+    base = ((long)tile.z * a.T + tile.x) * a.r + row;
   }
-  if (c0 < 0) return;
-  const int i = row / a.r, j = row - i * a.r;
-  const long base = ((long)tile.z * a.T + tile.x) * a.r + row;  // part c of this row: row base + 128 c
   float M = -FLT_MAX, L = 0.f, o[N] = {};
-  for (int cb = c0; cb <= c1; cb += 32) {  // 32 parts at a time, usually all
-    const int c = cb + lane;
+  for (int cb = c0 + part; cb <= c1; cb += 32 * W) {  // 32 parts at a time, usually all
+    const int c = cb + W * lane;
     const float2 x = c <= c1 ? a.ml[base + 128L * c] : make_float2(-FLT_MAX, 0.f);
-    const int cnt = min(32, c1 - cb + 1);
     float m = x.y == 0.f ? -FLT_MAX : x.x;  // a part of weight 0 stored no values
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
@@ -827,32 +460,58 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PArgs a) {
     L = L * f + (x.y == 0.f ? 0.f : w * x.y);
 #pragma unroll
     for (int e = 0; e < N; e++) o[e] *= f;
-    const uint32_t have = __ballot_sync(0xffffffffu, x.y != 0.f);
-    for (int k0 = 0; k0 < cnt; k0 += 8) {  // eight parts' values on their way
-      float v[8][N];
+    uint32_t have = __ballot_sync(0xffffffffu, x.y != 0.f);
+    while (have) {  // four parts' values on their way
+      float v[4][N], wk[4];
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const float *p = a.O + (base + 128L * (cb + min(k0 + k, cnt - 1))) * D + N * lane;
-        if (N == 2) {
-          *reinterpret_cast<float2 *>(v[k]) = *reinterpret_cast<const float2 *>(p);
-        } else {
+      for (int k = 0; k < 4; k++) {
+        const int at = have ? __ffs(have) - 1 : 0;
+        const float *p = a.O + (base + 128L * (cb + W * at)) * D + N * lane;
+        wk[k] = __shfl_sync(0xffffffffu, w, at);
 #pragma unroll
-          for (int e = 0; e < N; e += 4) *reinterpret_cast<float4 *>(v[k] + e) = *reinterpret_cast<const float4 *>(p + e);
+        for (int e = 0; e < N; e++) v[k][e] = 0.f;
+        if (have) {
+          if (N == 2) {
+            *reinterpret_cast<float2 *>(v[k]) = *reinterpret_cast<const float2 *>(p);
+          } else {
+#pragma unroll
+            for (int e = 0; e < N; e += 4) *reinterpret_cast<float4 *>(v[k] + e) = *reinterpret_cast<const float4 *>(p + e);
+          }
         }
+        have &= have - 1;
       }
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const float wk = __shfl_sync(0xffffffffu, w, (k0 + k) & 31);
-        const bool use = k0 + k < cnt && ((have >> (k0 + k)) & 1u);
+      for (int k = 0; k < 4; k++)
 #pragma unroll
-        for (int e = 0; e < N; e++) o[e] = use ? fmaf(wk, v[k][e], o[e]) : o[e];
-      }
+        for (int e = 0; e < N; e++) o[e] = fmaf(wk[k], v[k][e], o[e]);
     }
   }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) L += __shfl_xor_sync(0xffffffffu, L, s);
+  if (W > 1) {
+    if (lane == 0) s_m[warp] = M, s_l[warp] = L;
+    __syncthreads();
+    float all = -FLT_MAX;
+#pragma unroll
+    for (int w = 0; w < W; w++) all = s_l[w] != 0.f ? fmaxf(all, s_m[w]) : all;
+    const float f = s_l[warp] != 0.f ? ex2_approx(M - all) : 0.f;
+#pragma unroll
+    for (int e = 0; e < N; e++) s_o[warp][N * lane + e] = s_l[warp] != 0.f ? o[e] * f : 0.f;
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; w++)
+      if (s_l[w] != 0.f) L += s_l[w] * ex2_approx(s_m[w] - all);
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      o[e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; w++) o[e] += s_o[w][N * lane + e];
+    }
+  }
   const float inv = L == 0.f ? 0.f : 1.0f / L;
-  __half *y = a.Y + (long)(tile.x + i) * a.ystride + (long)(tile.z * a.r + j) * D + N * lane;
+  __half *y = a.Y + t * a.ystride + (long)h * D + N * lane;
 #pragma unroll
   for (int e = 0; e < N; e += 2)
     *reinterpret_cast<__half2 *>(y + e) = __floats2half2_rn(o[e] * inv, o[e + 1] * inv);
@@ -883,16 +542,18 @@ int encode(CUtensorMap *m, const void *p, int rank, const cuuint64_t *dims, cons
 
 size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// The workspace: a status word, the CTAs' records, parts' maxima and sums, parts' sums of values. Part c of a tile
+// The workspace: a status word, the join's records, parts' maxima and sums, parts' sums of values. Part c of a tile
 // starts at row (kvh T + first row) r + 128 c: along the line either the tile moves on, by at least its rows, or c does,
 // so no two parts meet.
 struct Ws {
-  size_t head, tail, ml, O, bytes;
+  size_t first, last, head, tail, ml, O, bytes;
 };
-Ws ws_layout(int T, int heads, int D, int ctas) {
+Ws ws_layout(int T, int heads, int kv, int D, int ctas) {
   Ws w;
   const size_t rows = (size_t)T * heads + 128 * (size_t)(ctas + 1);
-  w.head = 256;
+  w.first = 256;
+  w.last = w.first + up((size_t)T * kv * 4);
+  w.head = w.last + up((size_t)T * kv * 4);
   w.tail = w.head + up((size_t)ctas * 16);
   w.ml = w.tail + up((size_t)ctas * 4);
   w.O = w.ml + up(rows * 8);
@@ -900,26 +561,35 @@ Ws ws_layout(int T, int heads, int D, int ctas) {
   return w;
 }
 
+bool paged_few(int D, int T, int r, int G) { return D <= 128 && (long)T * r <= 128L * std::max(G, 1); }
+
 template <int D>
-int launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, const PArgs &a) {
-  using C = PCfg<D>;
+int launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, PArgs a, bool few) {
+  using C = WideCfg<D>;
   CUtensorMap tq;
   const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)a.heads, (cuuint64_t)a.T};
   const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)qs * 2};
   const cuuint32_t box[3] = {64, (cuuint32_t)a.r, (cuuint32_t)a.tpt};
   int rc = encode(&tq, Q, 3, dims, strides, box);
   if (rc) return rc;
-  static uint64_t attr_done = 0;
-  if (!(attr_done & (1ull << ctx->device))) {
-    DC_CUDA(cudaFuncSetAttribute(attention_paged_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    attr_done |= 1ull << ctx->device;
+  if (few) {
+    rc = attn_few_launch(ctx, D, tq, c->mapK, c->mapV, a);
+  } else {
+    static uint64_t attr_done = 0;
+    if (!(attr_done & (1ull << ctx->device))) {
+      DC_CUDA(cudaFuncSetAttribute(attention_paged_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+      attr_done |= 1ull << ctx->device;
+    }
+    DC_CUDA(dc_launch_pdl(ctx->stream, attention_paged_kernel<D>, dim3(ctx->sms), dim3(PA_THREADS), C::SMEM, tq, c->mapK,
+                          c->mapV, a));
+    rc = dc_launch_check("attention_paged");
   }
-  DC_CUDA(dc_launch_pdl(ctx->stream, attention_paged_kernel<D>, dim3(ctx->sms), dim3(PA_THREADS), C::SMEM, tq,
-                        c->mapK, c->mapV, a));
-  rc = dc_launch_check("attention_paged");
   if (rc) return rc;
-  const dim3 grid((std::min((long)a.T * a.r, 128L) + 3) / 4, ctx->sms);
-  DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D>, grid, dim3(128), 0, a));
+  if (a.by_row)
+    DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D, 4>, dim3((unsigned)((long)a.T * a.heads)), dim3(128), 0, a));
+  else
+    DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D, 1>, dim3((unsigned)((std::min((long)a.T * a.r, 128L) + 3) / 4), a.ctas),
+                          dim3(128), 0, a));
   return dc_launch_check("attention_paged (join)");
 }
 
@@ -934,27 +604,34 @@ int attn_cache_maps(dc_kv_cache *c) {
 }
 
 size_t attn_paged_ws(dc_ctx *ctx, const dc_kv_cache *c, int T, int heads) {
-  return ws_layout(T, heads, c->D, ctx->sms).bytes;
+  return ws_layout(T, heads, c->kv, c->D, 2 * ctx->sms).bytes;
 }
 
 int attn_paged_launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, const int *table, int tstride,
                       const int *lens, const int *qoff, int S, const int *ptable, int pstride, const int *plens,
                       const int *goff, int G, void *Y, long ys, int T, int heads, float scale, void *ws) {
-  const Ws w = ws_layout(T, heads, c->D, ctx->sms);
+  const Ws w = ws_layout(T, heads, c->kv, c->D, 2 * ctx->sms);
   char *p = static_cast<char *>(ws);
   PArgs a;
   a.Y = static_cast<__half *>(Y), a.ystride = ys;
   a.table = table, a.lens = lens, a.qoff = qoff, a.ptable = ptable, a.plens = plens, a.goff = goff;
+  a.first = reinterpret_cast<int *>(p + w.first), a.last = reinterpret_cast<int *>(p + w.last);
   a.hdr = reinterpret_cast<int *>(p), a.head = reinterpret_cast<int4 *>(p + w.head);
   a.tail = reinterpret_cast<int *>(p + w.tail), a.ml = reinterpret_cast<float2 *>(p + w.ml);
   a.O = reinterpret_cast<float *>(p + w.O);
   a.err = ctx->d_err;
   a.tstride = tstride, a.pstride = pstride, a.S = S, a.G = G, a.T = T, a.heads = heads, a.kv = c->kv;
-  a.r = heads / c->kv, a.tpt = 128 / a.r, a.page = c->page, a.pages = c->pages;
+  a.r = heads / c->kv;
+  const bool few = paged_few(c->D, T, a.r, G);
+  const int ctas = few ? 2 * ctx->sms : ctx->sms;
+  a.tpt = 128 / a.r, a.page = c->page, a.pages = c->pages;
   a.pshift = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7, a.rows = c->pages * c->kv * c->page;
   a.chunk_min = 2;
+  a.ctas = ctas;
+  // few rows: most tiles are cut, into many parts
+  a.by_row = (long)T * heads <= 8192;
   a.scale_log2 = scale * 1.4426950408889634f;
-  if (c->D == 64) return launch<64>(ctx, c, Q, qs, a);
-  if (c->D == 128) return launch<128>(ctx, c, Q, qs, a);
-  return launch<256>(ctx, c, Q, qs, a);
+  if (c->D == 64) return launch<64>(ctx, c, Q, qs, a, few);
+  if (c->D == 128) return launch<128>(ctx, c, Q, qs, a, few);
+  return launch<256>(ctx, c, Q, qs, a, few);
 }
