@@ -629,7 +629,7 @@ int attn_paged_launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs,
   a.chunk_min = 2;
   a.ctas = ctas;
   // few rows: most tiles are cut, into many parts
-  a.by_row = (long)T * heads <= 8192;
+  a.by_row = few && (long)T * heads <= 8192;
   a.scale_log2 = scale * 1.4426950408889634f;
   if (c->D == 64) return launch<64>(ctx, c, Q, qs, a, few);
   if (c->D == 128) return launch<128>(ctx, c, Q, qs, a, few);

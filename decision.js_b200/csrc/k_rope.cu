@@ -4,8 +4,9 @@
 //   (a, b) -> f (a cos - b sin, b cos + a sin).
 // The angle is kept as a fraction of a turn in 64-bit fixed point: a plan holds w_i / 2 pi as a 64-bit fraction, and
 // p times it modulo 2^64 is the fraction of a turn left after the whole ones, with no rounding at all. A 32-bit
-// product p w_i would be off by 2^-24 of itself: 0.06 rad at a million radians. What is left is a number in [-1, 1)
-// half turns, which sincospif takes as it is.
+// product p w_i would be off by 2^-24 of itself: 0.06 rad at a million radians. What is left is an angle in [-pi, pi),
+// where the hardware's sine and cosine are off by 2^-20.9 at most: 1/500 of the rounding of the result to f16 (for a pair
+// of equal size; sincospif's 24 bits cost 300 instructions a lane and token, a sixth of the append).
 //
 // Both kernels read and write each row once and are bound by memory (many tokens) or by the launch (few).
 #include <cuda_fp16.h>
@@ -49,9 +50,8 @@ __device__ __forceinline__ void angles8(const uint64_t *freq, int p, float facto
 #pragma unroll
   for (int e = 0; e < 8; e++) {
     const uint64_t turn = (uint64_t)(int64_t)p * f[e];  // modulo one turn
-    const float half_turns = (float)(int)(turn >> 32) * 0x1p-31f;
     float s, c;
-    sincospif(half_turns, &s, &c);
+    __sincosf((float)(int)(turn >> 32) * 1.4629180792671596e-9f, &s, &c);  // pi 2^-31
     cs[e] = c * factor, sn[e] = s * factor;
   }
 }
@@ -101,7 +101,6 @@ __global__ void __launch_bounds__(256) rope_kernel(const __half *X, long xs, con
   const bool turn = u < rot / 16;
   if (!turn && X == Y) return;
   float cs[8], sn[8];
-  if (turn) angles8(freq + 8 * u, pos[t], factor, cs, sn);
   constexpr int NB = 4;  // heads in flight
   for (int h0 = hs; h0 < heads; h0 += NB * HS) {
     uint4 ra[NB], rb[NB];
@@ -110,6 +109,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const __half *X, long xs, con
       const int h = h0 + i * HS;
       if (h < heads) ra[i] = ld16(x + (long)h * D + 8 * ch.x), rb[i] = ld16(x + (long)h * D + 8 * ch.y);
     }
+    if (turn && h0 == hs) angles8(freq + 8 * u, pos[t], factor, cs, sn);  // while the first heads are on their way
 #pragma unroll
     for (int i = 0; i < NB; i++) {
       const int h = h0 + i * HS;
@@ -133,66 +133,86 @@ struct AppendArgs {
   const uint64_t *freq;
   uint32_t *err;
   long zs, qs;
-  int T, heads, kv, rot, page, nslots, vnorm, W;
+  int T, heads, kv, rot, page, pshift, nslots, vnorm, W;
   float eps, factor;
 };
 
 // W warps per token; a pass of a warp covers 32 / (D/16) of the token's q, k and v heads, U = D/16 lanes to a head
-// (one unit each), NP passes with their loads in flight.
+// (one unit each). NP passes are loaded at a time, the next NP while these are worked on.
 template <int D, bool INTER>
-__global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, 2) kv_append_kernel(const AppendArgs a) {
   dc_pdl_begin();
   constexpr int U = D / 16, HPP = 32 / U, NP = 4;
+  __shared__ __align__(16) float weights[2][D];  // the norms', in f32: converted once, not in every pass
   const long wid = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const long t = wid / a.W;
-  if (t >= a.T) return;  // the whole warp
-  const int wsub = (int)(wid % a.W);
+  const bool live = t < a.T;  // the whole warp
+  const int wsub = (int)(wid - t * a.W);
   const int lane = threadIdx.x & 31, u = lane % U, sub = lane / U;
   const int per = a.heads + 2 * a.kv, npass = (per + HPP - 1) / HPP;
   const int2 ch = unit_chunks<INTER>(u, a.rot);
-  const bool turn = u < a.rot / 16;
   const __half *z = a.Z + t * a.zs;
-  const int slot = a.slots[t];
-  const bool stored = slot >= 0 && slot < a.nslots;
-  if (slot >= a.nslots && lane == 0) atomicOr(a.err, (uint32_t)DC_DEVERR_BOUNDS);
-  const int pg = slot / a.page, off = slot % a.page;
-  float cs[8], sn[8];
-  uint4 wq[2] = {}, wk[2] = {};
-  if (a.qn) wq[0] = ld16(a.qn + 8 * ch.x), wq[1] = ld16(a.qn + 8 * ch.y);
-  if (a.kn) wk[0] = ld16(a.kn + 8 * ch.x), wk[1] = ld16(a.kn + 8 * ch.y);
-  if (turn) angles8(a.freq + 8 * u, a.pos[t], a.factor, cs, sn);
-  for (int p0 = wsub; p0 < npass; p0 += NP * a.W) {
-    uint4 ra[NP], rb[NP];
+  const int slot = live ? a.slots[t] : -1, pos = live && a.pos ? a.pos[t] : 0;
+  uint4 ra[NP], rb[NP];
+  // q heads are always loaded, k and v heads with them: the slot is not known yet
+  auto load = [&](int p0) {
 #pragma unroll
     for (int i = 0; i < NP; i++) {
       const int h = (p0 + i * a.W) * HPP + sub;
-      const bool live = h < a.heads || (h < per && stored);
-      ra[i] = live ? ld16(z + (long)h * D + 8 * ch.x) : make_uint4(0, 0, 0, 0);
-      rb[i] = live ? ld16(z + (long)h * D + 8 * ch.y) : make_uint4(0, 0, 0, 0);
+      ra[i] = rb[i] = make_uint4(0, 0, 0, 0);
+      if (live && h < per) ra[i] = ld16(z + (long)h * D + 8 * ch.x), rb[i] = ld16(z + (long)h * D + 8 * ch.y);
     }
+  };
+  load(wsub);
+  if (a.qn || a.kn) {
+    for (int d = threadIdx.x; d < D; d += 256) {
+      if (a.qn) weights[0][d] = __half2float(a.qn[d]);
+      if (a.kn) weights[1][d] = __half2float(a.kn[d]);
+    }
+    __syncthreads();
+  }
+  if (!live) return;
+  const bool turn = u < a.rot / 16, stored = slot >= 0 && slot < a.nslots;
+  if (slot >= a.nslots && lane == 0) atomicOr(a.err, (uint32_t)DC_DEVERR_BOUNDS);
+  const int pg = slot >> a.pshift, off = slot & (a.page - 1);
+  float cs[8], sn[8];
+  if (turn) angles8(a.freq + 8 * u, pos, a.factor, cs, sn);
+  for (int p0 = wsub; p0 < npass; p0 += NP * a.W) {
+    uint4 xa[NP], xb[NP];
+#pragma unroll
+    for (int i = 0; i < NP; i++) xa[i] = ra[i], xb[i] = rb[i];
+    if (p0 + NP * a.W < npass) load(p0 + NP * a.W);
 #pragma unroll
     for (int i = 0; i < NP; i++) {
       const int h = (p0 + i * a.W) * HPP + sub;
       const bool isq = h < a.heads, isk = !isq && h < a.heads + a.kv;
       const bool normed = isq ? a.qn != nullptr : isk ? a.kn != nullptr : a.vnorm != 0;
       float x[8], y[8];
-      unpack8(ra[i], x), unpack8(rb[i], y);
-      float ss = 0.f;
+      unpack8(xa[i], x), unpack8(xb[i], y);
+      if (a.qn || a.kn || a.vnorm) {
+        float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; e++) ss += x[e] * x[e] + y[e] * y[e];
+        for (int e = 0; e < 8; e++) s0 = fmaf(x[e], x[e], s0), s1 = fmaf(y[e], y[e], s1);
+        float ss = s0 + s1;
 #pragma unroll
-      for (int o = U / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);  // every lane of the warp
-      if (h >= per) continue;
-      if (normed) {
-        const float inv = rsqrtf(ss * (1.0f / D) + a.eps);
-        float wx[8], wy[8];
-        unpack8(isq ? wq[0] : wk[0], wx), unpack8(isq ? wq[1] : wk[1], wy);
+        for (int o = U / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);  // every lane of the warp
+        if (normed) {
+          const float inv = rsqrtf(ss * (1.0f / D) + a.eps);
+          const float *w = weights[isq ? 0 : 1];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          x[e] *= inv, y[e] *= inv;
-          if (isq || isk) x[e] *= wx[e], y[e] *= wy[e];
+          for (int e = 0; e < 8; e += 4) {
+            float4 wx = make_float4(inv, inv, inv, inv), wy = wx;
+            if (isq || isk) {
+              const float4 px = *reinterpret_cast<const float4 *>(w + 8 * ch.x + e), py = *reinterpret_cast<const float4 *>(w + 8 * ch.y + e);
+              wx = make_float4(px.x * inv, px.y * inv, px.z * inv, px.w * inv);
+              wy = make_float4(py.x * inv, py.y * inv, py.z * inv, py.w * inv);
+            }
+            x[e] *= wx.x, x[e + 1] *= wx.y, x[e + 2] *= wx.z, x[e + 3] *= wx.w;
+            y[e] *= wy.x, y[e + 1] *= wy.y, y[e + 2] *= wy.z, y[e + 3] *= wy.w;
+          }
         }
       }
+      if (h >= per) continue;
       if (turn && (isq || isk)) rotate<INTER>(x, y, cs, sn);
       __half *dst;
       if (isq) {
@@ -200,7 +220,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
       } else {
         if (!stored) continue;
         const int hk = h - a.heads - (isk ? 0 : a.kv);
-        dst = (isk ? a.K : a.V) + (((long)pg * a.kv + hk) * a.page + off) * D;
+        dst = (isk ? a.K : a.V) + ((((long)pg * a.kv + hk) << a.pshift) + off) * D;
       }
       st16(dst + 8 * ch.x, pack8(x));
       st16(dst + 8 * ch.y, pack8(y));
@@ -235,7 +255,7 @@ int ops_kv_append(dc_ctx *ctx, const dc_kv_cache *c, const dc_rope_plan *p, cons
   a.freq = p ? p->d_freq : nullptr, a.factor = p ? p->factor : 1.0f, a.rot = p ? p->rot : 0;
   a.err = ctx->d_err;
   a.zs = zs, a.qs = qs;
-  a.T = T, a.heads = heads, a.kv = c->kv, a.page = c->page, a.nslots = c->pages * c->page;
+  a.T = T, a.heads = heads, a.kv = c->kv, a.page = c->page, a.pshift = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7, a.nslots = c->pages * c->page;
   a.vnorm = vnorm, a.eps = eps;
   const int npass = (heads + 2 * c->kv + 512 / c->D - 1) / (512 / c->D);
   // warps per token: one, which works the angles out once for all heads, unless that leaves the card without warps
