@@ -122,18 +122,22 @@ def check(rc: int) -> None:
         raise DecisionError(rc, lib().dc_last_error().decode() or f"decision.js: error {rc}")
 
 
+_PLAIN = frozenset((int, float, bool, type(None)))  # arguments that go as they are
+
+
 def ptr(x) -> int | None:
     """A device or host address from a torch tensor, numpy array, int or None; a handle's from a RopePlan or KvCache."""
     if x is None:
         return None
     if isinstance(x, int):
         return x
+    address = getattr(x, "data_ptr", None)
+    if address is not None:
+        return address()
     if isinstance(x, _Handle):
         if not x.h:
             raise DecisionError(DC_EINVAL, f"decision.js: a closed {type(x).__name__}")
         return x.h.value
-    if hasattr(x, "data_ptr"):
-        return x.data_ptr()
     if hasattr(x, "ctypes"):
         return x.ctypes.data
     raise TypeError(type(x))
@@ -229,8 +233,9 @@ class Context:
 
     def call(self, name: str, *args):
         """Calls dc_<name>(ctx, *args), converting tensors / arrays to addresses, and raises on failure."""
-        conv = [ptr(a) if not isinstance(a, (float, bool)) else a for a in args]
-        check(getattr(lib(), "dc_" + name)(self.h, *conv))
+        rc = getattr(lib(), "dc_" + name)(self.h, *[a if type(a) in _PLAIN else ptr(a) for a in args])
+        if rc:
+            check(rc)
 
     def rope_plan(self, rot: int, layout: str = "half", frequencies=None, factor: float | None = None, **scaling):
         """A RopePlan for the first `rot` dims of a head, layout "half" or "interleaved": by the given frequencies

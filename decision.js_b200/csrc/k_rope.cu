@@ -140,9 +140,9 @@ struct AppendArgs {
 // W warps per token; a pass of a warp covers 32 / (D/16) of the token's q, k and v heads, U = D/16 lanes to a head
 // (one unit each). NP passes are loaded at a time, the next NP while these are worked on.
 template <int D, bool INTER>
-__global__ void __launch_bounds__(256, 2) kv_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, 3) kv_append_kernel(const AppendArgs a) {
   dc_pdl_begin();
-  constexpr int U = D / 16, HPP = 32 / U, NP = 4;
+  constexpr int U = D / 16, HPP = 32 / U, NP = 2;
   __shared__ __align__(16) float weights[2][D];  // the norms', in f32: converted once, not in every pass
   const long wid = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const long t = wid / a.W;
