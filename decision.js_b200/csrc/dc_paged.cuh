@@ -469,34 +469,46 @@ __device__ __forceinline__ void mark_rows(volatile uint32_t *mark, const Run &r,
   if (m) atomicOr(const_cast<uint32_t *>(mark) + lane, m);
 }
 
-// Looks over each V block before its product, one warp: the rows past the last key (of the 16 that a product step takes)
-// are zeroed, and values that are not finite too where some row of the tile would multiply them by a weight of 0, with a
-// mark on the rows that see them.
+// Whether the block of a run at key0 has to be looked over before its product: the 16 keys of a product step reach past
+// the last key, or a row of the tile that sees the block does not see all its keys (its first such row sees the fewest).
+template <int KB>
+__device__ __forceinline__ bool partly_seen(const Run &r, int key0) {
+  const int t = max(max(r.tok0, r.qb), key0 - r.len + r.qe);
+  return r.seg >= 0 && own_limit(t, r.qe, r.len) < min(key0 + KB, r.kend);
+}
+template <int KB>
+__device__ __forceinline__ bool to_look_over(const Run &r, int key0) {
+  return (min(KB, r.kend - key0) & 15) != 0 || partly_seen<KB>(r, key0);
+}
+
+// Looks those blocks over, one warp: the rows past the last key are zeroed, and values that are not finite too where some
+// row would multiply them by a weight of 0, with a mark on the rows that see them. The product of the c-th of them waits
+// for barrier B_VS + c % VST; the others go straight from V's arrival.
 template <class C>
 __device__ __forceinline__ void look_over(const Cta<C> &k) {
   constexpr int KB = C::KB, VST = C::VST, NA = C::NA;
   const int lane = k.lane;
   Run r;
-  int g = 0;
+  int g = 0, looked = 0;
   bool ok = true;
   for (int n = 0; ok && k.next_run(n, r); n++) {
     volatile uint32_t *mark = k.poison(r.item);
     if ((r.flags & RUN_FIRST) && lane < 4) mark[lane] = 0;
     __syncwarp();
     for (int b = 0; b < r.nb; b++, g++) {
-      const int st = g % VST;
+      const int st = g % VST, key0 = (r.kb + b) * KB;
       if (!(ok = k.wait_warp(C::B_VF + st, g / VST))) break;
-      const int key0 = (r.kb + b) * KB, valid = min(KB, r.kend - key0), pad = (valid + 15) & ~15;
-      uint8_t *v = k.smem + C::V_OFF + st * C::KV_BYTES + (lane & 7) * 16;
-      if (valid < pad) {  // up to 15 rows, four at a time
-        for (int row = valid + lane / 8; row < pad; row += 4)
-#pragma unroll
-          for (int at = 0; at < NA; at++) *reinterpret_cast<uint4 *>(v + at * (KB * 128) + row * 128) = make_uint4(0, 0, 0, 0);
+      // every block counts this warp among those that give its stage back, or it could fall a phase behind
+      if (!to_look_over<KB>(r, key0)) {
+        if (lane == 0) mbar_arrive(k.bar(C::B_VE + st));
+        continue;
       }
-      // own blocks: the first row of the tile that sees the block sees the fewest of its keys
-      const int t1 = max(max(r.tok0, r.qb), key0 - r.len + r.qe);
-      const bool scan = r.seg >= 0 && own_limit(t1, r.qe, r.len) < key0 + valid;
-      if (scan) {
+      const int valid = min(KB, r.kend - key0), pad = (valid + 15) & ~15;
+      uint8_t *v = k.smem + C::V_OFF + st * C::KV_BYTES + (lane & 7) * 16;
+      for (int row = valid + lane / 8; row < pad; row += 4)
+#pragma unroll
+        for (int at = 0; at < NA; at++) *reinterpret_cast<uint4 *>(v + at * (KB * 128) + row * 128) = make_uint4(0, 0, 0, 0);
+      if (partly_seen<KB>(r, key0)) {
         int worst = KB;  // the first row with a value that is not finite
 #pragma unroll 1
         for (int at = 0; at < NA; at++) {
@@ -506,9 +518,13 @@ __device__ __forceinline__ void look_over(const Cta<C> &k) {
         worst = __reduce_min_sync(0xffffffffu, worst);
         if (worst < KB) mark_rows(mark, r, key0 + worst, lane);
       }
-      if (scan || valid < pad) fence_proxy_async_smem();
+      fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(k.bar(C::B_VS + st));
+      if (lane == 0) {
+        mbar_arrive(k.bar(C::B_VS + looked % VST));
+        mbar_arrive(k.bar(C::B_VE + st));
+      }
+      looked++;
     }
     if (ok) k.done_run(n);
   }

@@ -58,6 +58,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     for (int i = 0; i < C::NBARS; i++) {
       const int n = i == C::B_OE || (i >= C::B_PF && i < C::B_PF + SB) ? FS
                     : i >= C::B_XB && i < C::B_XB + 4                  ? 2
+                    : i >= C::B_VE && i < C::B_VE + VST                ? 2
                     : i >= C::B_IE                                     ? FS + 3
                                                                        : 1;
       mbar_init(k.bar(i), n);
@@ -92,11 +93,18 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     Run r = {};
     int g = 0;
     bool ok = true, pend = false, begins = true;  // begins: the tile has had no block yet
-    int steps = 0;                                // of the pending product (block g - 1): 16 keys each,
+    int looked = 0;
+    bool look = false;                            // whether the pending product's (block g - 1) values are looked over first,
+    int steps = 0;                                // its steps of 16 keys,
     uint32_t off[4] = {};                         // and the rows that it leaves alone
     auto pv = [&](int x) -> bool {
       const int vs = x % VST;
-      if (!k.wait_warp(C::B_VS + vs, x / VST) || !k.wait_warp(C::B_PF + x % SB, x / SB)) return false;  // (VS: after VF)
+      if (!k.wait_warp(C::B_VF + vs, x / VST)) return false;
+      if (look) {
+        if (!k.wait_warp(C::B_VS + looked % VST, looked / VST)) return false;
+        looked++;
+      }
+      if (!k.wait_warp(C::B_PF + x % SB, x / SB)) return false;
       tc_fence_after();
       // the weights of keys [0, COLS) begin the scores' buffer, those of [COLS, KB) its second half
       const uint32_t p = tmem + (uint32_t)(C::S_COL + x % SB * KB);
@@ -133,6 +141,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
         __syncwarp();
         if (SB > 1 && pend && !(ok = pv(g - 1))) break;
         pend = true, begins = false;
+        look = to_look_over<KB>(r, key0);
         steps = (min(KB, r.kend - key0) + 15) >> 4;
         // own blocks: the rows of the sequence that see a key of it
         const int lo = r.seg < 0 ? 0 : (max(max(r.tok0, r.qb), key0 - r.len + r.qe) - r.tok0) * a.r;
@@ -161,7 +170,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     bool ok = true;
     // the tile's state
     bool valid = false, anyv = false, had = false, tfirst = false;
-    int t = 0, seq = -1, lim = 0;
+    int t = 0;
     float ref = -FLT_MAX, l = 0.f;
     auto meet = [&]() -> bool {  // both warps of the quadrant have written their halves
       __syncwarp();
@@ -177,16 +186,6 @@ __global__ void __launch_bounds__(F_THREADS, 2)
         anyv = __any_sync(0xffffffffu, valid);
         had = false, tfirst = (r.flags & RUN_TFIRST) != 0;
         ref = -FLT_MAX, l = 0.f;
-        seq = -1, lim = 0;
-        if (valid && t >= r.qb) {  // its sequence: the last at or after the run's whose rows begin at or before it
-          int x = r.s, y = a.S;
-          if (t < r.qe) y = x + 1;
-          while (y - x > 1) {
-            const int m = (x + y) >> 1;
-            if (a.qoff[m] <= t) x = m; else y = m;
-          }
-          seq = x, lim = own_limit(t, a.qoff[x + 1], a.lens[x]);
-        }
         if (anyv) {  // the accumulator to zero; the last tile's was read by this very warp
           const uint32_t z[16] = {};
           __syncwarp();
@@ -196,7 +195,8 @@ __global__ void __launch_bounds__(F_THREADS, 2)
           tc_fence_before();
         }
       }
-      const int rlim = !valid ? 0 : r.seg < 0 ? r.kend : seq == r.seg ? lim : 0;
+      // the run's keys that the row sees
+      const int rlim = !valid ? 0 : r.seg < 0 ? r.kend : t >= r.qb && t < r.qe ? own_limit(t, r.qe, r.len) : 0;
       const int nb = r.nb, kb = r.kb;
       // the run's first blocks that every row here sees whole (lanes without a row have no say)
       const int full = __reduce_min_sync(0xffffffffu, valid ? rlim : 0x7fffffff) / KB - kb;

@@ -51,7 +51,7 @@ template <int D>
 struct WideCfg {
   // keys per block; 64 at D = 256, whose tiles and accumulator leave room for no more
   static constexpr int KB = D == 256 ? 64 : 128, NA = D / 64, Q_ROWS = 128, THREADS = PA_THREADS;
-  static constexpr int KST = D == 64 ? 4 : D == 128 ? 3 : 2, VST = D == 64 ? 4 : 2;  // stages of the K and of the V ring
+  static constexpr int KST = D == 64 ? 4 : 2, VST = D == 64 ? 4 : D == 128 ? 3 : 2;  // stages of the K and of the V ring
   static constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = KB * D * 2;
   static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + KST * KV_BYTES;
   static constexpr int BAR_OFF = V_OFF + VST * KV_BYTES;
@@ -90,6 +90,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       const int n = i == C::B_OE                              ? PA_SOFT
                     : i >= C::B_PF && i < C::B_PF + PA_WG   ? 4
                     : i >= C::B_XB && i < C::B_XB + 4       ? PA_WG
+                    : i >= C::B_VE && i < C::B_VE + VST     ? 2
                     : i >= C::B_IE                          ? PA_SOFT + 4
                                                             : 1;
       mbar_init(bar(i), n);
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // V MN-major
     if (elect_one()) {
       const uint64_t v0 = desc_mn(sbase + C::V_OFF, KB * 128);
-      int g = 0;
+      int g = 0, looked = 0;
       bool ok = true;
       for (int n = 0; ok && wait1(C::B_IF + n % PA_RING, n / PA_RING); n++) {
         const Run r = runs[n % PA_RING];
@@ -174,7 +175,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 #pragma unroll
             for (int w = 0; w < 4; w++) off[w] = ~mask_word(lo, hi, w);
           }
-          if (!(ok = wait1(C::B_VS + st, g / VST) && wait1(C::B_PF + sb, g / PA_WG))) break;  // (VS: after VF)
+          if (!(ok = wait1(C::B_VF + st, g / VST))) break;
+          if (to_look_over<KB>(r, key0)) {
+            if (!(ok = wait1(C::B_VS + looked % VST, looked / VST))) break;
+            looked++;
+          }
+          if (!(ok = wait1(C::B_PF + sb, g / PA_WG))) break;
           tc_fence_after();
           const uint32_t p = tmem + (uint32_t)(C::S_COL + sb * KB);
           const uint64_t v = v0 + (uint32_t)(st * C::KV_BYTES >> 4);
@@ -200,7 +206,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     bool ok = true;
     // the tile's state
     bool valid = false, anyv = false, had = false, tfirst = false;
-    int t = 0, seq = -1, lim = 0;
+    int t = 0;
     float ref = -FLT_MAX, l = 0.f;  // l: the sum of this thread's weights, in units of 2^(ref - 7)
     auto zero = [&]() {             // this warp's share of its rows' accumulators: every third 16 columns
       const uint32_t z[16] = {};
@@ -222,18 +228,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         anyv = __any_sync(0xffffffffu, valid);
         had = false, tfirst = (r.flags & RUN_TFIRST) != 0;
         ref = -FLT_MAX, l = 0.f;
-        seq = -1, lim = 0;
-        if (valid && t >= r.qb) {  // its sequence: the last at or after the run's whose rows begin at or before it
-          int x = r.s, y = a.S;
-          if (t < r.qe) y = x + 1;
-          while (y - x > 1) {
-            const int m = (x + y) >> 1;
-            if (a.qoff[m] <= t) x = m; else y = m;
-          }
-          seq = x, lim = own_limit(t, a.qoff[x + 1], a.lens[x]);
-        }
       }
-      const int rlim = !valid ? 0 : r.seg < 0 ? r.kend : seq == r.seg ? lim : 0;
+      // the run's keys that the row sees
+      const int rlim = !valid ? 0 : r.seg < 0 ? r.kend : t >= r.qb && t < r.qe ? own_limit(t, r.qe, r.len) : 0;
       const int nb = r.nb, kb = r.kb, kend = r.kend;
       // the run's first blocks that every row here sees whole (lanes without a row have no say)
       const int full = __reduce_min_sync(0xffffffffu, valid ? rlim : 0x7fffffff) / KB - kb;

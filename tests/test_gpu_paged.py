@@ -419,6 +419,26 @@ def test_attention_paged_in_place_and_repeatable(ctx, dev):
     assert torch.equal(c.dq, c.y)
 
 
+@pytest.mark.parametrize("heads,kv,D,groups", [
+    (16, 8, 128, [(5000 - 300 * g, [(1, 40 * i + 1) for i in range(12)]) for g in range(6)]),
+    (32, 8, 64, [(3000, [(1, 70 * i) for i in range(9)]), (4111, [(1, 5)])]),
+    (24, 8, 128, [(2100, [(37, 37 + i) for i in range(20)])]), (8, 2, 256, [(1500, [(20, 90)] * 9)])])
+def test_attention_paged_many_calls_in_a_row(ctx, dev, heads, kv, D, groups):
+    """Two hundred calls without a wait between them, all the same bits: the roles within a CTA, which run at their own
+    pace, never lose step (a wait that ran out would flag the next sync)."""
+    import torch
+    c = Case(ctx, dev, groups, heads, kv, D, 32, seed=8)
+    c.call()
+    ctx.sync(60000)
+    first = c.y.clone()
+    for i in range(200):
+        c.call()
+        if i % 40 == 39:
+            ctx.sync(60000)
+            assert torch.equal(c.y, first)
+    c.check(rows={0, c.T - 1})
+
+
 def test_attention_paged_refuses_bad_arrays(ctx, dev, pkg):
     """Offsets that fall, reach past their table or rows: nothing is written, the next sync says so, and the context
     works on."""
