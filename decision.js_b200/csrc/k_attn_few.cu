@@ -5,8 +5,12 @@
 //   warps 0-7  softmax: two warps per TMEM lane quadrant, thread = row, each half of a block's keys; the halves' maxima
 //              meet in shared memory. Quadrants without rows only keep step.
 //   warp 8     walks the line, loads Q and K; warp 9 loads V; warp 10 Q K^T and P V (and TMEM); warp 11 looks values over
-// Blocks are 64 keys with two scores' buffers at D = 128, 128 keys with one at D = 64: 256 columns of tensor memory either
-// way, and about the same bytes a block. The weights are scaled by 2^7 as in the wide kernel.
+// Blocks are 64 keys with two scores' buffers, which leaves each warp 32 scores: they stay in registers from the maximum
+// to the weights. The weights are scaled by 2^7 as in the wide kernel.
+// Bound by the chain of a block, not by the cache's bytes: 64 sequences of one token over a shared prefix of 32,768 tokens
+// (24 heads over 8, D = 128) take 40 us where the bytes need 18.6. Kept steps: two CTAs an SM with halves of rows 45 -> 40
+// us, the join by row, unneeded waits on the look-over removed. Measured and not taken: blocks of 128 keys in one scores'
+// buffer at D = 64, one pass with the weights kept in registers, products by warps' own matrix instructions.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -94,9 +98,9 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     int g = 0;
     bool ok = true, pend = false, begins = true;  // begins: the tile has had no block yet
     int looked = 0;
-    bool look = false;                            // whether the pending product's (block g - 1) values are looked over first,
-    int steps = 0;                                // its steps of 16 keys,
-    uint32_t off[4] = {};                         // and the rows that it leaves alone
+    bool look = false;     // whether the pending product's (block g - 1) values are looked over first,
+    int steps = 0;         // its steps of 16 keys,
+    uint32_t off[4] = {};  // and the rows that it leaves alone
     auto pv = [&](int x) -> bool {
       const int vs = x % VST;
       if (!k.wait_warp(C::B_VF + vs, x / VST)) return false;
@@ -126,20 +130,19 @@ __global__ void __launch_bounds__(F_THREADS, 2)
       for (int b = 0; ok && b < r.nb; b++, g++) {
         const int ks = g % KST, key0 = (r.kb + b) * KB;
         if (!(ok = k.wait_warp(C::B_KF + ks, g / KST))) break;
-        if (SB == 1 && pend && !(ok = pv(g - 1))) break;  // the one buffer holds its weights
         tc_fence_after();
         if (elect_one()) {
           const uint32_t sc = tmem + (uint32_t)(C::S_COL + g % SB * KB);
           const uint64_t kd0 = k0 + (uint32_t)(ks * C::KV_BYTES >> 4);
 #pragma unroll
           for (int kd = 0; kd < D / 16; kd++)
-            mma_f16(sc, q0 + (((kd >> 2) * 128 * 128 + (kd & 3) * 32) >> 4), kd0 + (((kd >> 2) * KB * 128 + (kd & 3) * 32) >> 4),
-                    idesc_qk, kd > 0);
+            mma_f16(sc, q0 + (((kd >> 2) * 128 * 128 + (kd & 3) * 32) >> 4),
+                    kd0 + (((kd >> 2) * KB * 128 + (kd & 3) * 32) >> 4), idesc_qk, kd > 0);
           mma_commit(k.bar(C::B_SF + g % SB));
           mma_commit(k.bar(C::B_KE + ks));
         }
         __syncwarp();
-        if (SB > 1 && pend && !(ok = pv(g - 1))) break;
+        if (pend && !(ok = pv(g - 1))) break;
         pend = true, begins = false;
         look = to_look_over<KB>(r, key0);
         steps = (min(KB, r.kend - key0) + 15) >> 4;
@@ -210,27 +213,22 @@ __global__ void __launch_bounds__(F_THREADS, 2)
           const uint32_t scol = lrow + (uint32_t)(C::S_COL + sb * KB + hf * COLS);
           float sc = a.scale_log2;
           uint32_t x[32];
-          auto load = [&](int c) {  // 32 scores; minus infinity where the row does not see the key
-            __syncwarp();
-            tmem_ld32(scol + c, x);
-            tmem_ld_wait(x);
-            if (a.scale_log2 <= 0.f)  // the largest score is not the largest product: scale first
+          __syncwarp();
+          tmem_ld32(scol, x);
+          tmem_ld_wait(x);
+          if (sc <= 0.f) {  // the largest score is not the largest product: scale first
 #pragma unroll
-              for (int e = 0; e < 32; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * a.scale_log2);
-            if (part)
+            for (int e = 0; e < 32; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * sc);
+            sc = 1.f;
+          }
+          if (part)  // minus infinity where the row does not see the key
 #pragma unroll
-              for (int e = 0; e < 32; e++) x[e] = hf * COLS + c + e < nv ? x[e] : 0xff800000u;
-          };
-          if (sc <= 0.f) sc = 1.f;
+            for (int e = 0; e < 32; e++) x[e] = hf * COLS + e < nv ? x[e] : 0xff800000u;
           float m2[2] = {__uint_as_float(0xff800000u), __uint_as_float(0xff800000u)};
-#pragma unroll 1
-          for (int c = 0; c < COLS; c += 32) {
-            load(c);
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              m2[0] = max3(m2[0], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-              m2[1] = max3(m2[1], __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
-            }
+          for (int e = 0; e < 32; e += 4) {
+            m2[0] = max3(m2[0], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+            m2[1] = max3(m2[1], __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
           }
           const float pmx = fmaxf(m2[0], m2[1]) * sc;
           const int par = meets & 1;
@@ -240,8 +238,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
           const bool grow = mx > ref + 8.0f;
           const bool resc = grow && ref > -FLT_MAX;
           if (__any_sync(0xffffffffu, resc)) {
-            // the products so far (with one scores' buffer they were done before this block's scores)
-            if (SB > 1 && !(ok = k.wait_warp(C::B_OR, g - 1))) break;
+            if (!(ok = k.wait_warp(C::B_OR, g - 1))) break;  // the products so far
             tc_fence_after();
             const float f = resc ? ex2_approx(ref - mx) : 1.0f;
             l *= f;
@@ -261,22 +258,18 @@ __global__ void __launch_bounds__(F_THREADS, 2)
           if (grow) ref = mx;
           const uint64_t ref2 = f32x2(7.0f - ref, 7.0f - ref), sc2 = f32x2(sc, sc);
           uint64_t sum[2] = {0, 0};
-#pragma unroll 1
-          for (int c = 0; c < COLS; c += 32) {
-            if (COLS > 32) load(c);  // (one chunk of 32 is still in registers)
-            uint32_t w[16];
+          uint32_t w[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 v = f32x2_split(fma_f32x2(f32x2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, ref2));
-              const float p0 = ex2_approx(v.x), p1 = ex2_approx(v.y);
-              sum[(e >> 1) & 1] = add_f32x2(sum[(e >> 1) & 1], f32x2(p0, p1));
-              const __half2 hp = __floats2half2_rn(p0, p1);
-              w[e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
-            }
-            // 32 weights over 16 of this warp's own scores, all done with
-            __syncwarp();
-            tmem_st16(scol + c / 2, w);
+          for (int e = 0; e < 32; e += 2) {
+            const float2 v = f32x2_split(fma_f32x2(f32x2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, ref2));
+            const float p0 = ex2_approx(v.x), p1 = ex2_approx(v.y);
+            sum[(e >> 1) & 1] = add_f32x2(sum[(e >> 1) & 1], f32x2(p0, p1));
+            const __half2 hp = __floats2half2_rn(p0, p1);
+            w[e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
           }
+          // 32 weights over 16 of this warp's own scores, all done with
+          __syncwarp();
+          tmem_st16(scol, w);
           const float2 add = f32x2_split(add_f32x2(sum[0], sum[1]));
           l += add.x + add.y;
           tmem_st_wait();

@@ -3,10 +3,11 @@
 // For a query row, o = sum_j p_j v_j / sum_j p_j with p_j = exp(scale q . k_j), j over its group's prefix and its own
 // keys up to its own. A tile is 128 rows of one kv head: TPT = 128 / r consecutive tokens of a group (r query heads to
 // a kv head), so tokens of several sequences share the tile and the prefix passes through the tensor cores once for
-// all of them. The keys of a tile are a list of 64-key blocks: the prefix's, then, sequence by sequence, the own
-// blocks of the sequences that the tile's tokens belong to, seen by that sequence's rows alone.
+// all of them. The keys of a tile are a list of blocks: the prefix's, then, sequence by sequence, the own blocks of the
+// sequences that the tile's tokens belong to, seen by that sequence's rows alone (the product leaves the other rows'
+// accumulators as they are).
 //
-// The blocks of all tiles of all kv heads in a row make one line of B units (a sequence piece without keys counts as
+// The blocks of all tiles of all kv heads in a row make one line of units (a sequence piece without keys counts as
 // one unit, so that every tile is visited). Each CTA of a resident grid takes an equal stretch of it, whatever the
 // lengths: a long prefix is cut over many CTAs, short tiles are walked one after the other. Every CTA works the line
 // out for itself from the offsets and lengths (one scan over the sequences), so nothing is planned on the host and a
@@ -14,18 +15,28 @@
 // f32 parts (value sums, row maximum and weight sum) that a second kernel joins in order of the stretches, so results
 // do not depend on timing.
 //
-// Within a CTA:
-//   warps 0-7  softmax, two warpgroups that take the blocks in turn, thread = row. A row's reference (the maximum its
-//              weights are relative to) goes from block to block through shared memory, each warp waiting for its
-//              twin's turn only between its own maximum and its weights; the exp2 weights are scaled by 2^7 (the row reference moves when the maximum
-//              grows past 2^8, so they stay under 2^15) to keep small ones out of f16's subnormals
-//   warp 16    walks the line, hands runs of blocks to the others through a ring of descriptors, loads Q and K
-//   warp 13    loads V
-//   warp 14    Q K^T (and TMEM), warp 15 P V: two threads, as one would be busy issuing for longer than the products take
+// This file holds the kernel for many rows, the join and the host side; k_attn_few.cu the kernel for few rows; the line
+// and what both kernels' producers do with it are in dc_paged.cuh. Within a CTA here, one to an SM:
+//   warps 0-11 softmax, three warpgroups that take the blocks (128 keys; 64 at D = 256) in turn, thread = row. A row's
+//              reference (what its weights are relative to) goes from block to block through shared memory: a warp waits
+//              for its turn only between its own maximum and its weights. The reference moves when a maximum is more than
+//              2^8 above it, and weights are scaled by 2^7: they stay under 2^15, and small ones out of f16's subnormals.
+//              The rounding of a weight to f16, half a step of itself, is the matrix unit's operand type; sums are f32.
 //   warp 12    looks over V blocks that some row of the tile does not see: rows past the last key are zeroed, and
 //              values that are not finite too (a weight of 0 times them would be NaN in every row), with a mark on
 //              the rows that see them
-// All roles run ahead across tiles: only Q (single buffer) and the accumulator wait for a tile's end.
+//   warp 13    loads V
+//   warp 14    Q K^T (and TMEM), warp 15 P V: two threads, as one would be busy issuing for longer than the products take
+//   warp 16    walks the line, hands runs of blocks to the others through a ring of descriptors, loads Q and K
+// All roles run ahead across tiles; Q (single buffer) and the accumulator wait for a tile's end, which the warpgroup of the
+// tile's last block sees to while the other two go on.
+//
+// What bounds it. Many rows over a long prefix (60 sequences of up to 50 tokens, 16,000 keys, 24 heads over 8, D = 128):
+// 218 us, 818 TFLOP/s, half the measured matrix rate; without the softmax it still takes 167, as every tile of 128 rows
+// brings all its keys from L2 (about 39 bytes a clock and SM): only tiles of 256 rows would change that, and tensor memory
+// has no room for their scores next to two accumulators. Short tiles (a few blocks each): the chain from a tile's last
+// product over its stores to the next tile's first product. Steps measured: two softmax warpgroups in turn 264 -> 245
+// us, three with 128-key blocks 232, the tile's end by one warpgroup instead of all three 2% (8% at D = 64).
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -55,7 +66,7 @@ struct WideCfg {
   static constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = KB * D * 2;
   static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + KST * KV_BYTES;
   static constexpr int BAR_OFF = V_OFF + VST * KV_BYTES;
-  static constexpr int B_QF = 0, B_QE = 1, B_OD = 2, B_OE = 3, B_XB = 4, B_SF = 8, B_PF = B_SF + PA_WG,
+  static constexpr int B_QF = 0, B_QE = 1, B_OE = 2, B_OD = 3, B_XB = 7, B_SF = 23, B_PF = B_SF + PA_WG,
                        B_SE = B_PF + PA_WG, B_CH = B_SE + PA_WG, B_KF = B_CH + 4 * PA_WG, B_KE = B_KF + KST, B_VF = B_KE + KST,
                        B_VE = B_VF + VST, B_VS = B_VE + VST, B_IF = B_VS + VST, B_IE = B_IF + PA_RING,
                        NBARS = B_IE + PA_RING;
@@ -64,7 +75,7 @@ struct WideCfg {
   static constexpr int POISON_OFF = MISC_OFF + 32, SCAN_OFF = POISON_OFF + 64,
                        RUN_OFF = SCAN_OFF + ((PA_THREADS / 32 * 8 + 15) & ~15), GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run),
                        XCH_OFF = GOFF_OFF + 3 * (PA_GOFF + 4) * 4;
-  static constexpr int SMEM = XCH_OFF + (1 + 2 * PA_WG) * 128 * 4 + 1024;
+  static constexpr int SMEM = XCH_OFF + 128 * 4 + 4 * PA_WG * 128 * 8 + 1024;
   static constexpr int S_COL = 0, O_COL = PA_WG * KB;  // tensor memory: a scores' buffer per warpgroup, the accumulator
   static constexpr int TCOLS = 512;
   static_assert(O_COL + D <= TCOLS, "tensor memory");
@@ -87,12 +98,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 
   if (tid == 0) {
     for (int i = 0; i < C::NBARS; i++) {
-      const int n = i == C::B_OE                              ? PA_SOFT
-                    : i >= C::B_PF && i < C::B_PF + PA_WG   ? 4
-                    : i >= C::B_XB && i < C::B_XB + 4       ? PA_WG
-                    : i >= C::B_VE && i < C::B_VE + VST     ? 2
-                    : i >= C::B_IE                          ? PA_SOFT + 4
-                                                            : 1;
+      const int n = i == C::B_OE || (i >= C::B_PF && i < C::B_PF + PA_WG) ? 4
+                    : i >= C::B_XB && i < C::B_XB + 16                     ? PA_WG - 1
+                    : i >= C::B_VE && i < C::B_VE + VST                    ? 2
+                    : i >= C::B_IE                                         ? PA_SOFT + 4
+                                                                           : 1;
       mbar_init(bar(i), n);
     }
     *k.abort() = 0;
@@ -143,8 +153,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           const uint64_t k = k0 + (uint32_t)(st * C::KV_BYTES >> 4);
 #pragma unroll
           for (int kd = 0; kd < D / 16; kd++)
-            mma_f16(sc, q0 + (((kd >> 2) * 128 * 128 + (kd & 3) * 32) >> 4), k + (((kd >> 2) * KB * 128 + (kd & 3) * 32) >> 4),
-                    idesc_qk, kd > 0);
+            mma_f16(sc, q0 + (((kd >> 2) * 128 * 128 + (kd & 3) * 32) >> 4),
+                    k + (((kd >> 2) * KB * 128 + (kd & 3) * 32) >> 4), idesc_qk, kd > 0);
           mma_commit(bar(C::B_SF + sb));
           mma_commit(bar(C::B_KE + st));
         }
@@ -190,7 +200,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           mma_commit(bar(C::B_SE + sb));
           mma_commit(bar(C::B_VE + st));
         }
-        if (ok && (r.flags & RUN_LAST)) mma_commit(bar(C::B_OD));
+        if (ok && (r.flags & RUN_LAST)) mma_commit(bar(C::B_OD + (r.item & 3)));
         if (ok) mbar_arrive(bar(C::B_IE + n % PA_RING));
       }
     }
@@ -200,25 +210,26 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const int row = 32 * q + lane, irow = row / a.r, jrow = row - irow * a.r;
     const uint32_t lrow = tmem + ((uint32_t)(32 * q) << 16), ocol = lrow + (uint32_t)C::O_COL;
     const uint32_t scol = lrow + (uint32_t)(C::S_COL + wg * KB);
-    float *s_ref = reinterpret_cast<float *>(smem + C::XCH_OFF), *s_sum = s_ref + 128;  // [128], [2 turns][PA_WG][128]
-    int g = 0, turn = 0, meets = 0;  // blocks before the run, this warpgroup's blocks before this one
+    float *s_ref = reinterpret_cast<float *>(smem + C::XCH_OFF);
+    float2 *s_sum = reinterpret_cast<float2 *>(s_ref + 128);  // [tile % 4][PA_WG][128]
+    int g = 0, turn = 0;  // blocks before the run, this warpgroup's blocks before this one
     const int prev = wg == 0 ? PA_WG - 1 : wg - 1;
     bool ok = true;
     // the tile's state
     bool valid = false, anyv = false, had = false, tfirst = false;
     int t = 0;
     float ref = -FLT_MAX, l = 0.f;  // l: the sum of this thread's weights, in units of 2^(ref - 7)
-    auto zero = [&]() {             // this warp's share of its rows' accumulators: every third 16 columns
+    auto zero = [&]() {             // its rows' accumulators, for the next tile
       const uint32_t z[16] = {};
       __syncwarp();
 #pragma unroll 1
-      for (int c = 16 * wg; c < D; c += 16 * PA_WG) tmem_st16(ocol + c, z);
+      for (int c = 0; c < D; c += 16) tmem_st16(ocol + c, z);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(C::B_OE));
     };
-    zero();
+    if (wg == 0) zero();
     for (int n = 0; ok && wait_warp(C::B_IF + n % PA_RING, n / PA_RING); n++) {
       const Run &r = runs[n % PA_RING];  // (stays as it is until done_run)
       if (r.flags & RUN_END) break;
@@ -342,57 +353,60 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
       if (!ok) break;
       g += nb, had = had || nb > 0;
+      // The tile's end is the work of the warpgroup that took its last block: the others leave their sums and go on to the
+      // next tile, whose first product waits for the accumulator.
       if (r.flags & RUN_LAST) {
-        if (!(ok = wait_warp(C::B_OD, r.item))) break;
-        tc_fence_after();
-        const bool tlast = (r.flags & RUN_TLAST) != 0, direct = tfirst && tlast;
-        if (!direct && !a.by_row && tid == 0) {
-          if (tlast) a.head[blockIdx.x] = make_int4(r.tok0, r.ntok, r.kvh, 0);
-          if (tfirst) a.tail[blockIdx.x] = 1;
-        }
-        if (anyv) {
-          // the quadrant's warps add their sums at the row's last reference
-          const float fin = had ? s_ref[row] : -FLT_MAX;
-          float *sums = s_sum + (meets & 1) * (PA_WG * 128);
-          sums[wg * 128 + row] = l * ex2_approx(ref - fin);
+        const int four = r.item & 3, turn4 = r.item >> 2;
+        float2 *sums = s_sum + four * PA_WG * 128 + row;
+        if (wg != (g + PA_WG - 1) % PA_WG) {
+          sums[wg * 128] = make_float2(l, ref);
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(C::B_XB + q));
-          if (!(ok = wait_warp(C::B_XB + q, meets++))) break;
-          float lt = 0.f;
-#pragma unroll
-          for (int w = 0; w < PA_WG; w++) lt += sums[w * 128 + row];
-          if (had && valid && ((k.poison(r.item)[irow >> 5] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
-          const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
-          if (a.by_row && valid && jrow == 0 && wg == 0) {
-            if (tfirst) a.first[(long)r.kvh * a.T + t] = direct ? -1 : (int)blockIdx.x;
-            if (tlast) a.last[(long)r.kvh * a.T + t] = (int)blockIdx.x;
+          if (lane == 0) mbar_arrive(bar(C::B_XB + 4 * q + four));
+        } else {
+          if (!(ok = wait_warp(C::B_XB + 4 * q + four, turn4) && wait_warp(C::B_OD + four, turn4))) break;
+          tc_fence_after();
+          const bool tlast = (r.flags & RUN_TLAST) != 0, direct = tfirst && tlast;
+          if (!direct && q == 0 && lane == 0) {
+            if (tlast) a.head[blockIdx.x] = make_int4(r.tok0, r.ntok, r.kvh, 0);
+            if (tfirst) a.tail[blockIdx.x] = 1;
           }
-          if (!direct && valid && wg == 0) a.ml[prow] = make_float2(fin, lt);
-          const float inv = lt == 0.f ? 0.f : 1.0f / lt;
-          __half *y = a.Y + (long)t * a.ystride + (long)(r.kvh * a.r + jrow) * D;
-          float *po = a.O + prow * D;
-#pragma unroll 1
-          for (int c = 16 * wg; c < D; c += 16 * PA_WG) {
-            uint32_t o[16];
-            __syncwarp();
-            tmem_ld16(ocol + c, o);
-            tmem_ld_wait(o);
-            if (!valid) continue;
-            if (direct) {
-              uint32_t w[8];
+          if (anyv) {
+            float lt = l;  // at the row's last reference, which the last block's warpgroup has
 #pragma unroll
-              for (int e = 0; e < 8; e++) {
-                const __half2 hv = __floats2half2_rn(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-                w[e] = *reinterpret_cast<const uint32_t *>(&hv);
+            for (int w = 1; w < PA_WG; w++) {
+              const float2 x = sums[(wg + w) % PA_WG * 128];
+              lt += x.x * ex2_approx(x.y - ref);
+            }
+            if (had && valid && ((k.poison(r.item)[irow >> 5] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
+            const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
+            if (!direct && valid) a.ml[prow] = make_float2(ref, lt);
+            const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+            __half *y = a.Y + (long)t * a.ystride + (long)(r.kvh * a.r + jrow) * D;
+            float *po = a.O + prow * D;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              __syncwarp();
+              tmem_ld32(ocol + c, o);
+              tmem_ld_wait(o);
+              if (!valid) continue;
+              if (direct) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                  __half2 hv[4];
+#pragma unroll
+                  for (int i = 0; i < 4; i++)
+                    hv[i] = __floats2half2_rn(__uint_as_float(o[e + 2 * i]) * inv, __uint_as_float(o[e + 2 * i + 1]) * inv);
+                  *reinterpret_cast<uint4 *>(y + c + e) = *reinterpret_cast<const uint4 *>(hv);
+                }
+              } else if (lt != 0.f) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) st_global_v8(po + c + e, o + e);
               }
-              *reinterpret_cast<uint4 *>(y + c) = make_uint4(w[0], w[1], w[2], w[3]);
-              *reinterpret_cast<uint4 *>(y + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-            } else if (lt != 0.f) {
-              st_global_v8(po + c, o), st_global_v8(po + c + 8, o + 8);
             }
           }
+          zero();
         }
-        zero();
       }
       k.done_run(n);
     }
@@ -558,7 +572,12 @@ Ws ws_layout(int T, int heads, int kv, int D, int ctas) {
   return w;
 }
 
-bool paged_few(int D, int T, int r, int G) { return D <= 128 && (long)T * r <= 128L * std::max(G, 1); }
+// The kernel for few rows where a group has four tiles or less. Measured, few against many rows' kernel, us: decode of 64
+// sequences over a prefix of 32,768 tokens 40 against 44, over 24 prefixes 100 against 119; 32 groups of 3 questions of 40
+// tokens over 512 tokens 75 against 80; 512 rows over 16,000 keys 42 against 45 (D = 64: 38 against 37); 2,048 rows over
+// 16,000 keys 74 against 66, 8,192 rows 237 against 217. (8,192 rows over 4,000 keys would still gain, 84 against 92; how
+// long a prefix is the host does not know.) At D = 256 the accumulators of two CTAs do not fit.
+bool paged_few(int D, int T, int r, int G) { return D <= 128 && (long)T * r <= 512L * std::max(G, 1); }
 
 template <int D>
 int launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, PArgs a, bool few) {
@@ -569,7 +588,7 @@ int launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, PArgs a, b
   const cuuint32_t box[3] = {64, (cuuint32_t)a.r, (cuuint32_t)a.tpt};
   int rc = encode(&tq, Q, 3, dims, strides, box);
   if (rc) return rc;
-  if (few) {
+  if (few) {  // (D <= 128)
     rc = attn_few_launch(ctx, D, tq, c->mapK, c->mapV, a);
   } else {
     static uint64_t attr_done = 0;
@@ -582,11 +601,14 @@ int launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, PArgs a, b
     rc = dc_launch_check("attention_paged");
   }
   if (rc) return rc;
-  if (a.by_row)
-    DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D, 4>, dim3((unsigned)((long)a.T * a.heads)), dim3(128), 0, a));
-  else
-    DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D, 1>, dim3((unsigned)((std::min((long)a.T * a.r, 128L) + 3) / 4), a.ctas),
-                          dim3(128), 0, a));
+  if constexpr (D <= 128)
+    if (a.by_row) {
+      const dim3 grid((unsigned)((long)a.T * a.heads));
+      DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D, 4>, grid, dim3(128), 0, a));
+      return dc_launch_check("attention_paged (join)");
+    }
+  const dim3 grid((unsigned)((std::min((long)a.T * a.r, 128L) + 3) / 4), a.ctas);
+  DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D, 1>, grid, dim3(128), 0, a));
   return dc_launch_check("attention_paged (join)");
 }
 
@@ -623,9 +645,11 @@ int attn_paged_launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs,
   const int ctas = few ? 2 * ctx->sms : ctx->sms;
   a.tpt = 128 / a.r, a.page = c->page, a.pages = c->pages;
   a.pshift = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7, a.rows = c->pages * c->kv * c->page;
-  a.chunk_min = 2;
+  a.chunk_min = 2;  // no stretch is shorter, so that short calls have few parts (1 and 4 measured the same)
   a.ctas = ctas;
-  // few rows: most tiles are cut, into many parts
+  // Few rows: most tiles are cut, into many parts, and a join by row takes them up in four warps (one sequence over 30,000
+  // keys 29 us against 37 by tile, 64 over a shared prefix 40 against 48). Many: most rows were never cut, and blocks
+  // for all of them would cost more than the tiles' search (32 groups of 3 questions 43 us by tile, 53 by row).
   a.by_row = few && (long)T * heads <= 8192;
   a.scale_log2 = scale * 1.4426950408889634f;
   if (c->D == 64) return launch<64>(ctx, c, Q, qs, a, few);

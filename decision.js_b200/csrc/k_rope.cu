@@ -203,7 +203,8 @@ __global__ void __launch_bounds__(256, 3) kv_append_kernel(const AppendArgs a) {
           for (int e = 0; e < 8; e += 4) {
             float4 wx = make_float4(inv, inv, inv, inv), wy = wx;
             if (isq || isk) {
-              const float4 px = *reinterpret_cast<const float4 *>(w + 8 * ch.x + e), py = *reinterpret_cast<const float4 *>(w + 8 * ch.y + e);
+              const float4 px = *reinterpret_cast<const float4 *>(w + 8 * ch.x + e);
+              const float4 py = *reinterpret_cast<const float4 *>(w + 8 * ch.y + e);
               wx = make_float4(px.x * inv, px.y * inv, px.z * inv, px.w * inv);
               wy = make_float4(py.x * inv, py.y * inv, py.z * inv, py.w * inv);
             }
@@ -255,7 +256,8 @@ int ops_kv_append(dc_ctx *ctx, const dc_kv_cache *c, const dc_rope_plan *p, cons
   a.freq = p ? p->d_freq : nullptr, a.factor = p ? p->factor : 1.0f, a.rot = p ? p->rot : 0;
   a.err = ctx->d_err;
   a.zs = zs, a.qs = qs;
-  a.T = T, a.heads = heads, a.kv = c->kv, a.page = c->page, a.pshift = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7, a.nslots = c->pages * c->page;
+  a.T = T, a.heads = heads, a.kv = c->kv, a.page = c->page, a.nslots = c->pages * c->page;
+  a.pshift = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
   a.vnorm = vnorm, a.eps = eps;
   const int npass = (heads + 2 * c->kv + 512 / c->D - 1) / (512 / c->D);
   // warps per token: one, which works the angles out once for all heads, unless that leaves the card without warps

@@ -311,6 +311,17 @@ def test_attention_paged(ctx, dev, heads, kv, D, page, shape):
     c.check()
 
 
+@pytest.mark.parametrize("heads,kv,D,page", [h for h in HEADS if h[2] <= 128])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_attention_paged_with_rows_behind(ctx, dev, heads, kv, D, page, shape):
+    """The same sequences in front of rows that are nobody's, so many that the kernel for many rows takes the call."""
+    groups = SHAPES[shape]
+    c = Case(ctx, dev, groups, heads, kv, D, page, first=1, after=512 * len(groups) * kv // heads, seed=len(shape) + D)
+    c.call()
+    ctx.sync(60000)
+    c.check()
+
+
 @pytest.mark.parametrize("heads,kv,D,page", [(16, 8, 128, 16), (3, 1, 64, 64), (8, 2, 256, 128), (1, 1, 128, 32)])
 @pytest.mark.parametrize("n,plen,own", [(1, 9000, 2000), (64, 5003, 77), (3, 0, 7001)])
 def test_attention_paged_cut_over_many_ctas(ctx, dev, heads, kv, D, page, n, plen, own):
@@ -342,8 +353,8 @@ def test_attention_paged_many_sequences_and_groups(ctx, dev):
 
 def test_attention_paged_sharp_and_flat_rows(ctx, dev):
     """Weights from one key alone to all alike, growing and falling along the keys, a scale below zero."""
-    for i, qscale in enumerate((0.0, 0.01, 8.0, 60.0)):
-        c = Case(ctx, dev, [(900, [(3, 200), (1, 70)])], 8, 4, 128, 32, seed=i, qscale=qscale)
+    for i, (qscale, after) in enumerate(zip((0.0, 0.01, 8.0, 60.0) * 2, (0,) * 4 + (260,) * 4)):
+        c = Case(ctx, dev, [(900, [(3, 200), (1, 70)])], 8, 4, 128, 32, seed=i % 4, qscale=qscale, after=after)
         ramp = np.linspace(-3, 3, c.k.shape[0], dtype=np.float16)[:, None, None, None]
         for flip in (1, -1):
             c.k = (c.k * 0 + ramp * flip + c.k * np.float16(0.1)).astype(np.float16)
@@ -374,12 +385,12 @@ def test_attention_paged_weights_far_below_the_largest(ctx, dev):
     c.check()
 
 
-@pytest.mark.parametrize("D,heads,kv", [(128, 16, 8), (64, 4, 1), (256, 2, 1)])
+@pytest.mark.parametrize("D,heads,kv,after", [(128, 16, 8, 0), (64, 4, 1, 0), (256, 2, 1, 0), (128, 16, 8, 300), (64, 4, 1, 200)])
 @pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
-def test_attention_paged_keeps_broken_rows_apart(ctx, dev, D, heads, kv, value):
+def test_attention_paged_keeps_broken_rows_apart(ctx, dev, D, heads, kv, after, value):
     """A sequence whose last token has a key and a value that are not finite: its own earlier rows do not see them, nor
     do the other sequences of the tile; the row that sees them is not finite."""
-    c = Case(ctx, dev, [(100, [(5, 70), (9, 9), (1, 130), (3, 3)])], heads, kv, D, 16, seed=3)
+    c = Case(ctx, dev, [(100, [(5, 70), (9, 9), (1, 130), (3, 3)])], heads, kv, D, 16, seed=3, after=after)
     s, n = 1, 9
     p, off = c.table[s, (n - 1) // 16], (n - 1) % 16
     c.v[p, :, off, 3] = value
@@ -422,7 +433,8 @@ def test_attention_paged_in_place_and_repeatable(ctx, dev):
 @pytest.mark.parametrize("heads,kv,D,groups", [
     (16, 8, 128, [(5000 - 300 * g, [(1, 40 * i + 1) for i in range(12)]) for g in range(6)]),
     (32, 8, 64, [(3000, [(1, 70 * i) for i in range(9)]), (4111, [(1, 5)])]),
-    (24, 8, 128, [(2100, [(37, 37 + i) for i in range(20)])]), (8, 2, 256, [(1500, [(20, 90)] * 9)])])
+    (24, 8, 128, [(2100, [(37, 37 + i) for i in range(20)])]), (8, 2, 256, [(1500, [(20, 90)] * 9)]),
+    (32, 8, 64, [(700, [(80, 80 + i) for i in range(9)])] * 3)])
 def test_attention_paged_many_calls_in_a_row(ctx, dev, heads, kv, D, groups):
     """Two hundred calls without a wait between them, all the same bits: the roles within a CTA, which run at their own
     pace, never lose step (a wait that ran out would flag the next sync)."""
