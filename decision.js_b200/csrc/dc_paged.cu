@@ -29,11 +29,15 @@ static bool apart(const void *A, long as, long aw, const void *B, long bs, long 
   return d >= aw && d + bw <= as;
 }
 
+// Whether n rows of aw halves, as apart, from A lie outside `size` bytes from B.
+static bool outside(const void *A, long as, long aw, long n, const void *B, uintptr_t size) {
+  const uintptr_t a = (uintptr_t)A, ae = a + 2 * (uintptr_t)((n - 1) * as + aw), b = (uintptr_t)B;
+  return ae <= b || b + size <= a;
+}
+
+static uintptr_t cache_bytes(const dc_kv_cache *c) { return 2 * (uintptr_t)c->pages * c->kv * c->page * c->D; }
 static bool clear_of(const void *A, long as, long aw, long n, const dc_kv_cache *c) {
-  const uintptr_t a = (uintptr_t)A, ae = a + 2 * (uintptr_t)((n - 1) * as + aw);
-  const uintptr_t size = 2 * (uintptr_t)c->pages * c->kv * c->page * c->D;
-  const uintptr_t k = (uintptr_t)c->K, v = (uintptr_t)c->V;
-  return (ae <= k || k + size <= a) && (ae <= v || v + size <= a);
+  return outside(A, as, aw, n, c->K, cache_bytes(c)) && outside(A, as, aw, n, c->V, cache_bytes(c));
 }
 
 extern "C" int dc_rope_frequencies(int rot, double theta, int scaling, double factor, double trained, double a,
@@ -252,6 +256,10 @@ extern "C" int dc_attention_paged(dc_ctx *ctx, const dc_kv_cache *cache, const v
   const size_t need = attn_paged_ws(ctx, cache, T, heads);
   DC_CHECK(ws_bytes >= need, DC_EINVAL, "decision.js: attention_paged: a workspace of %zu bytes, %zu are needed",
            ws_bytes, need);
+  if (T > 0)
+    DC_CHECK(outside(Q, qs, w, T, ws, need) && outside(Y, ys, w, T, ws, need) &&
+                 clear_of(ws, (long)need, (long)((need + 1) / 2), 1, cache),
+             DC_EINVAL, "decision.js: attention_paged: the workspace overlaps Q, Y or the cache");
   if (T == 0 || S == 0) return DC_OK;
   dc_prof_begin(ctx, DC_K_ATTN, 0, 0);
   rc = attn_paged_launch(ctx, cache, Q, qs, table, tstride, lens, qoff, S, ptable, pstride, plens, goff, G, Y, ys, T,

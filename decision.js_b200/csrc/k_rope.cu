@@ -8,7 +8,9 @@
 // where the hardware's sine and cosine are off by 2^-20.9 at most: 1/500 of the rounding of the result to f16 (for a pair
 // of equal size; sincospif's 24 bits cost 300 instructions a lane and token, a sixth of the append).
 //
-// Both kernels read and write each row once and are bound by memory (many tokens) or by the launch (few).
+// Both kernels read and write each row once and are bound by memory (many tokens) or by the launch (few): the rotation of
+// 16,384 x 32 heads of 128 takes 42.9 us, 96% of the measured copy rate, the append of 16 x 1,024 tokens of 24 + 2 x 8 heads
+// 57.3 us, 90% of it; one token takes 1.8 and 2.7 us within a graph.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -138,7 +140,8 @@ struct AppendArgs {
 };
 
 // W warps per token; a pass of a warp covers 32 / (D/16) of the token's q, k and v heads, U = D/16 lanes to a head
-// (one unit each). NP passes are loaded at a time, the next NP while these are worked on.
+// (one unit each). NP passes are loaded at a time, the next NP while these are worked on: 16 x 1,024 tokens take 57 us with
+// two passes at three blocks an SM, 68 with four at two blocks, 63 with two at four, 70 with three at three.
 template <int D, bool INTER>
 __global__ void __launch_bounds__(256, 3) kv_append_kernel(const AppendArgs a) {
   dc_pdl_begin();
@@ -234,7 +237,9 @@ __global__ void __launch_bounds__(256, 3) kv_append_kernel(const AppendArgs a) {
 int ops_rope(dc_ctx *ctx, const dc_rope_plan *p, const void *X, long xs, const int *pos, void *Y, long ys, int T,
              int heads, int D) {
   const int U = D / 16;
-  // heads apart: 4 (a warp's threads cover 64 U halves in a row) unless that leaves the card without threads
+  // Heads apart: 4 (a warp's threads cover 64 U halves in a row) unless that leaves the card without threads. 16,384 x 32
+  // heads: 42.9 us with 4, 46.9 with 1, 69.8 with as many as fit (each thread works its angles out for fewer heads); one
+  // token of 32 heads 2.3 us with 4, 1.8 with as many as fit.
   const long want = (148L * 2048 / 2 + (long)T * U - 1) / ((long)T * U);
   const int most = std::max(1, std::min(heads, 256 / U));
   const int HS = (int)std::min<long>(most, std::max<long>(want, std::min(4, most)));
@@ -260,7 +265,9 @@ int ops_kv_append(dc_ctx *ctx, const dc_kv_cache *c, const dc_rope_plan *p, cons
   a.pshift = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
   a.vnorm = vnorm, a.eps = eps;
   const int npass = (heads + 2 * c->kv + 512 / c->D - 1) / (512 / c->D);
-  // warps per token: one, which works the angles out once for all heads, unless that leaves the card without warps
+  // Warps per token: one, which works the angles out once for all heads, unless that leaves the card without warps.
+  // 16 x 1,024 tokens of 24 + 2 x 8 heads: 57 us with one, 131 with a warp to every pass; one token 6.5 us with one, 2.7
+  // with a warp to every pass.
   a.W = (int)std::max<long>(1, std::min<long>(npass, (148L * 32 + T - 1) / T));
   const dim3 grid((unsigned)(((long)T * a.W + 7) / 8));
   const bool inter = p && p->layout == DC_ROPE_INTERLEAVED;

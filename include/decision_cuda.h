@@ -308,9 +308,9 @@ DC_API int dc_kv_cache_free(dc_kv_cache *cache);
  * (eps added to the mean square), then q and k turn by `plan` (NULL: not at all) to position d_pos[t] (NULL without a
  * plan). q goes to row t of Q (qstride halves), k and v to slot d_slots[t] of the cache; all in f32, rounded to f16
  * once. A negative slot stores no k and v (its q is made); one past the cache does the same and flags the device error
- * word (the next dc_sync returns DC_EINVAL). The slots of a call must differ: of two tokens at one slot either may
- * stay. Q may be Z itself (same stride: q in place); another overlap of Q with Z, or of the cache with either, is
- * DC_EINVAL. zstride and qstride are multiples of 8; pointers 16-byte aligned, d_pos and d_slots 4-byte. */
+ * word (the next dc_sync returns DC_EINVAL). The slots of a call must differ: of two tokens at one slot, parts of
+ * either may stay. Q may be Z itself (same stride: q in place); another overlap of Q with Z, or of the cache with
+ * either, is DC_EINVAL. zstride and qstride are multiples of 8; pointers 16-byte aligned, d_pos and d_slots 4-byte. */
 DC_API int dc_kv_append(dc_ctx *ctx, const dc_kv_cache *cache, const dc_rope_plan *plan, const void *d_Z, long zstride,
                         const void *d_qn, const void *d_kn, float eps, int vnorm, const int32_t *d_pos,
                         const int32_t *d_slots, void *d_Q, long qstride, int T, int heads);
@@ -321,15 +321,15 @@ DC_API int dc_kv_append(dc_ctx *ctx, const dc_kv_cache *cache, const dc_rope_pla
  * d_ptable[g * ptable_stride + i]; G = 0: no prefixes. Query row i of the n of a sequence reads its group's whole
  * prefix and its own tokens [0, lens - n + 1 + i): its last query row sees all, as after dc_kv_append of the n rows
  * (fewer own tokens than rows leave the first rows none). Y (ystride halves a row) gets softmax(scale q . k) v, heads
- * by GQA as in dc_attention; a row with no key gets zeros. Rows outside [d_qoff[0], d_qoff[S]) are neither read nor
- * written, nor is anything of the cache past a length. Scores, sums and outputs are f32; the weights are rounded to
- * f16 for the product with v. A value row that is not finite stays out of the rows that do not see it; those that do
+ * by GQA as in dc_attention; a row with no key gets zeros. Rows outside [d_qoff[0], d_qoff[S]) are not written and
+ * have no influence (rows next to a sequence's may be fetched with it), nor has anything of the cache past a length.
+ * Scores and sums are f32; the weights are rounded to f16 for the product with v, the output to f16 once. A value row that is not finite stays out of the rows that do not see it; those that do
  * get NaN in its columns or in the whole head.
  * Offsets must not fall, qoff must lie in [0, T], goff start at 0 and end at S, lens and plens fit their table's row;
  * otherwise nothing is written, and the next dc_sync returns DC_EINVAL, as it does for a page id outside the cache
- * (which reads zeros). Unused table entries are not read. Q and Y must not overlap unless Y is Q with its stride.
- * d_ws: at least dc_attention_paged_workspace bytes, 16-byte aligned, for this call alone until it has run (calls on
- * one stream can share it; graphs that may run at the same time cannot). heads / kv at most 64; strides are multiples
+ * (which reads zeros). Table entries past a length may hold anything. Q and Y must not overlap unless Y is Q with its
+ * stride. d_ws: at least dc_attention_paged_workspace bytes, 16-byte aligned, apart from Q, Y and the cache, for this
+ * call alone until it has run (calls on one stream can share it; graphs that may run at the same time cannot). heads / kv at most 64; strides are multiples
  * of 8; Q, Y 16-byte aligned. Runs of one input give the same bits. */
 DC_API int dc_attention_paged(dc_ctx *ctx, const dc_kv_cache *cache, const void *d_Q, long qstride,
                               const int32_t *d_table, int table_stride, const int32_t *d_lens, const int32_t *d_qoff,

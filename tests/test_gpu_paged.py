@@ -451,6 +451,28 @@ def test_attention_paged_many_calls_in_a_row(ctx, dev, heads, kv, D, groups):
     c.check(rows={0, c.T - 1})
 
 
+def test_attention_paged_from_two_contexts_at_once(ctx, dev, pkg):
+    """Calls of two contexts side by side on the device, of both kernels, each with its own workspace and cache."""
+    import torch
+    cases = [Case(ctx, dev, [(2000, [(1, 40 * i + 1) for i in range(12)])], 16, 8, 128, 32, seed=1),
+             Case(ctx, dev, [(900, [(60, 60 + i) for i in range(8)])], 32, 8, 64, 32, seed=2)]
+    firsts = []
+    for c in cases:
+        c.call()
+        ctx.sync(60000)
+        c.check(rows={0, c.T - 1})
+        firsts.append(c.y.clone())
+    torch.cuda.synchronize()
+    other = pkg.Context(0)
+    for i in range(60):
+        cases[0].call()
+        cases[1].call(ctx=other)
+        if i % 20 == 19:
+            ctx.sync(60000), other.sync(60000)
+            assert all(torch.equal(c.y, f) for c, f in zip(cases, firsts))
+    other.close()
+
+
 def test_attention_paged_refuses_bad_arrays(ctx, dev, pkg):
     """Offsets that fall, reach past their table or rows: nothing is written, the next sync says so, and the context
     works on."""
@@ -482,6 +504,29 @@ def test_attention_paged_refuses_bad_arrays(ctx, dev, pkg):
     c.call()
     ctx.sync(60000)
     c.check()
+
+
+def test_attention_paged_refuses_a_workspace_in_its_tensors(ctx, dev, pkg):
+    import torch
+    c = Case(ctx, dev, [(20, [(2, 30)])], 4, 2, 64, 16)
+    c.call()
+    ctx.sync(60000)
+    n = c.ws.numel() + (1 << 16)
+    big = torch.zeros(2 * n, dtype=torch.uint8, device=dev)
+    inside = big[n - 256:]
+    for name in ("dq", "y"):
+        mine = big[n - 2 * c.T * 256:].view(torch.float16)[:c.T * 256].view(c.T, 256)
+        was, ws = getattr(c, name), c.ws
+        setattr(c, name, mine), setattr(c, "ws", inside[:ws.numel()])
+        with pytest.raises(pkg.DecisionError) as e:
+            c.call()
+        assert e.value.code == 1 and "workspace overlaps" in str(e.value)
+        setattr(c, name, was), setattr(c, "ws", ws)
+    k, v = torch.zeros(2, n // 512 + 1, 2, 16, 64, dtype=torch.float16, device=dev)
+    c.cache, c.ws = ctx.kv_cache(k, v), v.view(-1).view(torch.uint8)[:c.ws.numel()]
+    with pytest.raises(pkg.DecisionError) as e:
+        c.call()
+    assert e.value.code == 1 and "workspace overlaps" in str(e.value)
 
 
 def test_attention_paged_in_a_graph(ctx, dev):
@@ -581,6 +626,37 @@ def test_append_then_attend_as_a_decoder_does(ctx, dev, pkg):
         got = _f64(y).reshape(T, heads, D)
         for t, (a, size) in want.items():
             _within(got[t], a, R.HALF_STEP * np.abs(a) + 3 * R.HALF_STEP * size + SMALL)
+
+
+def test_far_pages_of_a_long_cache(ctx, dev, pkg):
+    """Pages past 2^32 elements of K and of V: the same answers, to the bit, as from a cache of a few pages."""
+    import torch
+    heads, kv, D, page, far = 16, 8, 128, 64, 66_000  # 65,536 elements a page
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("two caches of 8.7 GB")
+    c = Case(ctx, dev, [(150, [(1, 70), (3, 64), (2, 1)])], heads, kv, D, page, seed=6)
+    n = len(c.k)
+    k, v = (torch.empty((far, kv, page, D), dtype=torch.float16, device=dev) for _ in range(2))
+    k[-n:].copy_(c.dk), v[-n:].copy_(c.dv)
+    cache = ctx.kv_cache(k, v)
+    z = torch.randn((6, (heads + 2 * kv) * D), device=dev).half()
+    q = [torch.empty((6, heads * D), dtype=torch.float16, device=dev) for _ in range(2)]
+    own = [(s, lo - m + i) for s, (m, lo) in enumerate([(1, 70), (3, 64), (2, 1)]) for i in range(m)]
+    slots = [-1 if at < 0 else int(c.table[s, at // page]) * page + at % page for s, at in own]
+    far_slots = [x if x < 0 else x + (far - n) * page for x in slots]
+    torch.cuda.synchronize()
+    y = [c.y, torch.full_like(c.y, 55.0)]
+    tables = [torch.where((c.meta[t] >= 0) & (c.meta[t] < n), c.meta[t] + far - n, c.meta[t]) for t in ("table", "ptable")]
+    for i, (kc, sl, (table, ptable)) in enumerate([(c.cache, slots, (c.meta["table"], c.meta["ptable"])), (cache, far_slots, tables)]):
+        sl = _i32(sl, dev)
+        torch.cuda.synchronize()
+        ctx.call("kv_append", kc, None, z, z.shape[1], None, None, 0.0, 0, None, sl, q[i], heads * D, 6, heads)
+        m = c.meta
+        ctx.call("attention_paged", kc, q[i], heads * D, table, table.shape[1], m["lens"], m["qoff"], 3, ptable, ptable.shape[1],
+                 m["plens"], m["goff"], 1, y[i], heads * D, 6, heads, c.scale, c.ws, c.ws.numel())
+        ctx.sync(60000)
+    assert torch.equal(q[0], q[1]) and torch.equal(y[0], y[1]) and torch.isfinite(y[0]).all() and (y[0] != 55.0).any()
+    assert torch.equal(k[-n:].nan_to_num(7), c.dk.nan_to_num(7)) and torch.equal(v[-n:].nan_to_num(7), c.dv.nan_to_num(7))
 
 
 @pytest.mark.parametrize("D,heads,kv", [(128, 16, 8), (64, 32, 8), (256, 8, 2)])
