@@ -134,10 +134,6 @@ def ptr(x) -> int | None:
     address = getattr(x, "data_ptr", None)
     if address is not None:
         return address()
-    if isinstance(x, _Handle):
-        if not x.h:
-            raise DecisionError(DC_EINVAL, f"decision.js: a closed {type(x).__name__}")
-        return x.h.value
     if hasattr(x, "ctypes"):
         return x.ctypes.data
     raise TypeError(type(x))
@@ -172,6 +168,11 @@ class _Handle:
 
     h = None
     _free = ""
+
+    def data_ptr(self) -> int:
+        if not self.h:
+            raise DecisionError(DC_EINVAL, f"decision.js: a closed {type(self).__name__}")
+        return self.h.value
 
     def close(self):
         if self.h:
@@ -233,7 +234,11 @@ class Context:
 
     def call(self, name: str, *args):
         """Calls dc_<name>(ctx, *args), converting tensors / arrays to addresses, and raises on failure."""
-        rc = getattr(lib(), "dc_" + name)(self.h, *[a if type(a) in _PLAIN else ptr(a) for a in args])
+        try:  # (a call's conversions are a good part of its time from the host)
+            args = [a if type(a) in _PLAIN else a.data_ptr() for a in args]
+        except AttributeError:
+            args = [a if type(a) in _PLAIN else ptr(a) for a in args]
+        rc = getattr(lib(), "dc_" + name)(self.h, *args)
         if rc:
             check(rc)
 
