@@ -13,7 +13,8 @@
 namespace dcx {
 
 constexpr int PA_RING = 4;    // runs handed out ahead
-constexpr int PA_GOFF = 512;  // groups whose offsets are kept in shared memory
+constexpr int PA_GOFF = 512;  // groups and sequences whose offsets and lengths are kept in shared memory
+constexpr int PA_META = 4 * (PA_GOFF + 4) * 4;  // bytes
 
 enum { RUN_FIRST = 1, RUN_LAST = 2, RUN_TFIRST = 4, RUN_TLAST = 8, RUN_END = 16 };
 
@@ -63,10 +64,9 @@ __device__ __forceinline__ int own_limit(int t, int qe, int len) { return max(le
 template <int KB>
 __device__ __forceinline__ int blocks_of(int keys) { return (keys + KB - 1) / KB; }
 
-struct Groups {  // offsets, prefix lengths and first rows, from shared memory when they fit
-  const int *goff, *plens, *rows;
-  int G;
-  int2 whole;  // without groups: all rows
+struct Groups {  // offsets and lengths of groups and sequences, from shared memory when they fit
+  const int *goff, *plens, *qoff, *lens;
+  int G, S;
   __device__ __forceinline__ int of(int s) const {  // the last g with goff[g] <= s
     int lo = 0, hi = G;
     while (hi - lo > 1) {
@@ -81,11 +81,9 @@ struct Group {
   int tg, te, pb;  // its rows, its prefix's blocks
 };
 template <int KB>
-__device__ __forceinline__ Group group_of(const PArgs &a, const Groups &gs, int g) {
-  if (gs.G == 0) return Group{gs.whole.x, gs.whole.y, 0};
-  const int pb = blocks_of<KB>(gs.plens[g]);
-  if (gs.rows) return Group{gs.rows[g], gs.rows[g + 1], pb};
-  return Group{a.qoff[min(max(gs.goff[g], 0), a.S)], a.qoff[min(max(gs.goff[g + 1], 0), a.S)], pb};
+__device__ __forceinline__ Group group_of(const Groups &gs, int g) {
+  if (gs.G == 0) return Group{gs.qoff[0], gs.qoff[gs.S], 0};
+  return Group{gs.qoff[min(max(gs.goff[g], 0), gs.S)], gs.qoff[min(max(gs.goff[g + 1], 0), gs.S)], blocks_of<KB>(gs.plens[g])};
 }
 
 // The units of a sequence: for each tile its rows touch, the prefix's blocks if the tile starts in it, and its own.
@@ -119,14 +117,17 @@ struct Blocks {
     return a.rows;  // past the cache: zeros
   }
   __device__ __forceinline__ int ld(const PArgs &a, int i) const { return i < count ? row_of(a, tab[i]) : a.rows; }
-  // `ahead`: the ids of the first 32 pages of sequence ahead_seq, if they were read already
+  // `ahead`: the ids of the first 32 pages of sequence ahead_seq, if they were read already. The ids are on their way
+  // until settle() looks at them.
   __device__ __forceinline__ void start(const PArgs &a, const Run &r, int lane, int ahead_seq, int ahead) {
     tab = r.tab, kend = r.kend, kvh = r.kvh, count = (kend + a.page - 1) >> a.pshift, base = (r.kb * KB) >> a.pshift;
-    if (r.seg >= 0 && r.seg == ahead_seq && base == 0)
-      cur = lane < count ? row_of(a, ahead) : a.rows;
-    else
-      cur = ld(a, base + lane);
-    nxt = base + 32 < count ? ld(a, base + 32 + lane) : a.rows;
+    const bool have = r.seg >= 0 && r.seg == ahead_seq && base == 0;
+    cur = have ? ahead : base + lane < count ? tab[base + lane] : 0;
+    nxt = base + 32 + lane < count ? tab[base + 32 + lane] : 0;
+  }
+  __device__ __forceinline__ void settle(const PArgs &a, int lane) {
+    cur = base + lane < count ? row_of(a, cur) : a.rows;
+    nxt = base + 32 + lane < count ? row_of(a, nxt) : a.rows;
   }
   // The whole warp: block `kb`'s rows, one per box of min(page, 64) rows (boxes that hold none of the run's keys are
   // left out).
@@ -218,24 +219,25 @@ __device__ __forceinline__ bool line_start(const Cta<C> &k, Groups &gs, Stretch 
   int *s_start = k.start(), *s_goff = reinterpret_cast<int *>(k.smem + C::GOFF_OFF);
   long *s_scan = reinterpret_cast<long *>(k.smem + C::SCAN_OFF);
   bool bad = false;
-  gs = Groups{a.goff, a.plens, nullptr, a.G};
-  if (a.G > 0) {
-    if (a.G <= PA_GOFF) {  // offsets, prefix lengths and first rows into shared memory
-      for (int i = tid; i <= a.G; i += C::THREADS) {
-        const int x = a.goff[i];
-        s_goff[i] = x;
-        s_goff[2 * (PA_GOFF + 4) + i] = a.qoff[min(max(x, 0), a.S)];
-        if (i < a.G) s_goff[PA_GOFF + 4 + i] = a.plens[i];
-      }
-      gs = Groups{s_goff, s_goff + PA_GOFF + 4, s_goff + 2 * (PA_GOFF + 4), a.G};
+  gs = Groups{a.goff, a.plens, a.qoff, a.lens, a.G, a.S};
+  // into shared memory, all in one round of loads
+  int *s_plens = s_goff + PA_GOFF + 4, *s_qoff = s_plens + PA_GOFF + 4, *s_lens = s_qoff + PA_GOFF + 4;
+  if (a.S <= PA_GOFF) {
+    for (int i = tid; i <= a.S; i += C::THREADS) {
+      s_qoff[i] = a.qoff[i];
+      if (i < a.S) s_lens[i] = a.lens[i];
     }
-  } else {
-    gs.whole = make_int2(a.qoff[0], a.qoff[a.S]);
+    gs.qoff = s_qoff, gs.lens = s_lens;
+  }
+  if (a.G > 0 && a.G <= PA_GOFF) {
+    for (int i = tid; i <= a.G; i += C::THREADS) {
+      s_goff[i] = a.goff[i];
+      if (i < a.G) s_plens[i] = a.plens[i];
+    }
+    gs.goff = s_goff, gs.plens = s_plens;
   }
   const int per = (a.S + C::THREADS - 1) / C::THREADS;
   const int sb = min(tid * per, a.S), se = min(sb + per, a.S);
-  int qb = 0, qe = 0, len = 0;  // the thread's (first) sequence
-  if (sb < se) qb = a.qoff[sb], qe = a.qoff[sb + 1], len = a.lens[sb];
   __syncthreads();
   dc_pdl_launch_dependents();
   if (a.G > 0) {
@@ -248,12 +250,12 @@ __device__ __forceinline__ bool line_start(const Cta<C> &k, Groups &gs, Stretch 
   // a sequence's units; nothing for offsets that are refused below (the sum is then not used)
   auto units = [&](int s, int qb, int qe, int len) -> long {
     if (qb < 0 || qe <= qb || qe > a.T || len < 0) return 0;
-    const Group g = group_of<KB>(a, gs, a.G ? gs.of(s) : 0);
+    const Group g = group_of<KB>(gs, a.G ? gs.of(s) : 0);
     return g.tg < 0 || g.tg > qb ? 0 : seq_cost<KB>(a.tpt, g, qb, qe, len);
   };
   long mine = 0;
   for (int s = sb; s < se; s++) {
-    const int x = s == sb ? qb : a.qoff[s], y = s == sb ? qe : a.qoff[s + 1], n = s == sb ? len : a.lens[s];
+    const int x = gs.qoff[s], y = gs.qoff[s + 1], n = gs.lens[s];
     bad |= x < 0 || y < x || y > a.T || n < 0 || n > (long)a.tstride * a.page || n > (1 << 30);
     mine += units(s, x, y, n);
   }
@@ -296,7 +298,7 @@ __device__ __forceinline__ bool line_start(const Cta<C> &k, Groups &gs, Stretch 
     if (off >= 0 && off < mine) {
       int s = sb;
       for (; s < se - 1; s++) {
-        const long c = units(s, a.qoff[s], a.qoff[s + 1], a.lens[s]);
+        const long c = units(s, gs.qoff[s], gs.qoff[s + 1], gs.lens[s]);
         if (off < c) break;
         off -= c;
       }
@@ -318,27 +320,27 @@ __device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, con
   bool ok = true, first = true;
   long pos = st.p0, off = (long)(uint32_t)s_start[1] | (long)s_start[2] << 32;  // on the line; in the sequence's pieces
   int s = s_start[0], kvh = st.kvh, gi = a.G ? gs.of(s) : 0;
-  Group gr = group_of<KB>(a, gs, gi);
-  int qb = a.qoff[s], qe = a.qoff[s + 1], len = a.lens[s];
+  Group gr = group_of<KB>(gs, gi);
+  int qb = gs.qoff[s], qe = gs.qoff[s + 1], len = gs.lens[s];
   int lo = qb - gr.tg, hi = qe - gr.tg, ts = lo / a.tpt * a.tpt;  // from the group's first row; ts: the piece's tile
   // the next sequence's offset, length and first pages, on their way while this one's blocks are loaded
-  int nqe = s + 1 < a.S ? a.qoff[s + 2] : 0, nlen = s + 1 < a.S ? a.lens[s + 1] : 0;
+  int nqe = s + 1 < a.S ? gs.qoff[s + 2] : 0, nlen = s + 1 < a.S ? gs.lens[s + 1] : 0;
   int ahead_seq = -1, ahead = 0, coming = read_ahead(a, s + 1, lane);
   auto advance = [&]() {
     do {
       if (++s == a.S) {
         s = 0, kvh++, gi = 0;
-        qb = a.qoff[0], qe = a.qoff[1], len = a.lens[0];
+        qb = gs.qoff[0], qe = gs.qoff[1], len = gs.lens[0];
         ahead_seq = -1;
       } else {
         qb = qe, qe = nqe, len = nlen;
         ahead_seq = s, ahead = coming;
       }
-      if (s + 1 < a.S) nqe = a.qoff[s + 2], nlen = a.lens[s + 1];
+      if (s + 1 < a.S) nqe = gs.qoff[s + 2], nlen = gs.lens[s + 1];
       coming = read_ahead(a, s + 1, lane);
     } while (qe <= qb && kvh < a.kv);
     while (gi + 1 < a.G && gs.goff[gi + 1] <= s) gi++;
-    gr = group_of<KB>(a, gs, gi);
+    gr = group_of<KB>(gs, gi);
     lo = qb - gr.tg, hi = qe - gr.tg, ts = lo / a.tpt * a.tpt;
   };
   while (pos < st.p1 && kvh < a.kv) {
@@ -370,6 +372,8 @@ __device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, con
     if (r.nb == 0 && !(r.flags & (RUN_FIRST | RUN_LAST))) continue;  // (a run in a tile's midst always has blocks)
     if (first) item++;
     r.item = item;
+    Blocks<C> bl;
+    bl.start(a, r, lane, use_seq, use);
     if (!(ok = k.wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1))) break;
     if (lane == 0) {
       k.runs()[n % PA_RING] = r;
@@ -377,8 +381,6 @@ __device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, con
     }
     n++;
     __syncwarp();
-    Blocks<C> bl;
-    bl.start(a, r, lane, use_seq, use);
     if (first) {
       if (!(ok = k.wait_warp(C::B_QE, item + 1))) break;
       if (elect_one()) {
@@ -388,6 +390,7 @@ __device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, con
       }
       __syncwarp();
     }
+    bl.settle(a, lane);
     for (int b = 0; b < r.nb; b++, g++) {
       const int stage = g % KST;
       const typename Blocks<C>::Rows x = bl.rows(a, r.kb + b, lane);
@@ -417,6 +420,7 @@ __device__ __forceinline__ void load_values(const Cta<C> &k, const CUtensorMap *
     if (r.nb > 0) {
       Blocks<C> bl;
       bl.start(a, r, lane, ahead_seq, ahead);
+      bl.settle(a, lane);
       ahead_seq = r.seg < 0 ? r.s : r.s + 1, ahead = read_ahead(a, ahead_seq, lane);  // what usually comes next
       for (int b = 0; b < r.nb; b++, g++) {
         const int st = g % VST;

@@ -42,7 +42,7 @@ struct FewCfg {
   static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15);
   static constexpr int POISON_OFF = MISC_OFF + 32, SCAN_OFF = POISON_OFF + 64,
                        RUN_OFF = SCAN_OFF + ((F_THREADS / 32 * 8 + 15) & ~15), GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run),
-                       XCH_OFF = GOFF_OFF + 3 * (PA_GOFF + 4) * 4;  // floats [2 turns][2 halves][128 rows]
+                       XCH_OFF = GOFF_OFF + PA_META;  // floats [2 turns][2 halves][128 rows]
   static constexpr int SMEM = XCH_OFF + 2 * 2 * 128 * 4 + 1024;
   static constexpr int S_COL = 0, O_COL = SB * KB, TCOLS = 256;
   static_assert(O_COL + D <= TCOLS, "tensor memory");

@@ -74,7 +74,7 @@ struct WideCfg {
   // misc: tmem slot, abort, start (s, offset); poison; scan; runs; groups; references and sums
   static constexpr int POISON_OFF = MISC_OFF + 32, SCAN_OFF = POISON_OFF + 64,
                        RUN_OFF = SCAN_OFF + ((PA_THREADS / 32 * 8 + 15) & ~15), GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run),
-                       XCH_OFF = GOFF_OFF + 3 * (PA_GOFF + 4) * 4;
+                       XCH_OFF = GOFF_OFF + PA_META;
   static constexpr int SMEM = XCH_OFF + 128 * 4 + 4 * PA_WG * 128 * 8 + 1024;
   static constexpr int S_COL = 0, O_COL = PA_WG * KB;  // tensor memory: a scores' buffer per warpgroup, the accumulator
   static constexpr int TCOLS = 512;
@@ -457,6 +457,20 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PArgs a) {
     t = tile.x + i, h = tile.z * a.r + row - i * a.r;
     base = ((long)tile.z * a.T + tile.x) * a.r + row;
   }
+  auto fetch = [&](float (&v)[N], int c) {
+    const float *p = a.O + (base + 128L * c) * D + N * lane;
+    if (N == 2) {
+      *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; e += 4) *reinterpret_cast<float4 *>(v + e) = *reinterpret_cast<const float4 *>(p + e);
+    }
+  };
+  // the first parts' values are on their way with their weights, whether those turn out 0 (and nothing was stored) or not
+  float v[4][N];
+#pragma unroll
+  for (int k = 0; k < 4; k++)
+    if (c0 + part + W * k <= c1) fetch(v[k], c0 + part + W * k);
   float M = -FLT_MAX, L = 0.f, o[N] = {};
   for (int cb = c0 + part; cb <= c1; cb += 32 * W) {  // 32 parts at a time, usually all
     const int c = cb + W * lane;
@@ -472,23 +486,28 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PArgs a) {
 #pragma unroll
     for (int e = 0; e < N; e++) o[e] *= f;
     uint32_t have = __ballot_sync(0xffffffffu, x.y != 0.f);
+    if (cb == c0 + part) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const float wk = __shfl_sync(0xffffffffu, w, k);
+        if ((have >> k) & 1u)
+#pragma unroll
+          for (int e = 0; e < N; e++) o[e] = fmaf(wk, v[k][e], o[e]);
+      }
+      have &= ~15u;
+    }
     while (have) {  // four parts' values on their way
-      float v[4][N], wk[4];
+      float wk[4];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         const int at = have ? __ffs(have) - 1 : 0;
-        const float *p = a.O + (base + 128L * (cb + W * at)) * D + N * lane;
         wk[k] = __shfl_sync(0xffffffffu, w, at);
 #pragma unroll
         for (int e = 0; e < N; e++) v[k][e] = 0.f;
-        if (have) {
-          if (N == 2) {
-            *reinterpret_cast<float2 *>(v[k]) = *reinterpret_cast<const float2 *>(p);
-          } else {
-#pragma unroll
-            for (int e = 0; e < N; e += 4) *reinterpret_cast<float4 *>(v[k] + e) = *reinterpret_cast<const float4 *>(p + e);
-          }
-        }
+        if (have)
+          fetch(v[k], cb + W * at);
+        else
+          wk[k] = 0.f;
         have &= have - 1;
       }
 #pragma unroll
