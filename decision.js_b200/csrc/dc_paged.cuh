@@ -69,6 +69,7 @@ struct Groups {  // offsets and lengths of groups and sequences, from shared mem
   int G, S;
   __device__ __forceinline__ int of(int s) const {  // the last g with goff[g] <= s
     int lo = 0, hi = G;
+#pragma unroll 1
     while (hi - lo > 1) {
       const int m = (lo + hi) >> 1;
       if (goff[m] <= s) lo = m; else hi = m;
@@ -88,10 +89,11 @@ __device__ __forceinline__ Group group_of(const Groups &gs, int g) {
 
 // The units of a sequence: for each tile its rows touch, the prefix's blocks if the tile starts in it, and its own.
 template <int KB>
-static __device__ __noinline__ long seq_cost(int tpt, Group g, int qb, int qe, int len) {
+static __device__ __forceinline__ long seq_cost(int tpt, Group g, int qb, int qe, int len) {
   long c = 0;
   const int lo = qb - g.tg, hi = qe - g.tg;
   if (hi <= lo) return 0;
+#pragma unroll 1
   for (int ts = lo / tpt * tpt; ts < hi; ts += tpt) {
     if (ts >= lo) c += g.pb;
     c += max(1, blocks_of<KB>(own_limit(g.tg + min(hi, ts + tpt) - 1, qe, len)));
@@ -223,6 +225,7 @@ __device__ __forceinline__ bool line_start(const Cta<C> &k, Groups &gs, Stretch 
   // into shared memory, all in one round of loads
   int *s_plens = s_goff + PA_GOFF + 4, *s_qoff = s_plens + PA_GOFF + 4, *s_lens = s_qoff + PA_GOFF + 4;
   if (a.S <= PA_GOFF) {
+#pragma unroll 1
     for (int i = tid; i <= a.S; i += C::THREADS) {
       s_qoff[i] = a.qoff[i];
       if (i < a.S) s_lens[i] = a.lens[i];
@@ -230,6 +233,7 @@ __device__ __forceinline__ bool line_start(const Cta<C> &k, Groups &gs, Stretch 
     gs.qoff = s_qoff, gs.lens = s_lens;
   }
   if (a.G > 0 && a.G <= PA_GOFF) {
+#pragma unroll 1
     for (int i = tid; i <= a.G; i += C::THREADS) {
       s_goff[i] = a.goff[i];
       if (i < a.G) s_plens[i] = a.plens[i];
@@ -241,6 +245,7 @@ __device__ __forceinline__ bool line_start(const Cta<C> &k, Groups &gs, Stretch 
   __syncthreads();
   dc_pdl_launch_dependents();
   if (a.G > 0) {
+#pragma unroll 1
     for (int i = tid; i < a.G; i += C::THREADS) {
       const int x = gs.goff[i], y = gs.goff[i + 1], n = gs.plens[i];
       bad |= x < 0 || y < x || y > a.S || n < 0 || n > (long)a.pstride * a.page || n > (1 << 30);
@@ -254,6 +259,7 @@ __device__ __forceinline__ bool line_start(const Cta<C> &k, Groups &gs, Stretch 
     return g.tg < 0 || g.tg > qb ? 0 : seq_cost<KB>(a.tpt, g, qb, qe, len);
   };
   long mine = 0;
+#pragma unroll 1
   for (int s = sb; s < se; s++) {
     const int x = gs.qoff[s], y = gs.qoff[s + 1], n = gs.lens[s];
     bad |= x < 0 || y < x || y > a.T || n < 0 || n > (long)a.tstride * a.page || n > (1 << 30);
@@ -284,19 +290,22 @@ __device__ __forceinline__ bool line_start(const Cta<C> &k, Groups &gs, Stretch 
   const long B = line * a.kv;
   long chunk;
   st.kvh = 0;
-  if (B < 0x7fff0000) {  // (64-bit divisions take a microsecond)
-    chunk = max((unsigned)a.chunk_min, ((unsigned)B + gridDim.x - 1) / gridDim.x);
-    st.p0 = chunk * blockIdx.x;
-    if (st.p0 < B) st.kvh = (unsigned)st.p0 / (unsigned)line;
-  } else {
-    chunk = (B + gridDim.x - 1) / gridDim.x, st.p0 = chunk * blockIdx.x;
-    if (st.p0 < B) st.kvh = (int)(st.p0 / line);
+  const int sh = B < 0x7fff0000 ? 0 : 16;  // (64-bit divisions take a microsecond)
+  chunk = max((long)a.chunk_min, (long)(((unsigned)(B >> sh) + gridDim.x - (sh ? 0 : 1)) / gridDim.x) << sh);
+  st.p0 = chunk * blockIdx.x;
+  if (st.p0 < B) {
+    if (sh == 0)
+      st.kvh = (unsigned)st.p0 / (unsigned)line;
+    else
+#pragma unroll 1
+      while (line * (st.kvh + 1) <= st.p0) st.kvh++;
   }
   st.p1 = min(st.p0 + chunk, B);
   if (st.p0 < st.p1 && mine > 0) {
     long off = st.p0 - st.kvh * line - before;
     if (off >= 0 && off < mine) {
       int s = sb;
+#pragma unroll 1
       for (; s < se - 1; s++) {
         const long c = units(s, gs.qoff[s], gs.qoff[s + 1], gs.lens[s]);
         if (off < c) break;
