@@ -43,7 +43,7 @@ struct PArgs {
   float *O;
   uint32_t *err;
   long ystride;
-  int tstride, pstride, S, G, T, heads, kv, r, tpt, page, pshift, pages, rows, chunk_min, ctas, by_row;
+  int tstride, pstride, S, G, T, heads, kv, r, tpt, page, pshift, pages, rows, chunk_min, ctas, by_row, y32;
   float scale_log2;
 };
 
@@ -53,10 +53,20 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t lbo) {
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-__device__ __forceinline__ void st_global_v8(float *p, const uint32_t *r) {
+__device__ __forceinline__ void st_global_v8(void *p, const uint32_t *r) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
+}
+
+// 16 values of a row of Y: whole 32-byte sectors where Y's rows begin at them (y32).
+__device__ __forceinline__ void store_row16(__half *y, const uint32_t *w, int y32) {
+  if (y32) {
+    st_global_v8(y, w);
+  } else {
+    reinterpret_cast<uint4 *>(y)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4 *>(y)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
 }
 
 // own keys that query row `t` of a sequence [.., qe) with `len` own tokens sees
@@ -106,6 +116,8 @@ __device__ __forceinline__ int read_ahead(const PArgs &a, int s, int lane) {
   return s < a.S && lane < a.tstride ? a.table[(long)s * a.tstride + lane] : 0;
 }
 
+static __device__ __noinline__ void bad_page(uint32_t *err) { atomicOr(err, (uint32_t)DC_DEVERR_BOUNDS); }
+
 // A run's blocks for a producer warp: page ids are read 32 at a time, the next 32 on their way, and turned into rows of
 // the cache as tensor-map coordinates before the stage is waited for.
 template <class C>
@@ -114,8 +126,8 @@ struct Blocks {
   const int *tab;
   int base, count, cur, nxt, kend, kvh;
   __device__ __forceinline__ int row_of(const PArgs &a, int id) const {
-    if (id >= 0 && id < a.pages) return (id * a.kv + kvh) << a.pshift;
-    atomicOr(a.err, (uint32_t)DC_DEVERR_BOUNDS);
+    if ((unsigned)id < (unsigned)a.pages) return (id * a.kv + kvh) << a.pshift;
+    bad_page(a.err);
     return a.rows;  // past the cache: zeros
   }
   __device__ __forceinline__ int ld(const PArgs &a, int i) const { return i < count ? row_of(a, tab[i]) : a.rows; }
@@ -373,16 +385,11 @@ __device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, con
     r.flags = (first ? RUN_FIRST : 0) | (off == 0 && starts ? RUN_TFIRST : 0) |
               (done || pos + units == st.p1 ? RUN_LAST : 0) | (done ? RUN_TLAST : 0);
     pos += units, off += units;
-    const int use_seq = ahead_seq, use = ahead;
-    if (off == all) {
-      off = 0, ts += a.tpt;
-      if (ts >= hi) advance();
-    }
     if (r.nb == 0 && !(r.flags & (RUN_FIRST | RUN_LAST))) continue;  // (a run in a tile's midst always has blocks)
     if (first) item++;
     r.item = item;
     Blocks<C> bl;
-    bl.start(a, r, lane, use_seq, use);
+    bl.start(a, r, lane, ahead_seq, ahead);
     if (!(ok = k.wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1))) break;
     if (lane == 0) {
       k.runs()[n % PA_RING] = r;
@@ -448,7 +455,7 @@ __device__ __forceinline__ bool all_finite(const uint8_t *p, int step, int n) {
   __half2 sum[4];
 #pragma unroll
   for (int e = 0; e < 4; e++) sum[e] = __half2half2(__ushort_as_half(0));
-#pragma unroll 8
+#pragma unroll 4
   for (int i = 0; i < n; i++) {
     const uint4 x = *reinterpret_cast<const uint4 *>(p + i * step);
     const __half2 *h = reinterpret_cast<const __half2 *>(&x);

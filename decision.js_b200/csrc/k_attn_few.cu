@@ -114,10 +114,9 @@ __global__ void __launch_bounds__(F_THREADS, 2)
       const uint32_t p = tmem + (uint32_t)(C::S_COL + x % SB * KB);
       const uint64_t v = v0 + (uint32_t)(vs * C::KV_BYTES >> 4);
       if (elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < KB / 16; kk++)
-          if (kk < steps)
-            mma_f16_ts_rows(tmem + C::O_COL, p + (kk * 16 < COLS ? 8 * kk : COLS + 8 * kk - COLS / 2), v + kk * (2048 >> 4),
+#pragma unroll 1
+        for (int kk = 0; kk < steps; kk++)
+          mma_f16_ts_rows(tmem + C::O_COL, p + (kk * 16 < COLS ? 8 * kk : COLS + 8 * kk - COLS / 2), v + kk * (2048 >> 4),
                             idesc_pv, off);
         mma_commit(k.bar(C::B_VE + vs));
         mma_commit(k.bar(C::B_OR));
@@ -127,23 +126,35 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     };
     for (int n = 0; ok && k.next_run(n, r); n++) {
       if (r.flags & RUN_FIRST) ok = k.wait_warp(C::B_QF, r.item), begins = true;
-      for (int b = 0; ok && b < r.nb; b++, g++) {
-        const int ks = g % KST, key0 = (r.kb + b) * KB;
-        if (!(ok = k.wait_warp(C::B_KF + ks, g / KST))) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t sc = tmem + (uint32_t)(C::S_COL + g % SB * KB);
-          const uint64_t kd0 = k0 + (uint32_t)(ks * C::KV_BYTES >> 4);
+      // each turn a block's scores and the product before them; the tile's last run has one more for its last product
+      const bool last = (r.flags & RUN_LAST) != 0;
+      for (int b = 0; ok && b < r.nb + last; b++) {
+        const int key0 = (r.kb + b) * KB;
+        const bool more = b < r.nb;
+        if (more) {
+          const int ks = g % KST;
+          if (!(ok = k.wait_warp(C::B_KF + ks, g / KST))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t sc = tmem + (uint32_t)(C::S_COL + g % SB * KB);
+            const uint64_t kd0 = k0 + (uint32_t)(ks * C::KV_BYTES >> 4);
 #pragma unroll
-          for (int kd = 0; kd < D / 16; kd++)
-            mma_f16(sc, q0 + (((kd >> 2) * 128 * 128 + (kd & 3) * 32) >> 4),
-                    kd0 + (((kd >> 2) * KB * 128 + (kd & 3) * 32) >> 4), idesc_qk, kd > 0);
-          mma_commit(k.bar(C::B_SF + g % SB));
-          mma_commit(k.bar(C::B_KE + ks));
+            for (int kd = 0; kd < D / 16; kd++)
+              mma_f16(sc, q0 + (((kd >> 2) * 128 * 128 + (kd & 3) * 32) >> 4),
+                      kd0 + (((kd >> 2) * KB * 128 + (kd & 3) * 32) >> 4), idesc_qk, kd > 0);
+            mma_commit(k.bar(C::B_SF + g % SB));
+            mma_commit(k.bar(C::B_KE + ks));
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (last && b == max(r.nb - 1, 0)) {
+          if (elect_one()) mma_commit(k.bar(C::B_QE));
+          __syncwarp();
+        }
         if (pend && !(ok = pv(g - 1))) break;
-        pend = true, begins = false;
+        pend = more;
+        if (!more) break;
+        begins = false, g++;
         look = to_look_over<KB>(r, key0);
         steps = (min(KB, r.kend - key0) + 15) >> 4;
         // own blocks: the rows of the sequence that see a key of it
@@ -152,13 +163,9 @@ __global__ void __launch_bounds__(F_THREADS, 2)
 #pragma unroll
         for (int w = 0; w < 4; w++) off[w] = ~mask_word(lo, hi, w);
       }
-      if (ok && (r.flags & RUN_LAST)) {
-        if (elect_one()) mma_commit(k.bar(C::B_QE));
-        __syncwarp();
-        if (pend) ok = pv(g - 1);
-        pend = false;
+      if (ok && last) {
         // a tile without keys: the last tile's end has to be past before this one's is announced
-        if (ok && begins) ok = k.wait_warp(C::B_OE, r.item + 1);
+        if (begins) ok = k.wait_warp(C::B_OE, r.item + 1);
         if (ok && elect_one()) mma_commit(k.bar(C::B_OD));
         __syncwarp();
       }
@@ -281,18 +288,21 @@ __global__ void __launch_bounds__(F_THREADS, 2)
       if (!ok) break;
       had = had || nb > 0;
       if (r.flags & RUN_LAST) {
-        if (!(ok = k.wait_warp(C::B_OD, r.item))) break;
-        tc_fence_after();
         const bool tlast = (r.flags & RUN_TLAST) != 0, direct = tfirst && tlast;
         if (!direct && !a.by_row && tid == 0) {
           if (tlast) a.head[blockIdx.x] = make_int4(r.tok0, r.ntok, r.kvh, 0);
           if (tfirst) a.tail[blockIdx.x] = 1;
         }
-        if (anyv) {
+        float lt = 0.f;
+        if (anyv) {  // the sums meet while the last product runs
           const int par = meets & 1;
           xch[(par * 2 + hf) * 128 + row] = l;
           if (!(ok = meet())) break;
-          float lt = l + xch[(par * 2 + (hf ^ 1)) * 128 + row];
+          lt = l + xch[(par * 2 + (hf ^ 1)) * 128 + row];
+        }
+        if (!(ok = k.wait_warp(C::B_OD, r.item))) break;
+        tc_fence_after();
+        if (anyv) {
           if (had && valid && ((k.poison(r.item)[irow >> 5] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
           const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
           if (a.by_row && valid && jrow == 0 && hf == 0) {
@@ -311,14 +321,12 @@ __global__ void __launch_bounds__(F_THREADS, 2)
             tmem_ld_wait(o);
             if (!valid) continue;
             if (direct) {
-              uint32_t w[8];
 #pragma unroll
               for (int e = 0; e < 8; e++) {
                 const __half2 hv = __floats2half2_rn(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-                w[e] = *reinterpret_cast<const uint32_t *>(&hv);
+                o[e] = *reinterpret_cast<const uint32_t *>(&hv);
               }
-              *reinterpret_cast<uint4 *>(y + c) = make_uint4(w[0], w[1], w[2], w[3]);
-              *reinterpret_cast<uint4 *>(y + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+              store_row16(y + c, o, a.y32);
             } else if (lt != 0.f) {
               st_global_v8(po + c, o), st_global_v8(po + c + 8, o + 8);
             }

@@ -392,13 +392,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
               if (!valid) continue;
               if (direct) {
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                  __half2 hv[4];
-#pragma unroll
-                  for (int i = 0; i < 4; i++)
-                    hv[i] = __floats2half2_rn(__uint_as_float(o[e + 2 * i]) * inv, __uint_as_float(o[e + 2 * i + 1]) * inv);
-                  *reinterpret_cast<uint4 *>(y + c + e) = *reinterpret_cast<const uint4 *>(hv);
+                for (int e = 0; e < 16; e++) {
+                  const __half2 hv =
+                      __floats2half2_rn(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+                  o[e] = *reinterpret_cast<const uint32_t *>(&hv);
                 }
+                store_row16(y + c, o, a.y32), store_row16(y + c + 16, o + 8, a.y32);
               } else if (lt != 0.f) {
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) st_global_v8(po + c + e, o + e);
@@ -670,6 +669,7 @@ int attn_paged_launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs,
   // keys 29 us against 37 by tile, 64 over a shared prefix 40 against 48). Many: most rows were never cut, and blocks
   // for all of them would cost more than the tiles' search (32 groups of 3 questions 43 us by tile, 53 by row).
   a.by_row = few && (long)T * heads <= 8192;
+  a.y32 = (reinterpret_cast<uintptr_t>(Y) & 31) == 0 && ys % 16 == 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   if (c->D == 64) return launch<64>(ctx, c, Q, qs, a, few);
   if (c->D == 128) return launch<128>(ctx, c, Q, qs, a, few);
