@@ -24,7 +24,6 @@ struct Run {
   int tok0, ntok, kvh;     // the tile
   int flags, item;
   int seg;                 // sequence, or -1: the prefix
-  int s;                   // the sequence the run was found at
   int kb, nb, kend;        // first block, blocks, keys of the segment that the tile's last row in it sees
   int qb, qe, len;         // own runs: the sequence's rows and own keys
 };
@@ -329,15 +328,19 @@ __device__ __forceinline__ bool line_start(const Cta<C> &k, Groups &gs, Stretch 
   return true;
 }
 
-// The producer of K, which also walks the line, hands out the runs and loads Q: one warp.
+// The producers of K and of V, a warp each, in the same code (which the instruction caches then hold once). Both walk the
+// line; K's hands out the runs and loads Q.
 template <class C>
-__device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, const Stretch &st, const CUtensorMap *tmQ,
-                                          const CUtensorMap *tmK) {
-  constexpr int KB = C::KB, KST = C::KST, NA = C::NA;
+__device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, const Stretch &st, const bool values,
+                                          const CUtensorMap *tmQ, const CUtensorMap *map) {
+  constexpr int KB = C::KB, NA = C::NA;
+  const int stages = values ? C::VST : C::KST, filled = values ? C::B_VF : C::B_KF, empty = values ? C::B_VE : C::B_KE;
+  const uint32_t ring = k.base + (values ? C::V_OFF : C::K_OFF);
+  int stage = 0, turn = 1;
   const PArgs &a = k.a;
   const int lane = k.lane;
   const int *s_start = k.start();
-  int g = 0, item = -1, n = 0;  // blocks, tiles, runs
+  int item = -1, n = 0;  // tiles, runs
   bool ok = true, first = true;
   long pos = st.p0, off = (long)(uint32_t)s_start[1] | (long)s_start[2] << 32;  // on the line; in the sequence's pieces
   int s = s_start[0], kvh = st.kvh, gi = a.G ? gs.of(s) : 0;
@@ -377,7 +380,7 @@ __device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, con
     const int units = (int)min((prefix ? pc : all) - off, st.p1 - pos);
     const bool done = off + units == all && ends;
     Run r;
-    r.s = s, r.qb = qb, r.qe = qe, r.len = len;
+    r.qb = qb, r.qe = qe, r.len = len;
     r.tok0 = gr.tg + ts, r.ntok = min(rows - ts, a.tpt), r.kvh = kvh;
     r.tab = prefix ? a.ptable + (long)gi * a.pstride : a.table + (long)s * a.tstride;
     r.seg = prefix ? -1 : s, r.kend = prefix ? gs.plens[gi] : lim;
@@ -390,63 +393,43 @@ __device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, con
     r.item = item;
     Blocks<C> bl;
     bl.start(a, r, lane, ahead_seq, ahead);
-    if (!(ok = k.wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1))) break;
-    if (lane == 0) {
-      k.runs()[n % PA_RING] = r;
-      mbar_arrive(k.bar(C::B_IF + n % PA_RING));
-    }
-    n++;
-    __syncwarp();
-    if (first) {
-      if (!(ok = k.wait_warp(C::B_QE, item + 1))) break;
-      if (elect_one()) {
-        mbar_expect_tx(k.bar(C::B_QF), (uint32_t)(a.r * a.tpt * 128 * NA));
-        for (int j = 0; j < NA; j++)
-          tma_load_3d(k.base + j * C::Q_ROWS * 128, tmQ, 64 * j, r.kvh * a.r, r.tok0, k.bar(C::B_QF));
+    if (!values) {
+      if (!(ok = k.wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1))) break;
+      if (lane == 0) {
+        k.runs()[n % PA_RING] = r;
+        mbar_arrive(k.bar(C::B_IF + n % PA_RING));
       }
+      n++;
       __syncwarp();
     }
     bl.settle(a, lane);
-    for (int b = 0; b < r.nb; b++, g++) {
-      const int stage = g % KST;
+    // Q comes after as many blocks as the ring takes without it: its buffer is free only when the tile before is done
+    const int q_at = !first || values ? -1 : item == 0 ? 0 : min(r.nb, C::KST);
+#pragma unroll 1
+    for (int b = 0;; b++) {
+      if (b == q_at) {
+        if (!(ok = k.wait_warp(C::B_QE, item + 1))) break;
+        if (elect_one()) {
+          mbar_expect_tx(k.bar(C::B_QF), (uint32_t)(a.r * a.tpt * 128 * NA));
+#pragma unroll 1
+          for (int j = 0; j < NA; j++)
+            tma_load_3d(k.base + j * C::Q_ROWS * 128, tmQ, 64 * j, r.kvh * a.r, r.tok0, k.bar(C::B_QF));
+        }
+        __syncwarp();
+      }
+      if (b == r.nb) break;
       const typename Blocks<C>::Rows x = bl.rows(a, r.kb + b, lane);
-      if (!(ok = k.wait_warp(C::B_KE + stage, g / KST + 1))) break;
-      if (elect_one()) bl.load(tmK, x, k.base + C::K_OFF + stage * C::KV_BYTES, k.bar(C::B_KF + stage));
+      if (!(ok = k.wait_warp(empty + stage, turn))) break;
+      if (elect_one()) bl.load(map, x, ring + stage * C::KV_BYTES, k.bar(filled + stage));
       __syncwarp();
+      if (++stage == stages) stage = 0, turn ^= 1;
     }
     if (!ok) break;
     first = (r.flags & RUN_LAST) != 0;
   }
-  if (ok && k.wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1) && lane == 0) {
+  if (!values && ok && k.wait_warp(C::B_IE + n % PA_RING, n / PA_RING + 1) && lane == 0) {
     k.runs()[n % PA_RING].flags = RUN_END;
     mbar_arrive(k.bar(C::B_IF + n % PA_RING));
-  }
-}
-
-// The producer of V: one warp.
-template <class C>
-__device__ __forceinline__ void load_values(const Cta<C> &k, const CUtensorMap *tmV) {
-  constexpr int VST = C::VST;
-  const PArgs &a = k.a;
-  const int lane = k.lane;
-  Run r;
-  int g = 0, ahead_seq = -1, ahead = 0;
-  bool ok = true;
-  for (int n = 0; ok && k.next_run(n, r); n++) {
-    if (r.nb > 0) {
-      Blocks<C> bl;
-      bl.start(a, r, lane, ahead_seq, ahead);
-      bl.settle(a, lane);
-      ahead_seq = r.seg < 0 ? r.s : r.s + 1, ahead = read_ahead(a, ahead_seq, lane);  // what usually comes next
-      for (int b = 0; b < r.nb; b++, g++) {
-        const int st = g % VST;
-        const typename Blocks<C>::Rows x = bl.rows(a, r.kb + b, lane);
-        if (!(ok = k.wait_warp(C::B_VE + st, g / VST + 1))) break;
-        if (elect_one()) bl.load(tmV, x, k.base + C::V_OFF + st * C::KV_BYTES, k.bar(C::B_VF + st));
-        __syncwarp();
-      }
-    }
-    if (ok) k.done_run(n);
   }
 }
 

@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
       const int n = i == C::B_OE || (i >= C::B_PF && i < C::B_PF + SB) ? FS
                     : i >= C::B_XB && i < C::B_XB + 4                  ? 2
                     : i >= C::B_VE && i < C::B_VE + VST                ? 2
-                    : i >= C::B_IE                                     ? FS + 3
+                    : i >= C::B_IE                                     ? FS + 2
                                                                        : 1;
       mbar_init(k.bar(i), n);
     }
@@ -84,10 +84,8 @@ __global__ void __launch_bounds__(F_THREADS, 2)
   const uint32_t tmem = *k.tmem_slot();
 
   if (!fine || st.p0 >= st.p1) {
-  } else if (warp == FW_K) {
-    walk_line(k, gs, st, &tmQ, &tmK);
-  } else if (warp == FW_V) {
-    load_values(k, &tmV);
+  } else if (warp == FW_K || warp == FW_V) {
+    walk_line(k, gs, st, warp == FW_V, &tmQ, warp == FW_V ? &tmV : &tmK);
   } else if (warp == FW_C) {
     look_over(k);
   } else if (warp == FW_M) {

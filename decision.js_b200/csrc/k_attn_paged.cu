@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       const int n = i == C::B_OE || (i >= C::B_PF && i < C::B_PF + PA_WG) ? 4
                     : i >= C::B_XB && i < C::B_XB + 16                     ? PA_WG - 1
                     : i >= C::B_VE && i < C::B_VE + VST                    ? 2
-                    : i >= C::B_IE                                         ? PA_SOFT + 4
+                    : i >= C::B_IE                                         ? PA_SOFT + 3
                                                                            : 1;
       mbar_init(bar(i), n);
     }
@@ -126,10 +126,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   auto wait_warp = [&](int i, int parity) { return k.wait_warp(i, parity); };
   auto wait1 = [&](int i, int parity) { return k.wait1(i, parity); };
   if (!fine || st.p0 >= st.p1) {
-  } else if (warp == PA_WK) {
-    walk_line(k, gs, st, &tmQ, &tmK);
-  } else if (warp == PA_WV) {
-    load_values(k, &tmV);
+  } else if (warp == PA_WK || warp == PA_WV) {
+    walk_line(k, gs, st, warp == PA_WV, &tmQ, warp == PA_WV ? &tmV : &tmK);
   } else if (warp == PA_WC) {
     look_over(k);
   } else if (warp == PA_WM) {
