@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
           if (elect_one()) {
             const uint32_t sc = tmem + (uint32_t)(C::S_COL + g % SB * KB);
             const uint64_t kd0 = k0 + (uint32_t)(ks * C::KV_BYTES >> 4);
-#pragma unroll
+#pragma unroll 1
             for (int kd = 0; kd < D / 16; kd++)
               mma_f16(sc, q0 + (((kd >> 2) * 128 * 128 + (kd & 3) * 32) >> 4),
                       kd0 + (((kd >> 2) * KB * 128 + (kd & 3) * 32) >> 4), idesc_qk, kd > 0);
