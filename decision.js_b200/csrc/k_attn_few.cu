@@ -4,13 +4,17 @@
 // (scores, maximum, weights, product), so two CTAs share an SM and within each two warps share a row:
 //   warps 0-7  softmax: two warps per TMEM lane quadrant, thread = row, each half of a block's keys; the halves' maxima
 //              meet in shared memory. Quadrants without rows only keep step.
-//   warp 8     walks the line, loads Q and K; warp 9 loads V; warp 10 Q K^T and P V (and TMEM); warp 11 looks values over
+//   warp 8     walks the line, loads K and Q; warp 9 walks it and loads V; warp 10 Q K^T and P V (and TMEM); warp 11 looks
+//              values over
 // Blocks are 64 keys with two scores' buffers, which leaves each warp 32 scores: they stay in registers from the maximum
 // to the weights. The weights are scaled by 2^7 as in the wide kernel.
-// Bound by the chain of a block, not by the cache's bytes: 64 sequences of one token over a shared prefix of 32,768 tokens
-// (24 heads over 8, D = 128) take 40 us where the bytes need 18.6. Kept steps: two CTAs an SM with halves of rows 45 -> 40
-// us, the join by row, unneeded waits on the look-over removed. Measured and not taken: blocks of 128 keys in one scores'
-// buffer at D = 64, one pass with the weights kept in registers, products by warps' own matrix instructions.
+// Bound by the chain of a block (at D = 64; about 1 us for 64 keys, two CTAs at a time) and by L2 (at D = 128 with two
+// tiles to a prefix): 64 sequences of one token over a shared prefix of 32,768 tokens (16 heads over 8, D = 128) take 36 us
+// where the bytes need 18.6; 4 us of that are the line, 3 the join. 32 groups of 3 questions of 40 tokens over 512 tokens
+// take 61 us, of which the way from one tile to the next is the most. Kept steps: two CTAs an SM with halves of rows 45 ->
+// 40 us on the former; one code for both producers, Q after the keys, Q K^T from a loop 73 -> 61 on the latter (see the
+// instruction caches in the wide kernel). Measured and not taken: blocks of 128 keys in one scores' buffer at D = 64, one
+// pass with the weights kept in registers, products by warps' own matrix instructions, waits that poll.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

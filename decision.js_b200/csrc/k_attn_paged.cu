@@ -25,18 +25,20 @@
 //   warp 12    looks over V blocks that some row of the tile does not see: rows past the last key are zeroed, and
 //              values that are not finite too (a weight of 0 times them would be NaN in every row), with a mark on
 //              the rows that see them
-//   warp 13    loads V
+//   warp 13    walks the line and loads V
 //   warp 14    Q K^T (and TMEM), warp 15 P V: two threads, as one would be busy issuing for longer than the products take
-//   warp 16    walks the line, hands runs of blocks to the others through a ring of descriptors, loads Q and K
+//   warp 16    walks the line, hands runs of blocks to the others through a ring of descriptors, loads K and Q
 // All roles run ahead across tiles; Q (single buffer) and the accumulator wait for a tile's end, which the warpgroup of the
 // tile's last block sees to while the other two go on.
 //
 // What bounds it. Many rows over a long prefix (60 sequences of up to 50 tokens, 16,000 keys, 24 heads over 8, D = 128):
-// 218 us, 818 TFLOP/s, half the measured matrix rate; without the softmax it still takes 167, as every tile of 128 rows
-// brings all its keys from L2 (about 39 bytes a clock and SM): only tiles of 256 rows would change that, and tensor memory
-// has no room for their scores next to two accumulators. Short tiles (a few blocks each): the chain from a tile's last
-// product over its stores to the next tile's first product. Steps measured: two softmax warpgroups in turn 264 -> 245
-// us, three with 128-key blocks 232, the tile's end by one warpgroup instead of all three 2% (8% at D = 64).
+// 208 to 220 us with the power clock, about 850 TFLOP/s, half the measured matrix rate; without the softmax it still takes
+// 167, as every tile of 128 rows brings all its keys from L2 (about 39 bytes a clock and SM): only tiles of 256 rows would
+// change that, and tensor memory has no room for their scores next to two accumulators. Short tiles (a few blocks each):
+// the chain from a tile's last product over its stores to the next tile's first product, and the instruction caches, which
+// the roles' code (70 KB) does not fit: a look-up in four missed, and every loop that was rolled and every path that two
+// roles share has shortened such calls. Steps measured: two softmax warpgroups in turn 264 -> 245 us, three with 128-key
+// blocks 232, the tile's end by one warpgroup instead of all three 2% (8% at D = 64).
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -589,10 +591,11 @@ Ws ws_layout(int T, int heads, int kv, int D, int ctas) {
 }
 
 // The kernel for few rows where a group has four tiles or less. Measured, few against many rows' kernel, us: decode of 64
-// sequences over a prefix of 32,768 tokens 40 against 44, over 24 prefixes 100 against 119; 32 groups of 3 questions of 40
-// tokens over 512 tokens 75 against 80; 512 rows over 16,000 keys 42 against 45 (D = 64: 38 against 37); 2,048 rows over
-// 16,000 keys 74 against 66, 8,192 rows 237 against 217. (8,192 rows over 4,000 keys would still gain, 84 against 92; how
-// long a prefix is the host does not know.) At D = 256 the accumulators of two CTAs do not fit.
+// sequences over a prefix of 32,768 tokens 36 against 40, over 24 prefixes of 6,000 100 against 97, of one sequence over
+// 30,000 keys 26 against 27 (D = 64: 23 against 27); 32 groups of 3 questions of 40 tokens over 512 tokens 61 against 64;
+// about 300 rows over 16,000 keys 39 against 43 (D = 64: 36 against 37). 1,100 rows over 16,000 keys 75 against 64, 4,500
+// rows 276 against 208. (64 groups of 40 rows gain at 500 keys, 46 against 55, and lose at 4,000, 171 against 158; how long
+// a prefix is the host does not know.) At D = 256 the accumulators of two CTAs do not fit.
 bool paged_few(int D, int T, int r, int G) { return D <= 128 && (long)T * r <= 512L * std::max(G, 1); }
 
 template <int D>
