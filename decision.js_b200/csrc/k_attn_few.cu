@@ -40,14 +40,14 @@ struct FewCfg {
   static constexpr int Q_BYTES = Q_ROWS * D * 2, KV_BYTES = KB * D * 2;
   static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + KST * KV_BYTES;
   static constexpr int BAR_OFF = V_OFF + VST * KV_BYTES;
-  static constexpr int B_QF = 0, B_QE = 1, B_OD = 2, B_OE = 3, B_OR = 4, B_XB = 5, B_SF = 9, B_PF = B_SF + SB,
+  static constexpr int B_QF = 0, B_QE = 1, B_OD = 2, B_OE = 3, B_OR = 4, B_SF = 5, B_PF = B_SF + SB,
                        B_KF = B_PF + SB, B_KE = B_KF + KST, B_VF = B_KE + KST, B_VE = B_VF + VST, B_VS = B_VE + VST,
                        B_IF = B_VS + VST, B_IE = B_IF + PA_RING, NBARS = B_IE + PA_RING;
   static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15);
   static constexpr int POISON_OFF = MISC_OFF + 32, SCAN_OFF = POISON_OFF + 64,
                        RUN_OFF = SCAN_OFF + ((F_THREADS / 32 * 8 + 15) & ~15), GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run),
-                       XCH_OFF = GOFF_OFF + PA_META;  // floats [2 turns][2 halves][128 rows]
-  static constexpr int SMEM = XCH_OFF + 2 * 2 * 128 * 4 + 1024;
+                       XCH_OFF = GOFF_OFF + PA_META;  // (value, turn) [2 turns][2 halves][128 rows]
+  static constexpr int SMEM = XCH_OFF + 2 * 2 * 128 * 8 + 1024;
   static constexpr int S_COL = 0, O_COL = SB * KB, TCOLS = 256;
   static_assert(O_COL + D <= TCOLS, "tensor memory");
   static_assert(2 * SMEM <= 227 * 1024, "shared memory");
@@ -65,7 +65,6 @@ __global__ void __launch_bounds__(F_THREADS, 2)
   if (tid == 0) {
     for (int i = 0; i < C::NBARS; i++) {
       const int n = i == C::B_OE || (i >= C::B_PF && i < C::B_PF + SB) ? FS
-                    : i >= C::B_XB && i < C::B_XB + 4                  ? 2
                     : i >= C::B_VE && i < C::B_VE + VST                ? 2
                     : i >= C::B_IE                                     ? FS + 2
                                                                        : 1;
@@ -74,6 +73,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     *k.abort() = 0;
     mbar_init_fence();
   }
+  for (int i = tid; i < 512; i += F_THREADS) reinterpret_cast<int2 *>(k.smem + C::XCH_OFF)[i] = make_int2(0, 0);
   if (warp == FW_K && lane == 0) tma_prefetch_desc(&tmQ), tma_prefetch_desc(&tmK);
   if (warp == FW_V && lane == 0) tma_prefetch_desc(&tmV);
   // (tensor memory after the kernels before, and before the next is let in: see the wide kernel)
@@ -177,17 +177,32 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     const int q = warp & 3, hf = warp >> 2;
     const int row = 32 * q + lane, irow = row / a.r, jrow = row - irow * a.r;
     const uint32_t lrow = tmem + ((uint32_t)(32 * q) << 16), ocol = lrow + (uint32_t)(C::O_COL + hf * (D / 2));
-    float *xch = reinterpret_cast<float *>(k.smem + C::XCH_OFF);
+    const uint32_t xch = k.base + C::XCH_OFF + 8 * row;
     int g = 0, meets = 0;
     bool ok = true;
     // the tile's state
     bool valid = false, anyv = false, had = false, tfirst = false;
     int t = 0;
     float ref = -FLT_MAX, l = 0.f;
-    auto meet = [&]() -> bool {  // both warps of the quadrant have written their halves
-      __syncwarp();
-      if (lane == 0) mbar_arrive(k.bar(C::B_XB + q));
-      return k.wait_warp(C::B_XB + q, meets++);
+    // Gives this half's value of the row and takes the other's: both write theirs with the number of the turn, in one
+    // store, and look for the other's (a half writes to a place again only when the other has read it: it has then seen
+    // the other's value of the turn between).
+    auto meet = [&](float mine, float &theirs) -> bool {
+      const uint32_t at = xch + (meets & 1) * 2048, mark = ++meets;
+      asm volatile("st.volatile.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + 1024 * hf), "f"(mine), "r"(mark) : "memory");
+      uint64_t t0 = 0;
+#pragma unroll 1
+      for (uint32_t i = 1;; i++) {
+        uint32_t seen;
+        asm volatile("ld.volatile.shared.v2.b32 {%0, %1}, [%2];" : "=f"(theirs), "=r"(seen) : "r"(at + 1024 * (hf ^ 1)) : "memory");
+        if (__all_sync(0xffffffffu, seen == mark)) return true;
+        if ((i & 1023) == 0) {
+          const uint64_t now = globaltimer();
+          t0 = t0 ? t0 : now;
+          if (now - t0 > 2000000000ull) *k.abort() = 1, atomicOr(a.err, (uint32_t)DC_DEVERR_ATTN_WAIT);
+          if (__any_sync(0xffffffffu, *k.abort() != 0)) return false;
+        }
+      }
     };
     for (int n = 0; ok && k.wait_warp(C::B_IF + n % PA_RING, n / PA_RING); n++) {
       const Run &r = k.runs()[n % PA_RING];  // (stays as it is until done_run)
@@ -240,10 +255,9 @@ __global__ void __launch_bounds__(F_THREADS, 2)
             m2[1] = max3(m2[1], __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
           }
           const float pmx = fmaxf(m2[0], m2[1]) * sc;
-          const int par = meets & 1;
-          xch[(par * 2 + hf) * 128 + row] = pmx;
-          if (!(ok = meet())) break;
-          const float mx = fmaxf(pmx, xch[(par * 2 + (hf ^ 1)) * 128 + row]);
+          float omx;
+          if (!(ok = meet(pmx, omx))) break;
+          const float mx = fmaxf(pmx, omx);
           const bool grow = mx > ref + 8.0f;
           const bool resc = grow && ref > -FLT_MAX;
           if (__any_sync(0xffffffffu, resc)) {
@@ -297,10 +311,9 @@ __global__ void __launch_bounds__(F_THREADS, 2)
         }
         float lt = 0.f;
         if (anyv) {  // the sums meet while the last product runs
-          const int par = meets & 1;
-          xch[(par * 2 + hf) * 128 + row] = l;
-          if (!(ok = meet())) break;
-          lt = l + xch[(par * 2 + (hf ^ 1)) * 128 + row];
+          float ol;
+          if (!(ok = meet(l, ol))) break;
+          lt = l + ol;
         }
         if (!(ok = k.wait_warp(C::B_OD, r.item))) break;
         tc_fence_after();
