@@ -420,42 +420,27 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   }
 }
 
+template <int D>
+struct JoinRows {  // rows of a warp in the join by tile
+  static constexpr int R = D == 256 ? 2 : 4;
+};
+
 // Joins the parts of the tiles that were cut: y = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over the CTAs c from the
-// tile's first to its last. W = 4, for few rows in many parts: a block to a (row, head), each warp every fourth part,
-// joined in order of the warps. W = 1, for many rows, most of them whole or cut once: blockIdx.y is the CTA that ends a
-// cut tile, a block takes four rows of it.
-template <int D, int W>
+// tile's first to its last. For few rows in many parts: a block to a (row, head), each of its W warps every W-th part,
+// joined in order of the warps.
+template <int D>
 __global__ void __launch_bounds__(128) attention_join_kernel(const PArgs a) {
   dc_pdl_begin();
-  constexpr int N = D / 32;  // a lane's values
-  __shared__ float s_o[W][W > 1 ? D : 1], s_m[W], s_l[W];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = W > 1 ? warp : 0;
-  const int refused = a.hdr[0];  // (a refused call, or one whose waits ran out, has no records)
-  int c0 = -1, c1;
-  long t, base;  // part c of the row: row base + 128 c
-  int h;
-  if (W > 1) {
-    t = blockIdx.x / a.heads, h = blockIdx.x - (int)t * a.heads;
-    const int kvh = h / a.r;
-    const int t0 = a.qoff[0], t1 = a.qoff[a.S];
-    c0 = a.first[(long)kvh * a.T + t], c1 = a.last[(long)kvh * a.T + t];
-    if (refused || t < t0 || t >= t1 || c0 < 0 || c1 < c0 || c1 >= a.ctas) return;
-    base = ((long)kvh * a.T + t) * a.r + h - kvh * a.r;
-  } else {
-    const int row = blockIdx.x * 4 + warp;
-    c1 = blockIdx.y;
-    const int4 tile = a.head[c1];
-    if (refused || row >= tile.y * a.r) return;
-    for (int e = c1; e > 0 && c0 < 0; e -= 32) {  // the last CTA before that begins a tile and does not end it
-      const int c = e - 1 - lane;
-      const uint32_t at = __ballot_sync(0xffffffffu, c >= 0 && a.tail[c] != 0);
-      if (at) c0 = e - __ffs(at);
-    }
-    if (c0 < 0) return;
-    const int i = row / a.r;
-    t = tile.x + i, h = tile.z * a.r + row - i * a.r;
-    base = ((long)tile.z * a.T + tile.x) * a.r + row;
-  }
+  constexpr int N = D / 32, W = 4;  // a lane's values; warps
+  __shared__ float s_o[W][D], s_m[W], s_l[W];
+  const int part = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long t = blockIdx.x / a.heads;
+  const int h = blockIdx.x - (int)t * a.heads, kvh = h / a.r;
+  const int t0 = a.qoff[0], t1 = a.qoff[a.S];
+  const int c0 = a.first[(long)kvh * a.T + t], c1 = a.last[(long)kvh * a.T + t];
+  // (a refused call, or one whose waits ran out, has no records)
+  if (a.hdr[0] || t < t0 || t >= t1 || c0 < 0 || c1 < c0 || c1 >= a.ctas) return;
+  const long base = ((long)kvh * a.T + t) * a.r + h - kvh * a.r;  // part c of the row: row base + 128 c
   auto fetch = [&](float (&v)[N], int c) {
     const float *p = a.O + (base + 128L * c) * D + N * lane;
     if (N == 2) {
@@ -517,33 +502,115 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PArgs a) {
   }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) L += __shfl_xor_sync(0xffffffffu, L, s);
-  if (W > 1) {
-    if (lane == 0) s_m[warp] = M, s_l[warp] = L;
-    __syncthreads();
-    float all = -FLT_MAX;
+  if (lane == 0) s_m[part] = M, s_l[part] = L;
+  __syncthreads();
+  float all = -FLT_MAX;
 #pragma unroll
-    for (int w = 0; w < W; w++) all = s_l[w] != 0.f ? fmaxf(all, s_m[w]) : all;
-    const float f = s_l[warp] != 0.f ? ex2_approx(M - all) : 0.f;
+  for (int w = 0; w < W; w++) all = s_l[w] != 0.f ? fmaxf(all, s_m[w]) : all;
+  const float f = s_l[part] != 0.f ? ex2_approx(M - all) : 0.f;
 #pragma unroll
-    for (int e = 0; e < N; e++) s_o[warp][N * lane + e] = s_l[warp] != 0.f ? o[e] * f : 0.f;
-    L = 0.f;
+  for (int e = 0; e < N; e++) s_o[part][N * lane + e] = s_l[part] != 0.f ? o[e] * f : 0.f;
+  L = 0.f;
 #pragma unroll
-    for (int w = 0; w < W; w++)
-      if (s_l[w] != 0.f) L += s_l[w] * ex2_approx(s_m[w] - all);
-    __syncthreads();
-    if (warp) return;
+  for (int w = 0; w < W; w++)
+    if (s_l[w] != 0.f) L += s_l[w] * ex2_approx(s_m[w] - all);
+  __syncthreads();
+  if (part) return;
 #pragma unroll
-    for (int e = 0; e < N; e++) {
-      o[e] = 0.f;
+  for (int e = 0; e < N; e++) {
+    o[e] = 0.f;
 #pragma unroll
-      for (int w = 0; w < W; w++) o[e] += s_o[w][N * lane + e];
-    }
+    for (int w = 0; w < W; w++) o[e] += s_o[w][N * lane + e];
   }
   const float inv = L == 0.f ? 0.f : 1.0f / L;
   __half *y = a.Y + t * a.ystride + (long)h * D + N * lane;
 #pragma unroll
   for (int e = 0; e < N; e += 2)
     *reinterpret_cast<__half2 *>(y + e) = __floats2half2_rn(o[e] * inv, o[e + 1] * inv);
+}
+
+// The same for many rows, most of them whole or cut once: blockIdx.y is the CTA that ends a cut tile. A warp takes R rows
+// of it, two parts of each at a time, all on their way together, as what a row costs is the way to memory and back. 64
+// groups of 2 x 20 tokens over 500, D = 64: 40.2 us with a row to a warp, 35.2 with four rows and four parts at a time,
+// 34.0 with two parts (fewer registers, more warps), 35.4 with two rows.
+template <int D>
+__global__ void __launch_bounds__(128) attention_join_tiles_kernel(const PArgs a) {
+  dc_pdl_begin();
+  constexpr int N = D / 32, R = JoinRows<D>::R, P = 2;  // a lane's values; rows; parts
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c1 = blockIdx.y, row0 = (blockIdx.x * 4 + warp) * R;
+  const int refused = a.hdr[0];
+  const int4 tile = a.head[c1];
+  bool begins = c1 > lane && a.tail[c1 - 1 - lane] != 0;
+  const int rows = min(R, tile.y * a.r - row0);
+  if (refused || rows <= 0) return;
+  int c0 = c1;  // the last CTA before that begins a tile and does not end it
+  for (uint32_t at; (at = __ballot_sync(0xffffffffu, begins)) == 0;) {
+    c0 -= 32;
+    if (c0 <= 0) return;
+    begins = c0 > lane && a.tail[c0 - 1 - lane] != 0;
+  }
+  c0 -= __ffs(__ballot_sync(0xffffffffu, begins));
+  const long base = ((long)tile.z * a.T + tile.x) * a.r + row0;  // part c of a row: 128 c rows on
+  float M[R], L[R], o[R][N];
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    M[i] = -FLT_MAX, L[i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; e++) o[i][e] = 0.f;
+  }
+#pragma unroll 1
+  for (int cb = c0; cb <= c1; cb += P) {
+    float2 x[R][P];
+    float v[R][P][N];  // (where a part's weight is 0, nothing was stored and nothing is used)
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+      for (int k = 0; k < P; k++) {
+        x[i][k] = make_float2(-FLT_MAX, 0.f);
+#pragma unroll
+        for (int e = 0; e < N; e++) v[i][k][e] = 0.f;
+        if (i >= rows || cb + k > c1) continue;
+        const long at = base + i + 128L * (cb + k);
+        x[i][k] = a.ml[at];
+        const float *p = a.O + at * D + N * lane;
+        if (N == 2) {
+          *reinterpret_cast<float2 *>(v[i][k]) = *reinterpret_cast<const float2 *>(p);
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; e += 4)
+            *reinterpret_cast<float4 *>(v[i][k] + e) = *reinterpret_cast<const float4 *>(p + e);
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      float m = M[i];
+#pragma unroll
+      for (int k = 0; k < P; k++) m = x[i][k].y != 0.f ? fmaxf(m, x[i][k].x) : m;
+      const float f = ex2_approx(M[i] - m);  // what is there goes to the new maximum
+      M[i] = m, L[i] *= f;
+#pragma unroll
+      for (int e = 0; e < N; e++) o[i][e] *= f;
+#pragma unroll
+      for (int k = 0; k < P; k++)
+        if (x[i][k].y != 0.f) {
+          const float w = ex2_approx(x[i][k].x - m);
+          L[i] = fmaf(w, x[i][k].y, L[i]);
+#pragma unroll
+          for (int e = 0; e < N; e++) o[i][e] = fmaf(w, v[i][k][e], o[i][e]);
+        }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    if (i >= rows) break;
+    const int tok = (row0 + i) / a.r, h = tile.z * a.r + row0 + i - tok * a.r;
+    const float inv = L[i] == 0.f ? 0.f : 1.0f / L[i];
+    __half *y = a.Y + (long)(tile.x + tok) * a.ystride + (long)h * D + N * lane;
+#pragma unroll
+    for (int e = 0; e < N; e += 2)
+      *reinterpret_cast<__half2 *>(y + e) = __floats2half2_rn(o[i][e] * inv, o[i][e + 1] * inv);
+  }
 }
 
 typedef CUresult (*EncodeTiledP)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
@@ -623,11 +690,12 @@ int launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, PArgs a, b
   if constexpr (D <= 128)
     if (a.by_row) {
       const dim3 grid((unsigned)((long)a.T * a.heads));
-      DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D, 4>, grid, dim3(128), 0, a));
+      DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D>, grid, dim3(128), 0, a));
       return dc_launch_check("attention_paged (join)");
     }
-  const dim3 grid((unsigned)((std::min((long)a.T * a.r, 128L) + 3) / 4), a.ctas);
-  DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D, 1>, grid, dim3(128), 0, a));
+  constexpr int R = 4 * JoinRows<D>::R;  // of a block
+  const dim3 grid((unsigned)((std::min((long)a.T * a.r, 128L) + R - 1) / R), a.ctas);
+  DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_tiles_kernel<D>, grid, dim3(128), 0, a));
   return dc_launch_check("attention_paged (join)");
 }
 
@@ -666,10 +734,12 @@ int attn_paged_launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs,
   a.pshift = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7, a.rows = c->pages * c->kv * c->page;
   a.chunk_min = 2;  // no stretch is shorter, so that short calls have few parts (1 and 4 measured the same)
   a.ctas = ctas;
-  // Few rows: most tiles are cut, into many parts, and a join by row takes them up in four warps (one sequence over 30,000
-  // keys 29 us against 37 by tile, 64 over a shared prefix 40 against 48). Many: most rows were never cut, and blocks
-  // for all of them would cost more than the tiles' search (32 groups of 3 questions 43 us by tile, 53 by row).
-  a.by_row = few && (long)T * heads <= 8192;
+  // Few tiles are cut into many parts each, and a join by row takes them up in four warps (one sequence over 30,000 keys 26
+  // us against 48 by tile, 35 over a shared prefix 36 against 67, 8 groups of 4 x 16 tokens 20 against 23). Many tiles are
+  // whole or in two or three parts, and blocks for rows that were not cut would cost more than the tiles' search (24 groups
+  // of 12 tokens 95 us by row, 91 by tile; 16 groups of 8 x 8 tokens 34 and 31; 32 of 3 questions 54 and 41).
+  const long groups = std::max(G, 1), tiles = c->kv * groups * (((long)T * a.r + 128 * groups - 1) / (128 * groups));
+  a.by_row = few && 3 * tiles <= ctas;
   a.y32 = (reinterpret_cast<uintptr_t>(Y) & 31) == 0 && ys % 16 == 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   if (c->D == 64) return launch<64>(ctx, c, Q, qs, a, few);
