@@ -8,14 +8,16 @@
 //              values over
 // Blocks are 64 keys with two scores' buffers, which leaves each warp 32 scores: they stay in registers from the maximum
 // to the weights. The weights are scaled by 2^7 as in the wide kernel.
-// Bound by the chain of a block (at D = 64; about 1 us for 64 keys, two CTAs at a time) and by L2 (at D = 128 with two
-// tiles to a prefix): 64 sequences of one token over a shared prefix of 32,768 tokens (16 heads over 8, D = 128) take 36 us
-// where the bytes need 18.6; 4 us of that are the line, 3 the join. 32 groups of 3 questions of 40 tokens over 512 tokens
-// take 61 us, of which the way from one tile to the next is the most. Kept steps: two CTAs an SM with halves of rows 45 ->
-// 40 us on the former; one code for both producers, Q after the keys, Q K^T from a loop 73 -> 61 on the latter (see the
-// instruction caches in the wide kernel). Measured and not taken: blocks of 128 keys in one scores' buffer at D = 64, one
-// pass with the weights kept in registers, products by warps' own matrix instructions, waits that poll (but for the
-// halves' exchange of maxima: D = 64, 24 groups, 99.7 -> 95.1 us), rows of an SM's second CTA on the other two quadrants.
+// Bound by the chain of a block at D = 64 (0.9 us for 64 keys, two CTAs at a time: 218 sequences of one token over 24
+// prefixes of up to 6,000 tokens, 32 heads over 8, 90 us where the bytes need 44.5), by memory while it streams at D = 128
+// (35 sequences of one token over a shared prefix of 18,000 tokens, 16 heads over 8: 36 us where the bytes need 18.6; 22 us
+// of streaming, 4 for the line, 4 until the first keys are there, 5 for the last CTAs and the join). 32 groups of 3
+// questions of 40 tokens over 512 tokens take 58 us, of which the way from one tile to the next is the most. Kept steps: two
+// CTAs an SM with halves of rows 45 -> 40 us on the second; one code for both producers, Q after the keys, Q K^T from a loop
+// 73 -> 61 on the third (see the instruction caches in the wide kernel). Measured and not taken: blocks of 128 keys in one
+// scores' buffer at D = 64, one pass with the weights kept in registers, products by warps' own matrix instructions, waits
+// that poll (but for the halves' exchange of maxima: 24 prefixes, D = 64, 99.7 -> 95.1 us), rows of an SM's second CTA on
+// the other two quadrants.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -195,7 +197,10 @@ __global__ void __launch_bounds__(F_THREADS, 2)
 #pragma unroll 1
       for (uint32_t i = 1;; i++) {
         uint32_t seen;
-        asm volatile("ld.volatile.shared.v2.b32 {%0, %1}, [%2];" : "=f"(theirs), "=r"(seen) : "r"(at + 1024 * (hf ^ 1)) : "memory");
+        asm volatile("ld.volatile.shared.v2.b32 {%0, %1}, [%2];"
+                     : "=f"(theirs), "=r"(seen)
+                     : "r"(at + 1024 * (hf ^ 1))
+                     : "memory");
         if (__all_sync(0xffffffffu, seen == mark)) return true;
         if ((i & 1023) == 0) {
           const uint64_t now = globaltimer();

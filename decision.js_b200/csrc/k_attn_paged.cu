@@ -31,7 +31,7 @@
 // All roles run ahead across tiles; Q (single buffer) and the accumulator wait for a tile's end, which the warpgroup of the
 // tile's last block sees to while the other two go on.
 //
-// What bounds it. Many rows over a long prefix (60 sequences of up to 50 tokens, 16,000 keys, 24 heads over 8, D = 128):
+// What bounds it. Many rows over a long prefix (49 sequences of up to 50 tokens, 12,800 keys, 24 heads over 8, D = 128):
 // 208 to 220 us with the power clock, about 850 TFLOP/s, half the measured matrix rate; without the softmax it still takes
 // 167, as every tile of 128 rows brings all its keys from L2 (about 39 bytes a clock and SM): only tiles of 256 rows would
 // change that, and tensor memory has no room for their scores next to two accumulators. Short tiles (a few blocks each):
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           if (!(ok = wait_warp(C::B_XB + 4 * q + four, turn4) && wait_warp(C::B_OD + four, turn4))) break;
           tc_fence_after();
           const bool tlast = (r.flags & RUN_TLAST) != 0, direct = tfirst && tlast;
-          if (!direct && q == 0 && lane == 0) {
+          if (!direct && !a.by_row && q == 0 && lane == 0) {
             if (tlast) a.head[blockIdx.x] = make_int4(r.tok0, r.ntok, r.kvh, 0);
             if (tfirst) a.tail[blockIdx.x] = 1;
           }
@@ -380,6 +380,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             if (had && valid && ((k.poison(r.item)[irow >> 5] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
             const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
             if (!direct && valid) a.ml[prow] = make_float2(ref, lt);
+            if (a.by_row && valid && jrow == 0) {
+              if (tfirst) a.first[(long)r.kvh * a.T + t] = direct ? -1 : (int)blockIdx.x;
+              if (tlast) a.last[(long)r.kvh * a.T + t] = (int)blockIdx.x;
+            }
             const float inv = lt == 0.f ? 0.f : 1.0f / lt;
             __half *y = a.Y + (long)t * a.ystride + (long)(r.kvh * a.r + jrow) * D;
             float *po = a.O + prow * D;
@@ -657,12 +661,12 @@ Ws ws_layout(int T, int heads, int kv, int D, int ctas) {
   return w;
 }
 
-// The kernel for few rows where a group has four tiles or less. Measured, few against many rows' kernel, us: decode of 64
-// sequences over a prefix of 32,768 tokens 36 against 40, over 24 prefixes of 6,000 100 against 97, of one sequence over
-// 30,000 keys 26 against 27 (D = 64: 23 against 27); 32 groups of 3 questions of 40 tokens over 512 tokens 61 against 64;
-// about 300 rows over 16,000 keys 39 against 43 (D = 64: 36 against 37). 1,100 rows over 16,000 keys 75 against 64, 4,500
-// rows 276 against 208. (64 groups of 40 rows gain at 500 keys, 46 against 55, and lose at 4,000, 171 against 158; how long
-// a prefix is the host does not know.) At D = 256 the accumulators of two CTAs do not fit.
+// The kernel for few rows where a group has four tiles or less. Measured, few against many rows' kernel, us: decode of 218
+// sequences over 24 prefixes, D = 64, 90 against 94; about 300 rows over 16,000 keys 35 against 40, D = 128 39 against 42; 32
+// groups of 3 questions of 40 tokens over 512 tokens 58 against 60; 64 of 2 x 20 tokens over 500 tokens 34 against 44, D = 128
+// 43 against 53. 1,100 rows over 16,000 keys 62 against 56, D = 128 74 against 61; 4,500 rows 176 against 159, D = 128 260
+// against 206. (Over 4,000 tokens 64 groups of 2 x 20 would gain by the other, 171 against 157; how long a prefix is the host
+// does not know.) At D = 256 the accumulators of two CTAs do not fit.
 bool paged_few(int D, int T, int r, int G) { return D <= 128 && (long)T * r <= 512L * std::max(G, 1); }
 
 template <int D>
@@ -687,12 +691,11 @@ int launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs, PArgs a, b
     rc = dc_launch_check("attention_paged");
   }
   if (rc) return rc;
-  if constexpr (D <= 128)
-    if (a.by_row) {
-      const dim3 grid((unsigned)((long)a.T * a.heads));
-      DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D>, grid, dim3(128), 0, a));
-      return dc_launch_check("attention_paged (join)");
-    }
+  if (a.by_row) {
+    const dim3 grid((unsigned)((long)a.T * a.heads));
+    DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_kernel<D>, grid, dim3(128), 0, a));
+    return dc_launch_check("attention_paged (join)");
+  }
   constexpr int R = 4 * JoinRows<D>::R;  // of a block
   const dim3 grid((unsigned)((std::min((long)a.T * a.r, 128L) + R - 1) / R), a.ctas);
   DC_CUDA(dc_launch_pdl(ctx->stream, attention_join_tiles_kernel<D>, grid, dim3(128), 0, a));
@@ -737,9 +740,10 @@ int attn_paged_launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs,
   // Few tiles are cut into many parts each, and a join by row takes them up in four warps (one sequence over 30,000 keys 26
   // us against 48 by tile, 35 over a shared prefix 36 against 67, 8 groups of 4 x 16 tokens 20 against 23). Many tiles are
   // whole or in two or three parts, and blocks for rows that were not cut would cost more than the tiles' search (24 groups
-  // of 12 tokens 95 us by row, 91 by tile; 16 groups of 8 x 8 tokens 34 and 31; 32 of 3 questions 54 and 41).
+  // of 12 tokens 95 us by row, 91 by tile; 16 groups of 8 x 8 tokens 34 and 31; 32 of 3 questions 54 and 41). At D = 256
+  // fewer such blocks fit an SM: 4,000 rows 43 us by row, 41 by tile; 400 rows 35 and 36; one 25 and 40.
   const long groups = std::max(G, 1), tiles = c->kv * groups * (((long)T * a.r + 128 * groups - 1) / (128 * groups));
-  a.by_row = few && 3 * tiles <= ctas;
+  a.by_row = 3 * tiles <= ctas && (c->D < 256 || (long)T * heads <= 2048);
   a.y32 = (reinterpret_cast<uintptr_t>(Y) & 31) == 0 && ys % 16 == 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   if (c->D == 64) return launch<64>(ctx, c, Q, qs, a, few);

@@ -332,6 +332,17 @@ def test_attention_paged_cut_over_many_ctas(ctx, dev, heads, kv, D, page, n, ple
     c.check()
 
 
+@pytest.mark.parametrize("heads,kv,D,many,after", [(16, 8, 128, 70, 0), (2, 1, 64, 120, 0), (2, 1, 64, 120, 31000), (2, 1, 128, 120, 31000),
+                                                   (8, 4, 256, 60, 0)])
+def test_attention_paged_one_long_group_among_short_ones(ctx, dev, heads, kv, D, many, after):
+    """One tile in a hundred parts and more among many that are whole."""
+    c = Case(ctx, dev, [(20, [(1, 5)]), (30000, [(3, 5), (1, 70)])] + [(i % 3, [(1, 5 + i)]) for i in range(many)], heads, kv, D, 64,
+             after=after, seed=many)
+    c.call()
+    ctx.sync(60000)
+    c.check()
+
+
 @pytest.mark.parametrize("heads,kv,D", [(16, 8, 128), (32, 8, 64), (8, 2, 256)])
 def test_attention_paged_without_groups(ctx, dev, heads, kv, D):
     c = Case(ctx, dev, [(0, [(1, 40 + i) for i in range(50)] + [(70, 100), (2, 2), (0, 0), (9, 300)])], heads, kv, D, 16, prefixes=False,
