@@ -640,11 +640,13 @@ int encode(CUtensorMap *m, const void *p, int rank, const cuuint64_t *dims, cons
   return DC_OK;
 }
 
-size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
+size_t up(size_t x) { return (x + 255) & ~(size_t)255; }  // (WS_ALIGN)
 
 // The workspace: a status word, the join's records, parts' maxima and sums, parts' sums of values. Part c of a tile
 // starts at row (kvh T + first row) r + 128 c: along the line either the tile moves on, by at least its rows, or c does,
-// so no two parts meet.
+// so no two parts meet. The caller's address is a multiple of 16; the layout starts at the next multiple of WS_ALIGN (parts
+// are stored in 32-byte pieces, records of 16 and 8 bytes).
+constexpr size_t WS_ALIGN = 256;
 struct Ws {
   size_t first, last, head, tail, ml, O, bytes;
 };
@@ -657,7 +659,7 @@ Ws ws_layout(int T, int heads, int kv, int D, int ctas) {
   w.tail = w.head + up((size_t)ctas * 16);
   w.ml = w.tail + up((size_t)ctas * 4);
   w.O = w.ml + up(rows * 8);
-  w.bytes = w.O + up(rows * (size_t)D * 4);
+  w.bytes = w.O + up(rows * (size_t)D * 4) + WS_ALIGN - 16;
   return w;
 }
 
@@ -720,7 +722,7 @@ int attn_paged_launch(dc_ctx *ctx, const dc_kv_cache *c, const void *Q, long qs,
                       const int *lens, const int *qoff, int S, const int *ptable, int pstride, const int *plens,
                       const int *goff, int G, void *Y, long ys, int T, int heads, float scale, void *ws) {
   const Ws w = ws_layout(T, heads, c->kv, c->D, 2 * ctx->sms);
-  char *p = static_cast<char *>(ws);
+  char *p = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(ws) + WS_ALIGN - 1) & ~(uintptr_t)(WS_ALIGN - 1));
   PArgs a;
   a.Y = static_cast<__half *>(Y), a.ystride = ys;
   a.table = table, a.lens = lens, a.qoff = qoff, a.ptable = ptable, a.plens = plens, a.goff = goff;
