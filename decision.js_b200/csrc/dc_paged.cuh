@@ -13,6 +13,9 @@
 namespace dcx {
 
 constexpr int PA_RING = 4;    // runs handed out ahead
+// Tiles whose rows' marks (128 bits each) are held at a time. A tile's are cleared PA_RING tiles ahead (look_over), while
+// those of up to PA_RING tiles before may still be read.
+constexpr int PA_MARKS = 2 * PA_RING, PA_MARK_BYTES = PA_MARKS * 16;
 constexpr int PA_GOFF = 512;  // groups and sequences whose offsets and lengths are kept in shared memory
 constexpr int PA_META = 4 * (PA_GOFF + 4) * 4;  // bytes
 
@@ -190,7 +193,11 @@ struct Cta {
   __device__ __forceinline__ volatile int *abort() const { return reinterpret_cast<volatile int *>(smem + C::MISC_OFF + 4); }
   __device__ __forceinline__ int *start() const { return reinterpret_cast<int *>(smem + C::MISC_OFF + 8); }
   __device__ __forceinline__ volatile uint32_t *poison(int item) const {  // marked rows of a tile, 128 bits
-    return reinterpret_cast<volatile uint32_t *>(smem + C::POISON_OFF) + 4 * (item & 3);
+    return reinterpret_cast<volatile uint32_t *>(smem + C::POISON_OFF) + 4 * (item % PA_MARKS);
+  }
+  // every thread, before the first barrier: no marks
+  __device__ __forceinline__ void clear_marks() const {
+    if (tid < PA_MARK_BYTES / 4) reinterpret_cast<uint32_t *>(smem + C::POISON_OFF)[tid] = 0;
   }
   __device__ __forceinline__ Run *runs() const { return reinterpret_cast<Run *>(smem + C::RUN_OFF); }
   __device__ __forceinline__ bool wait(int i, int parity) const {
@@ -486,7 +493,11 @@ __device__ __forceinline__ bool to_look_over(const Run &r, int key0) {
 
 // Looks those blocks over, one warp: the rows past the last key are zeroed, and values that are not finite too where some
 // row would multiply them by a weight of 0, with a mark on the rows that see them. The product of the c-th of them waits
-// for barrier B_VS + c % VST; the others go straight from V's arrival.
+// for barrier B_VS + c % VST; the others go straight from V's arrival, so a tile without such a block can end, and its marks
+// be read, before this warp has come to it. Its marks are therefore cleared earlier, and the ring of runs gives the order:
+// at the start of tile i this warp clears those of tile i + PA_RING, whose runs are handed out only after its done_run of a
+// run of tile i or later (a tile has at least one run, the ring PA_RING); the place was last that of tile i - PA_RING, whose
+// last run every reader has given back before tile i's first is handed out. The first PA_RING tiles: clear_marks.
 template <class C>
 __device__ __forceinline__ void look_over(const Cta<C> &k) {
   constexpr int KB = C::KB, VST = C::VST, NA = C::NA;
@@ -496,7 +507,7 @@ __device__ __forceinline__ void look_over(const Cta<C> &k) {
   bool ok = true;
   for (int n = 0; ok && k.next_run(n, r); n++) {
     volatile uint32_t *mark = k.poison(r.item);
-    if ((r.flags & RUN_FIRST) && lane < 4) mark[lane] = 0;
+    if ((r.flags & RUN_FIRST) && lane < 4) k.poison(r.item + PA_RING)[lane] = 0;
     __syncwarp();
     for (int b = 0; b < r.nb; b++, g++) {
       const int st = g % VST, key0 = (r.kb + b) * KB;

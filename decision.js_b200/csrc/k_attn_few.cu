@@ -47,13 +47,13 @@ struct FewCfg {
                        B_KF = B_PF + SB, B_KE = B_KF + KST, B_VF = B_KE + KST, B_VE = B_VF + VST, B_VS = B_VE + VST,
                        B_IF = B_VS + VST, B_IE = B_IF + PA_RING, NBARS = B_IE + PA_RING;
   static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15);
-  static constexpr int POISON_OFF = MISC_OFF + 32, SCAN_OFF = POISON_OFF + 64,
+  static constexpr int POISON_OFF = MISC_OFF + 32, SCAN_OFF = POISON_OFF + PA_MARK_BYTES,
                        RUN_OFF = SCAN_OFF + ((F_THREADS / 32 * 8 + 15) & ~15), GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run),
                        XCH_OFF = GOFF_OFF + PA_META;  // (value, turn) [2 turns][2 halves][128 rows]
   static constexpr int SMEM = XCH_OFF + 2 * 2 * 128 * 8 + 1024;
   static constexpr int S_COL = 0, O_COL = SB * KB, TCOLS = 256;
   static_assert(O_COL + D <= TCOLS, "tensor memory");
-  static_assert(2 * SMEM <= 227 * 1024, "shared memory");
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "shared memory");  // (1 KB of each CTA's is the system's)
 };
 
 template <int D>
@@ -76,6 +76,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     *k.abort() = 0;
     mbar_init_fence();
   }
+  k.clear_marks();
   for (int i = tid; i < 512; i += F_THREADS) reinterpret_cast<int2 *>(k.smem + C::XCH_OFF)[i] = make_int2(0, 0);
   if (warp == FW_K && lane == 0) tma_prefetch_desc(&tmQ), tma_prefetch_desc(&tmK);
   if (warp == FW_V && lane == 0) tma_prefetch_desc(&tmV);

@@ -74,7 +74,7 @@ struct WideCfg {
                        NBARS = B_IE + PA_RING;
   static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15);
   // misc: tmem slot, abort, start (s, offset); poison; scan; runs; groups; references and sums
-  static constexpr int POISON_OFF = MISC_OFF + 32, SCAN_OFF = POISON_OFF + 64,
+  static constexpr int POISON_OFF = MISC_OFF + 32, SCAN_OFF = POISON_OFF + PA_MARK_BYTES,
                        RUN_OFF = SCAN_OFF + ((PA_THREADS / 32 * 8 + 15) & ~15), GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run),
                        XCH_OFF = GOFF_OFF + PA_META;
   static constexpr int SMEM = XCH_OFF + 128 * 4 + 4 * PA_WG * 128 * 8 + 1024;
@@ -110,6 +110,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     *k.abort() = 0;
     mbar_init_fence();
   }
+  k.clear_marks();
   if (warp == PA_WK && lane == 0) tma_prefetch_desc(&tmQ), tma_prefetch_desc(&tmK);
   if (warp == PA_WV && lane == 0) tma_prefetch_desc(&tmV);
   // Tensor memory is taken only when the kernels before are done, and the next kernel is let in only when every CTA

@@ -31,3 +31,30 @@ def test_workspace_at_any_multiple_of_16(ctx, dev, heads, kv, D, groups, after, 
     ctx.sync(60000)
     c.check()
     assert (whole[:lead] == 0xA5).all() and (whole[lead + n:] == 0xA5).all()
+
+
+@pytest.mark.parametrize("heads,kv,D,after", [(16, 8, 128, 0), (8, 2, 128, 54000), (32, 8, 64, 0), (32, 8, 64, 54000), (8, 4, 256, 0)])
+def test_marks_of_one_tile_reach_no_other(ctx, dev, heads, kv, D, after):
+    """Tiles in a row in which a row sees a value that is not finite (and is marked) among tiles of one block that nothing
+    is looked over in (one token, own keys a multiple of 16), whose end does not wait for that: only rows that see such a
+    value are not finite, in call after call."""
+    import torch
+    n = 420
+    groups = [(0, [(3, 19)]) if i % 5 == 0 else (0, [(1, 16 * (1 + i % 4))]) for i in range(n)]
+    c = Case(ctx, dev, groups, heads, kv, D, 16, after=after, seed=4)
+    broken = []
+    for s in range(0, n, 5):
+        p, off = c.table[s, 1], 18 - 16  # its last token: its last row alone sees it
+        c.v[p, :, off, 3] = np.nan
+        broken.append(int(c.qoff[s + 1]) - 1)
+    c.dv.copy_(_half(c.v, dev))
+    for i in range(60):
+        c.call()
+        if i % 20 == 0:
+            ctx.sync(60000)
+            finite = torch.isfinite(c.y).all(1)
+            assert finite.sum().item() == c.T - len(broken) and not finite[broken].any()
+    ctx.sync(60000)
+    for s in range(0, n, 5):
+        c.v[c.table[s, 1], :, 2, 3] = 0
+    c.check(rows=set(range(c.T)) - set(broken))
