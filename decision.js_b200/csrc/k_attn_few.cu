@@ -49,10 +49,11 @@ struct FewCfg {
   static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15);
   static constexpr int POISON_OFF = MISC_OFF + 32, SCAN_OFF = POISON_OFF + PA_MARK_BYTES,
                        RUN_OFF = SCAN_OFF + ((F_THREADS / 32 * 8 + 15) & ~15), GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run),
-                       XCH_OFF = GOFF_OFF + PA_META;  // (value, turn) [2 turns][2 halves][128 rows]
+                       XCH_OFF = GOFF_OFF + PA_META;  // (turn, value), 64 bits [2 turns][2 halves][128 rows]
   static constexpr int SMEM = XCH_OFF + 2 * 2 * 128 * 8 + 1024;
   static constexpr int S_COL = 0, O_COL = SB * KB, TCOLS = 256;
   static_assert(O_COL + D <= TCOLS, "tensor memory");
+  static_assert(XCH_OFF % 8 == 0, "64-bit accesses");
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "shared memory");  // (1 KB of each CTA's is the system's)
 };
 
@@ -189,19 +190,19 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     int t = 0;
     float ref = -FLT_MAX, l = 0.f;
     // Gives this half's value of the row and takes the other's: both write theirs with the number of the turn, in one
-    // store, and look for the other's (a half writes to a place again only when the other has read it: it has then seen
-    // the other's value of the turn between).
+    // 64-bit store (a vector of two would be two, in any order), and look for the other's (a half writes to a place again
+    // only when the other has read it: it has then seen the other's value of the turn between).
     auto meet = [&](float mine, float &theirs) -> bool {
       const uint32_t at = xch + (meets & 1) * 2048, mark = ++meets;
-      asm volatile("st.volatile.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + 1024 * hf), "f"(mine), "r"(mark) : "memory");
+      const uint64_t put = (uint64_t)mark << 32 | __float_as_uint(mine);
+      asm volatile("st.volatile.shared.b64 [%0], %1;" ::"r"(at + 1024 * hf), "l"(put) : "memory");
       uint64_t t0 = 0;
 #pragma unroll 1
       for (uint32_t i = 1;; i++) {
-        uint32_t seen;
-        asm volatile("ld.volatile.shared.v2.b32 {%0, %1}, [%2];"
-                     : "=f"(theirs), "=r"(seen)
-                     : "r"(at + 1024 * (hf ^ 1))
-                     : "memory");
+        uint64_t got;
+        asm volatile("ld.volatile.shared.b64 %0, [%1];" : "=l"(got) : "r"(at + 1024 * (hf ^ 1)) : "memory");
+        const uint32_t seen = (uint32_t)(got >> 32);
+        theirs = __uint_as_float((uint32_t)got);
         if (__all_sync(0xffffffffu, seen == mark)) return true;
         if ((i & 1023) == 0) {
           const uint64_t now = globaltimer();

@@ -58,3 +58,35 @@ def test_marks_of_one_tile_reach_no_other(ctx, dev, heads, kv, D, after):
     for s in range(0, n, 5):
         c.v[c.table[s, 1], :, 2, 3] = 0
     c.check(rows=set(range(c.T)) - set(broken))
+
+
+@pytest.mark.parametrize("heads,kv,D,n", [(2, 1, 128, 1), (16, 8, 128, 40), (32, 8, 64, 1), (4, 2, 64, 120)])
+def test_maxima_that_move_from_half_to_half(ctx, dev, heads, kv, D, n):
+    """In the kernel for few rows two warps share a row, half of a block's 64 keys each, and exchange maxima. Here the
+    largest score of each block is 2^12 above the one before and lies in the halves in turn: with a maximum of an earlier
+    turn the weights would leave f16's range."""
+    import torch
+    c = Case(ctx, dev, [(2500, [(1, 70 + i % 3) for i in range(n)])], heads, kv, D, 64, qscale=0)
+    c.q[:] = 0
+    c.q[:, 0::D] = 1
+    step = 12 * np.log(2)
+    for pages, length, start in [(c.ptable[0], 2500, 0)] + [(c.table[s], c.lens[s], 2560) for s in range(n)]:
+        for j in range(-(-length // 64)):
+            block = start // 64 + j
+            score = np.full(64, step * block - 30)
+            score[32 * (block & 1) + 5] = step * block
+            m = min(64, length - 64 * j)
+            if m <= 32 * (block & 1) + 5:
+                score[m - 1] = step * block
+            c.k[pages[j], :, :m] = 0
+            c.k[pages[j], :, :m, 0] = score[:m]
+    c.scale = 1.0
+    c.dq.copy_(_half(c.q, dev)), c.dk.copy_(_half(c.k, dev))
+    torch.cuda.synchronize()
+    c.call()
+    first = c.y.clone()
+    for _ in range(50):
+        c.call()
+    ctx.sync(60000)
+    c.check()
+    assert torch.equal(first, c.y)
