@@ -113,9 +113,10 @@ static __device__ __forceinline__ long seq_cost(int tpt, Group g, int qb, int qe
   return c;
 }
 
-// The page ids of a sequence's first 32 pages, read while the run before it is loaded (lanes past the table: 0).
-__device__ __forceinline__ int read_ahead(const PArgs &a, int s, int lane) {
-  return s < a.S && lane < a.tstride ? a.table[(long)s * a.tstride + lane] : 0;
+// The page ids of a sequence's first 32 pages (`len` tokens), read while the run before it is loaded (lanes past them: 0;
+// the table's row may end there, and the tensor with it).
+__device__ __forceinline__ int read_ahead(const PArgs &a, int s, int len, int lane) {
+  return s < a.S && lane < (len + a.page - 1) >> a.pshift ? a.table[(long)s * a.tstride + lane] : 0;
 }
 
 static __device__ __noinline__ void bad_page(uint32_t *err) { atomicOr(err, (uint32_t)DC_DEVERR_BOUNDS); }
@@ -356,7 +357,7 @@ __device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, con
   int lo = qb - gr.tg, hi = qe - gr.tg, ts = lo / a.tpt * a.tpt;  // from the group's first row; ts: the piece's tile
   // the next sequence's offset, length and first pages, on their way while this one's blocks are loaded
   int nqe = s + 1 < a.S ? gs.qoff[s + 2] : 0, nlen = s + 1 < a.S ? gs.lens[s + 1] : 0;
-  int ahead_seq = -1, ahead = 0, coming = read_ahead(a, s + 1, lane);
+  int ahead_seq = -1, ahead = 0, coming = read_ahead(a, s + 1, nlen, lane);
   auto advance = [&]() {
     do {
       if (++s == a.S) {
@@ -368,7 +369,7 @@ __device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, con
         ahead_seq = s, ahead = coming;
       }
       if (s + 1 < a.S) nqe = gs.qoff[s + 2], nlen = gs.lens[s + 1];
-      coming = read_ahead(a, s + 1, lane);
+      coming = read_ahead(a, s + 1, nlen, lane);
     } while (qe <= qb && kvh < a.kv);
     while (gi + 1 < a.G && gs.goff[gi + 1] <= s) gi++;
     gr = group_of<KB>(gs, gi);

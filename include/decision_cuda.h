@@ -323,13 +323,14 @@ DC_API int dc_kv_append(dc_ctx *ctx, const dc_kv_cache *cache, const dc_rope_pla
  * (fewer own tokens than rows leave the first rows none). Y (ystride halves a row) gets softmax(scale q . k) v, heads
  * by GQA as in dc_attention; a row with no key gets zeros. Rows outside [d_qoff[0], d_qoff[S]) are not written and
  * have no influence (rows next to a sequence's may be fetched with it), nor has anything of the cache past a length.
- * Scores and sums are f32; the weights are rounded to f16 for the product with v, the output to f16 once. A value row that is not finite stays out of the rows that do not see it; those that do
- * get NaN in its columns or in the whole head.
+ * Scores and sums are f32; the weights are rounded to f16 for the product with v, the output to f16 once. A value row
+ * that is not finite stays out of the rows that do not see it; those that do get NaN in its columns or in the whole head.
  * Offsets must not fall, qoff must lie in [0, T], goff start at 0 and end at S, lens and plens fit their table's row;
  * otherwise nothing is written, and the next dc_sync returns DC_EINVAL, as it does for a page id outside the cache
- * (which reads zeros). Table entries past a length may hold anything. Q and Y must not overlap unless Y is Q with its
- * stride. d_ws: at least dc_attention_paged_workspace bytes, 16-byte aligned, apart from Q, Y and the cache, for this
- * call alone until it has run (calls on one stream can share it; graphs that may run at the same time cannot). heads / kv at most 64; strides are multiples
+ * (which reads zeros). Table entries past a length may hold anything and are not read (a table may be columns of a wider
+ * array). Q and Y must not overlap unless Y is Q with its stride. d_ws: at least dc_attention_paged_workspace bytes,
+ * 16-byte aligned, apart from Q, Y and the cache, for this call alone until it has run (calls on one stream can share it;
+ * graphs that may run at the same time cannot). heads / kv at most 64; strides are multiples
  * of 8; Q, Y 16-byte aligned. Runs of one input give the same bits. */
 DC_API int dc_attention_paged(dc_ctx *ctx, const dc_kv_cache *cache, const void *d_Q, long qstride,
                               const int32_t *d_table, int table_stride, const int32_t *d_lens, const int32_t *d_qoff,

@@ -90,3 +90,32 @@ def test_maxima_that_move_from_half_to_half(ctx, dev, heads, kv, D, n):
     ctx.sync(60000)
     c.check()
     assert torch.equal(first, c.y)
+
+
+@pytest.mark.parametrize("heads,kv,D,after", [(16, 8, 128, 0), (16, 8, 128, 4000), (32, 8, 64, 0), (8, 2, 256, 0)])
+@pytest.mark.parametrize("S", [5, 600])
+def test_tables_that_end_with_their_memory(ctx, dev, pkg, heads, kv, D, after, S):
+    """Tables that are the last columns of wider arrays (rows far apart): of a row the pages of its length are read and
+    nothing behind them, which for the last row is the end of the allocation."""
+    from decision_js_b200._lib import lib
+    c = Case(ctx, dev, [(40, [(1, 1 + i % 20) for i in range(S)])], heads, kv, D, 16, after=after, seed=S)
+    stride, size = 48, 2 << 20
+    held = []
+    for name, rows in (("table", c.table), ("ptable", c.ptable)):
+        at = ctypes.c_void_p()
+        assert lib().dc_alloc(ctx.h, size, ctypes.byref(at)) == 0
+        held.append(at)
+        need = [-(-n // 16) for n in (c.lens if name == "table" else c.plens)]
+        host = np.full(size // 4, 1 << 30, np.int32)
+        start = size // 4 - stride * (len(rows) - 1) - need[-1]  # row r at start + r * stride, the last one's pages at the end
+        for r, n in enumerate(need):
+            host[start + r * stride:start + r * stride + n] = rows[r, :n]
+        assert lib().dc_upload(ctx.h, at, host.ctypes.data, size) == 0
+        c.meta[name] = at.value + 4 * start
+    m = c.meta
+    ctx.call("attention_paged", c.cache, c.dq, c.dq.shape[1], m["table"], stride, m["lens"], m["qoff"], S, m["ptable"], stride,
+             m["plens"], m["goff"], 1, c.y, c.y.shape[1], c.T, heads, c.scale, c.ws, c.ws.numel())
+    ctx.sync(60000)
+    c.check()
+    for at in held:
+        assert lib().dc_free(ctx.h, at) == 0
