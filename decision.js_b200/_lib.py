@@ -237,7 +237,7 @@ class Context:
         try:  # (a call's conversions are a good part of its time from the host)
             args = [a if type(a) in _PLAIN else a.data_ptr() for a in args]
         except AttributeError:
-            args = [a if type(a) in _PLAIN else ptr(a) for a in args]
+            args = [a if isinstance(a, (float, bool, type(None))) else ptr(a) for a in args]
         rc = getattr(lib(), "dc_" + name)(self.h, *args)
         if rc:
             check(rc)

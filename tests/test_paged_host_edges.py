@@ -2,6 +2,7 @@
 handles are test_paged_host.py's stand-ins."""
 import ctypes
 
+import numpy as np
 import pytest
 
 from test_paged_host import CACHE
@@ -23,3 +24,22 @@ def test_the_workspace_may_start_at_any_multiple_of_16(pkg, T, heads):
     """The header asks for 16 bytes, parts are stored 32 at a time: the layout (whole multiples of 256 bytes) starts at the
     next multiple of 256, up to 240 bytes behind the address given."""
     assert _workspace(T, heads) % 256 == 240
+
+
+def _no_context(pkg):
+    ctx = pkg.Context.__new__(pkg.Context)  # no device: a call's arguments are converted and checked, and it ends there
+    ctx.h = None
+    return ctx
+
+
+@pytest.mark.parametrize("eps", [1e-6, np.float64(1e-6)])
+def test_a_call_takes_any_float(pkg, eps):
+    """numpy's 64-bit scalar is a float, as it comes out of 1 / np.sqrt(D); with a host array next to it, too."""
+    import enum
+    ctx, x = _no_context(pkg), np.zeros(64, np.float32)
+    one = enum.IntEnum("One", dict(one=1)).one
+    for X in (0x10000, x):
+        with pytest.raises(pkg.DecisionError, match="null context"):
+            ctx.call("add_rmsnorm", X, None, 0x10000, 0x10000, one, 64, 0, eps)
+    with pytest.raises(TypeError):
+        ctx.call("add_rmsnorm", "x", None, 0x10000, 0x10000, 1, 64, 0, eps)
