@@ -263,7 +263,7 @@ class Context:
     def kv_cache(self, k, v):
         """A KvCache over two contiguous f16 tensors [pages, kv, page, D] on this context's device."""
         for x in (k, v):
-            if x.dim() != 4 or x.shape != k.shape or x.element_size() != 2 or not x.is_contiguous():
+            if x.dim() != 4 or x.shape != k.shape or str(x.dtype) != "torch.float16" or not x.is_contiguous():
                 raise DecisionError(DC_EINVAL, "decision.js: kv_cache: k and v are contiguous f16 [pages, kv, page, D]")
         pages, kv, page, D = k.shape
         h = ctypes.c_void_p()

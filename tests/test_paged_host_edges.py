@@ -43,3 +43,16 @@ def test_a_call_takes_any_float(pkg, eps):
             ctx.call("add_rmsnorm", X, None, 0x10000, 0x10000, one, 64, 0, eps)
     with pytest.raises(TypeError):
         ctx.call("add_rmsnorm", "x", None, 0x10000, 0x10000, 1, 64, 0, eps)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "int16", "float32", "uint8"])
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_cache_is_f16(pkg, dtype, which):
+    """Two-byte elements of another type would be read as f16."""
+    import torch
+    kv = [torch.zeros(2, 1, 16, 64, dtype=torch.float16) for _ in range(2)]
+    with pytest.raises(pkg.DecisionError, match="null context"):
+        _no_context(pkg).kv_cache(*kv)
+    kv[which] = kv[which].to(getattr(torch, dtype))
+    with pytest.raises(pkg.DecisionError, match="contiguous f16"):
+        _no_context(pkg).kv_cache(*kv)
