@@ -244,11 +244,14 @@ class Context:
 
     def rope_plan(self, rot: int, layout: str = "half", frequencies=None, factor: float | None = None, **scaling):
         """A RopePlan for the first `rot` dims of a head, layout "half" or "interleaved": by the given frequencies
-        (radians per position, [rot/2]) and factor on cos and sin, or by rope_frequencies(rot, **scaling)."""
+        (radians per position, [rot/2]) and factor on cos and sin, or by rope_frequencies(rot, factor=factor, **scaling),
+        whose factor is the context's and needs a scaling named."""
         if layout not in ROPE_LAYOUTS:
             raise DecisionError(DC_EINVAL, f"decision.js: rope_plan: unknown layout {layout!r}")
         if frequencies is None:
             if factor is not None:
+                if "scaling" not in scaling:
+                    raise DecisionError(DC_EINVAL, "decision.js: rope_plan: a factor without frequencies or a scaling")
                 scaling["factor"] = factor
             frequencies, factor = rope_frequencies(rot, **scaling)
         elif scaling:

@@ -56,3 +56,17 @@ def test_a_cache_is_f16(pkg, dtype, which):
     kv[which] = kv[which].to(getattr(torch, dtype))
     with pytest.raises(pkg.DecisionError, match="contiguous f16"):
         _no_context(pkg).kv_cache(*kv)
+
+
+def test_a_plan_refuses_a_factor_without_what_it_belongs_to(pkg):
+    """`factor` is the context's beside a scaling, that of cos and sin beside frequencies; alone it was left out."""
+    plan = _no_context(pkg).rope_plan
+    with pytest.raises(pkg.DecisionError, match="a factor without") as e:
+        plan(64, factor=8.0)
+    assert e.value.code == 1
+    with pytest.raises(pkg.DecisionError, match="a factor without"):
+        plan(64, theta=1e6, factor=8.0)
+    for good in (dict(), dict(theta=1e6), dict(scaling="linear", factor=8.0), dict(frequencies=[0.5] * 32, factor=8.0),
+                 dict(scaling="none", factor=8.0)):
+        with pytest.raises(pkg.DecisionError, match="null context"):
+            plan(64, **good)
