@@ -2,11 +2,15 @@
 //
 // Rotation: pair i of a head (dims i and i + rot/2, or 2i and 2i + 1) at position p turns by the angle p w_i:
 //   (a, b) -> f (a cos - b sin, b cos + a sin).
-// The angle is kept as a fraction of a turn in 64-bit fixed point: a plan holds w_i / 2 pi as a 64-bit fraction, and
-// p times it modulo 2^64 is the fraction of a turn left after the whole ones, with no rounding at all. A 32-bit
-// product p w_i would be off by 2^-24 of itself: 0.06 rad at a million radians. What is left is an angle in [-pi, pi),
-// where the hardware's sine and cosine are off by 2^-20.9 at most: 1/500 of the rounding of the result to f16 (for a pair
-// of equal size; sincospif's 24 bits cost 300 instructions a lane and token, a sixth of the append).
+// The angle is kept as a fraction of a turn in 64-bit fixed point: a plan holds w_i / 2 pi as a 64-bit fraction (53 bits of
+// it, as it comes from a double), and p times it modulo 2^64 is the fraction of a turn left after the whole ones, with no
+// further rounding. A 32-bit product p w_i would be off by 2^-24 of itself: 0.06 rad at a million radians. The nearest
+// quarter turns are taken out in the same fixed point, and cos and sin of what is left, at most pi/4, are their Taylor
+// series (cos_sin): off by 3.2 steps of 2^-24 of themselves at most (and 2^-54), however small, so that each term of a pair is
+// good to f32. The hardware's sine is off by 2^-21 of 1, which shows in results that are small beside their pair, by
+// hundreds of f16 steps. The series costs more instructions, so the lanes of a warp that need the same angles work
+// out a share each and exchange them (4,099 x 10 heads of 256, 64 dims, from the host: 9.2 us with the hardware's sine, 10.0
+// with the series in every lane, 9.3 shared; 2,332 rows of 32 + 2 x 8 heads of 64 appended 6.7, 7.6 and 6.6).
 //
 // Both kernels read and write each row once and are bound by memory (many tokens) or by the launch (few): the rotation of
 // 16,384 x 32 heads of 128 takes 42.9 us, 96% of the measured copy rate, the append of 16 x 1,024 tokens of 24 + 2 x 8 heads
@@ -41,21 +45,19 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   return u;
 }
 
-// factor * cos and factor * sin of eight consecutive pairs at position p
-__device__ __forceinline__ void angles8(const uint64_t *freq, int p, float factor, float (&cs)[8], float (&sn)[8]) {
-  uint64_t f[8];
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const ulonglong2 v = reinterpret_cast<const ulonglong2 *>(freq)[j];
-    f[2 * j] = v.x, f[2 * j + 1] = v.y;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; e++) {
-    const uint64_t turn = (uint64_t)(int64_t)p * f[e];  // modulo one turn
-    float s, c;
-    __sincosf((float)(int)(turn >> 32) * 1.4629180792671596e-9f, &s, &c);  // pi 2^-31
-    cs[e] = c * factor, sn[e] = s * factor;
-  }
+// cos and sin of `turn` / 2^64 turns. On |x| <= pi/4 the series' next terms, x^11 / 11! and x^12 / 12!, are below 2^-28 of sin
+// and 2^-32 of cos.
+__device__ __forceinline__ void cos_sin(uint64_t turn, float &cs, float &sn) {
+  const uint32_t hi = (uint32_t)(turn >> 32), quarter = (hi + (1u << 29)) >> 30;  // the nearest, modulo 4
+  const float x = fmaf((float)(int)(hi - (quarter << 30)), 1.4629180792671596e-9f,  // 2 pi 2^-32
+                       (float)(uint32_t)turn * 3.4061215800865545e-19f);            // 2 pi 2^-64
+  const float x2 = x * x;
+  const float p = fmaf(fmaf(fmaf(1.0f / 362880, x2, -1.0f / 5040), x2, 1.0f / 120), x2, -1.0f / 6);
+  const float q = fmaf(fmaf(fmaf(fmaf(-1.0f / 3628800, x2, 1.0f / 40320), x2, -1.0f / 720), x2, 1.0f / 24), x2, -0.5f);
+  const float s = fmaf(x * x2, p, x), c = fmaf(x2, q, 1.0f);
+  const float a = quarter & 1 ? s : c, b = quarter & 1 ? c : s;
+  cs = __uint_as_float(__float_as_uint(a) ^ (((quarter + 1) & 2) << 30));
+  sn = __uint_as_float(__float_as_uint(b) ^ ((quarter & 2) << 30));
 }
 
 // The eight pairs of a unit, two 16-byte chunks: dims 8c.. and 8c + rot/2.. (half layout), or 16 dims in a row.
@@ -86,9 +88,29 @@ __device__ __forceinline__ int2 unit_chunks(int u, int rot) {
   return make_int2(u, u + nr);
 }
 
+// factor * cos and factor * sin of unit u's eight pairs at position p, for SH lanes of a warp, U apart, that need the same:
+// each works out 8 / SH of them (this one the sub-th). The whole warp calls it.
+template <int SH>
+__device__ __forceinline__ void angles8(const uint64_t *freq, bool turn, int u, int U, int sub, int p, float factor,
+                                        float (&cs)[8], float (&sn)[8]) {
+  constexpr int N = 8 / SH;
+  float c[N], s[N];
+#pragma unroll
+  for (int j = 0; j < N; j++) {
+    cos_sin(turn ? (uint64_t)(int64_t)p * freq[8 * u + N * sub + j] : 0, c[j], s[j]);  // modulo one turn
+    c[j] *= factor, s[j] *= factor;
+  }
+  const int first = (threadIdx.x & 31) - U * sub;
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    cs[e] = SH == 1 ? c[e % N] : __shfl_sync(0xffffffffu, c[e % N], first + U * (e / N));
+    sn[e] = SH == 1 ? s[e % N] : __shfl_sync(0xffffffffu, s[e % N], first + U * (e / N));
+  }
+}
+
 // A thread takes one unit of one token for every HS-th head, so that its angles serve all of them; consecutive
-// threads take the units of a head, then HS heads, then the next token.
-template <bool INTER>
+// threads take the units of a head, then HS heads, then the next token. SH lanes of a warp have the same unit and token.
+template <bool INTER, int SH>
 __global__ void __launch_bounds__(256) rope_kernel(const __half *X, long xs, const int *pos, __half *Y, long ys, int T,
                                                    int heads, int D, int rot, const uint64_t *freq, float factor,
                                                    int HS, int tpb) {
@@ -96,22 +118,23 @@ __global__ void __launch_bounds__(256) rope_kernel(const __half *X, long xs, con
   const int U = D / 16;
   const int u = threadIdx.x % U, rest = threadIdx.x / U, hs = rest % HS, tok = rest / HS;
   const long t = (long)blockIdx.x * tpb + tok;
-  if (tok >= tpb || t >= T) return;
   const int2 ch = unit_chunks<INTER>(u, rot);
   const __half *x = X + t * xs;
   __half *y = Y + t * ys;
-  const bool turn = u < rot / 16;
-  if (!turn && X == Y) return;
+  const bool turn = u < rot / 16 && tok < tpb && t < T;
+  const bool live = tok < tpb && t < T && (turn || X != Y);
   float cs[8], sn[8];
   constexpr int NB = 4;  // heads in flight
-  for (int h0 = hs; h0 < heads; h0 += NB * HS) {
+  for (int h0 = hs; h0 == hs || (live && h0 < heads); h0 += NB * HS) {
     uint4 ra[NB], rb[NB];
 #pragma unroll
     for (int i = 0; i < NB; i++) {
       const int h = h0 + i * HS;
-      if (h < heads) ra[i] = ld16(x + (long)h * D + 8 * ch.x), rb[i] = ld16(x + (long)h * D + 8 * ch.y);
+      if (live && h < heads) ra[i] = ld16(x + (long)h * D + 8 * ch.x), rb[i] = ld16(x + (long)h * D + 8 * ch.y);
     }
-    if (turn && h0 == hs) angles8(freq + 8 * u, pos[t], factor, cs, sn);  // while the first heads are on their way
+    // while the first heads are on their way
+    if (h0 == hs) angles8<SH>(freq, turn, u, U, hs % SH, turn ? pos[t] : 0, factor, cs, sn);
+    if (!live) return;
 #pragma unroll
     for (int i = 0; i < NB; i++) {
       const int h = h0 + i * HS;
@@ -179,7 +202,7 @@ __global__ void __launch_bounds__(256, 3) kv_append_kernel(const AppendArgs a) {
   if (slot >= a.nslots && lane == 0) atomicOr(a.err, (uint32_t)DC_DEVERR_BOUNDS);
   const int pg = slot >> a.pshift, off = slot & (a.page - 1);
   float cs[8], sn[8];
-  if (turn) angles8(a.freq + 8 * u, pos, a.factor, cs, sn);
+  if (a.rot) angles8<HPP>(a.freq, turn, u, U, sub, pos, a.factor, cs, sn);
   for (int p0 = wsub; p0 < npass; p0 += NP * a.W) {
     uint4 xa[NP], xb[NP];
 #pragma unroll
@@ -245,9 +268,14 @@ int ops_rope(dc_ctx *ctx, const dc_rope_plan *p, const void *X, long xs, const i
   const int HS = (int)std::min<long>(most, std::max<long>(want, std::min(4, most)));
   const int tpb = std::max(1, 256 / (U * HS));
   const dim3 grid((unsigned)((T + (long)tpb - 1) / tpb));
-  DC_CUDA(dc_launch_pdl(ctx->stream, p->layout == DC_ROPE_INTERLEAVED ? rope_kernel<true> : rope_kernel<false>, grid,
-                        dim3(256), 0, (const __half *)X, xs, pos, (__half *)Y, ys, T, heads, D, p->rot, p->d_freq,
-                        p->factor, HS, tpb));
+  // lanes of a warp with one unit and token: those of up to 32 / U heads
+  const int SH = 32 % U ? 1 : 32 / U >= 4 && HS % 4 == 0 ? 4 : 32 / U >= 2 && HS % 2 == 0 ? 2 : 1;
+  const bool inter = p->layout == DC_ROPE_INTERLEAVED;
+  auto *kernel = SH == 4   ? (inter ? rope_kernel<true, 4> : rope_kernel<false, 4>)
+                 : SH == 2 ? (inter ? rope_kernel<true, 2> : rope_kernel<false, 2>)
+                           : (inter ? rope_kernel<true, 1> : rope_kernel<false, 1>);
+  DC_CUDA(dc_launch_pdl(ctx->stream, kernel, grid, dim3(256), 0, (const __half *)X, xs, pos, (__half *)Y, ys, T, heads, D, p->rot,
+                        p->d_freq, p->factor, HS, tpb));
   return dc_launch_check("rope");
 }
 

@@ -5,7 +5,8 @@ import ctypes
 import numpy as np
 import pytest
 
-from test_gpu_paged import Case, _half
+import paged_ref as R
+from test_gpu_paged import SMALL, Case, _f16, _f64, _half, _i32, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -119,3 +120,66 @@ def test_tables_that_end_with_their_memory(ctx, dev, pkg, heads, kv, D, after, S
     c.check()
     for at in held:
         assert lib().dc_free(ctx.h, at) == 0
+
+
+# Rotation, each term by itself: a cos and b sin are the product of a value, of cos or sin and of the factor. In steps of
+# u = 2^-24: cos and sin are off by 3.2 of themselves (an angle of at most pi/4 from 64-bit fixed point by 2.4, its series by
+# the rest), the factor and the two products by one each: 7 u < 2^-21 of the term, however small it is beside the pair; the
+# sum rounds once to f32, which the f16 rounding's half step covers with the rest of the 2^-21. The plan's frequency, 53
+# bits, adds 2^-40 rad at the positions here.
+def _rotate_terms(x, pos, freq, factor, rot, layout):
+    i = np.arange(rot // 2)
+    a = i if layout == "half" else 2 * i
+    only = np.zeros(x.shape[-1])
+    only[a] = 1
+    only[rot:] = 1
+    ya, _ = R.rotate(x * only, pos, freq, factor, rot, layout)
+    yb, _ = R.rotate(x * (1 - only), pos, freq, factor, rot, layout)
+    size = R.rotate(np.abs(x), pos, freq, factor, rot, layout)[1]
+    y = ya + yb
+    return y, R.HALF_STEP * np.abs(y) + 2.0 ** -21 * (np.abs(ya) + np.abs(yb)) + 2.0 ** -40 * size + SMALL
+
+
+def _unequal(rng, T, heads, D, rot, layout):
+    """Pairs with a zero, with one value 2^12 times the other, and like ones; angles small, and next to quarter turns."""
+    x = _f16(rng, T, heads, D)
+    i = np.arange(rot // 2)
+    a, b = (i, i + rot // 2) if layout == "half" else (2 * i, 2 * i + 1)
+    x[:, 0, a], x[:, 1, b] = 0, 0
+    x[:, 2, a] *= np.float16(2.0 ** 12)
+    x[:, 3, b] *= np.float16(2.0 ** 12)
+    freq = np.empty(rot // 2)
+    n = rot // 4
+    freq[:n] = 10000.0 ** (-np.arange(n) / n)
+    freq[n:] = np.pi / 2 * (1 + 2.0 ** -rng.uniform(8, 24, rot // 2 - n))
+    return x, freq
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("D,rot", [(128, 128), (256, 64)])
+@pytest.mark.parametrize("op", ["rope", "append"])
+def test_rotation_of_unequal_pairs(ctx, dev, layout, D, rot, op):
+    """A result that is small beside its pair is as good as any: an angle's sine that is off by 2^-21, not of itself but
+    of 1, would show in it."""
+    import torch
+    rng = np.random.default_rng(D + rot)
+    T, heads, factor = 1500, 5, 1.25
+    x, freq = _unequal(rng, T, heads, D, rot, layout)
+    pos = rng.integers(0, 4096, T)
+    plan = ctx.rope_plan(rot, layout, frequencies=list(freq), factor=factor)
+    dp = _i32(pos, dev)
+    if op == "rope":
+        dx = _half(x.reshape(T, -1), dev)
+        y = torch.empty_like(dx)
+        torch.cuda.synchronize()
+        ctx.call("rope", plan, dx, heads * D, dp, y, heads * D, T, heads, D)
+    else:
+        k = torch.zeros(2, 1, 16, D, dtype=torch.float16, device=dev)
+        cache = ctx.kv_cache(k, torch.zeros_like(k))
+        z = _half(np.concatenate([x.reshape(T, -1), np.zeros((T, 2 * D), np.float16)], 1), dev)
+        y, slots = torch.empty(T, heads * D, dtype=torch.float16, device=dev), _i32([-1] * T, dev)
+        torch.cuda.synchronize()
+        ctx.call("kv_append", cache, plan, z, z.shape[1], None, None, 0.0, 0, dp, slots, y, heads * D, T, heads)
+    ctx.sync(60000)
+    want, tol = _rotate_terms(x.astype(np.float64), pos, freq, factor, rot, layout)
+    _within(_f64(y).reshape(T, heads, D), want, tol)
