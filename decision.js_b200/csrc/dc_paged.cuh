@@ -19,6 +19,8 @@ constexpr int PA_MARKS = 2 * PA_RING, PA_MARK_BYTES = PA_MARKS * 16;
 constexpr int PA_GOFF = 512;  // groups and sequences whose offsets and lengths are kept in shared memory
 constexpr int PA_META = 4 * (PA_GOFF + 4) * 4;  // bytes
 
+#define MINUS_INF __uint_as_float(0xff800000u)
+
 enum { RUN_FIRST = 1, RUN_LAST = 2, RUN_TFIRST = 4, RUN_TLAST = 8, RUN_END = 16 };
 
 // A run of blocks of one segment (the prefix or one sequence's own keys) for one tile.
@@ -41,7 +43,7 @@ struct PArgs {
   int *first, *last;
   int4 *head;
   int *tail;
-  float2 *ml;
+  float2 *ml;  // a part's (maximum, sum of weights) by row; (minus infinity, 0): keys were seen and all scored that
   float *O;
   uint32_t *err;
   long ystride;

@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     int g = 0, meets = 0;
     bool ok = true;
     // the tile's state
-    bool valid = false, anyv = false, had = false, tfirst = false;
+    bool valid = false, anyv = false, seen = false, tfirst = false;  // seen: the row has seen a key
     int t = 0;
     float ref = -FLT_MAX, l = 0.f;
     // Gives this half's value of the row and takes the other's: both write theirs with the number of the turn, in one
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
         t = r.tok0 + irow;
         valid = irow < r.ntok && irow < a.tpt;
         anyv = __any_sync(0xffffffffu, valid);
-        had = false, tfirst = (r.flags & RUN_TFIRST) != 0;
+        seen = false, tfirst = (r.flags & RUN_TFIRST) != 0;
         ref = -FLT_MAX, l = 0.f;
         if (anyv) {  // the accumulator to zero; the last tile's was read by this very warp
           const uint32_t z[16] = {};
@@ -233,6 +233,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
       // the run's keys that the row sees
       const int rlim = !valid ? 0 : r.seg < 0 ? r.kend : t >= r.qb && t < r.qe ? own_limit(t, r.qe, r.len) : 0;
       const int nb = r.nb, kb = r.kb;
+      seen = seen || (nb > 0 && rlim > kb * KB);
       // the run's first blocks that every row here sees whole (lanes without a row have no say)
       const int full = __reduce_min_sync(0xffffffffu, valid ? rlim : 0x7fffffff) / KB - kb;
       for (int b = 0; b < nb; b++, g++) {
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
           if (part)  // minus infinity where the row does not see the key
 #pragma unroll
             for (int e = 0; e < 32; e++) x[e] = hf * COLS + e < nv ? x[e] : 0xff800000u;
-          float m2[2] = {__uint_as_float(0xff800000u), __uint_as_float(0xff800000u)};
+          float m2[2] = {MINUS_INF, MINUS_INF};
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
             m2[0] = max3(m2[0], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
@@ -310,7 +311,6 @@ __global__ void __launch_bounds__(F_THREADS, 2)
         if (lane == 0) mbar_arrive(k.bar(C::B_PF + sb));
       }
       if (!ok) break;
-      had = had || nb > 0;
       if (r.flags & RUN_LAST) {
         const bool tlast = (r.flags & RUN_TLAST) != 0, direct = tfirst && tlast;
         if (!direct && !a.by_row && tid == 0) {
@@ -326,7 +326,8 @@ __global__ void __launch_bounds__(F_THREADS, 2)
         if (!(ok = k.wait_warp(C::B_OD, r.item))) break;
         tc_fence_after();
         if (anyv) {
-          if (had && valid && ((k.poison(r.item)[irow >> 5] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
+          if (seen && ((k.poison(r.item)[irow >> 5] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
+          if (seen && lt == 0.f) ref = MINUS_INF, lt = direct ? __int_as_float(0x7fc00000) : 0.f;  // nothing but minus infinity
           const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
           if (a.by_row && valid && jrow == 0 && hf == 0) {
             if (tfirst) a.first[(long)r.kvh * a.T + t] = direct ? -1 : (int)blockIdx.x;

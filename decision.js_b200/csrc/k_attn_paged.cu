@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const int prev = wg == 0 ? PA_WG - 1 : wg - 1;
     bool ok = true;
     // the tile's state
-    bool valid = false, anyv = false, had = false, tfirst = false;
+    bool valid = false, anyv = false, had = false, seen = false, tfirst = false;  // seen: the row has seen a key
     int t = 0;
     float ref = -FLT_MAX, l = 0.f;  // l: the sum of this thread's weights, in units of 2^(ref - 7)
     auto zero = [&]() {             // its rows' accumulators, for the next tile
@@ -238,12 +238,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         t = r.tok0 + irow;
         valid = irow < r.ntok && irow < a.tpt;
         anyv = __any_sync(0xffffffffu, valid);
-        had = false, tfirst = (r.flags & RUN_TFIRST) != 0;
+        had = seen = false, tfirst = (r.flags & RUN_TFIRST) != 0;
         ref = -FLT_MAX, l = 0.f;
       }
       // the run's keys that the row sees
       const int rlim = !valid ? 0 : r.seg < 0 ? r.kend : t >= r.qb && t < r.qe ? own_limit(t, r.qe, r.len) : 0;
       const int nb = r.nb, kb = r.kb, kend = r.kend;
+      seen = seen || (nb > 0 && rlim > kb * KB);
       // the run's first blocks that every row here sees whole (lanes without a row have no say)
       const int full = __reduce_min_sync(0xffffffffu, valid ? rlim : 0x7fffffff) / KB - kb;
       for (int b = (wg + PA_WG - g % PA_WG) % PA_WG; b < nb; b += PA_WG, turn++) {
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             tmem_st_wait();
             sc = 1.f;
           }
-          float m2[2] = {__uint_as_float(0xff800000u), __uint_as_float(0xff800000u)};
+          float m2[2] = {MINUS_INF, MINUS_INF};
 #pragma unroll 1
           for (int c = 0; c < cols; c += 32) {
             uint32_t x[32];
@@ -378,7 +379,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
               const float2 x = sums[(wg + w) % PA_WG * 128];
               lt += x.x * ex2_approx(x.y - ref);
             }
-            if (had && valid && ((k.poison(r.item)[irow >> 5] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
+            if (seen && ((k.poison(r.item)[irow >> 5] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
+            if (seen && lt == 0.f) ref = MINUS_INF, lt = direct ? __int_as_float(0x7fc00000) : 0.f;  // nothing but minus infinity
             const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
             if (!direct && valid) a.ml[prow] = make_float2(ref, lt);
             if (a.by_row && valid && jrow == 0) {
@@ -431,7 +433,8 @@ struct JoinRows {  // rows of a warp in the join by tile
 };
 
 // Joins the parts of the tiles that were cut: y = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over the CTAs c from the
-// tile's first to its last. For few rows in many parts: a block to a (row, head), each of its W warps every W-th part,
+// tile's first to its last; NaN, as the formula has it, where all keys that the row sees score minus infinity (parts of
+// weight 0 with that maximum). For few rows in many parts: a block to a (row, head), each of its W warps every W-th part,
 // joined in order of the warps.
 template <int D>
 __global__ void __launch_bounds__(128) attention_join_kernel(const PArgs a) {
@@ -461,9 +464,11 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PArgs a) {
   for (int k = 0; k < 4; k++)
     if (c0 + part + W * k <= c1) fetch(v[k], c0 + part + W * k);
   float M = -FLT_MAX, L = 0.f, o[N] = {};
+  bool low = false;  // a part that saw nothing but minus infinity
   for (int cb = c0 + part; cb <= c1; cb += 32 * W) {  // 32 parts at a time, usually all
     const int c = cb + W * lane;
     const float2 x = c <= c1 ? a.ml[base + 128L * c] : make_float2(-FLT_MAX, 0.f);
+    low = low || (x.y == 0.f && x.x == MINUS_INF);
     float m = x.y == 0.f ? -FLT_MAX : x.x;  // a part of weight 0 stored no values
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
@@ -507,7 +512,8 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PArgs a) {
   }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) L += __shfl_xor_sync(0xffffffffu, L, s);
-  if (lane == 0) s_m[part] = M, s_l[part] = L;
+  low = __any_sync(0xffffffffu, low);
+  if (lane == 0) s_m[part] = low && L == 0.f ? MINUS_INF : M, s_l[part] = L;
   __syncthreads();
   float all = -FLT_MAX;
 #pragma unroll
@@ -527,6 +533,9 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PArgs a) {
 #pragma unroll
     for (int w = 0; w < W; w++) o[e] += s_o[w][N * lane + e];
   }
+  if (L == 0.f)
+#pragma unroll
+    for (int w = 0; w < W; w++) L = s_m[w] == MINUS_INF ? __int_as_float(0x7fc00000) : L;
   const float inv = L == 0.f ? 0.f : 1.0f / L;
   __half *y = a.Y + t * a.ystride + (long)h * D + N * lane;
 #pragma unroll
@@ -558,6 +567,7 @@ __global__ void __launch_bounds__(128) attention_join_tiles_kernel(const PArgs a
   c0 -= __ffs(__ballot_sync(0xffffffffu, begins));
   const long base = ((long)tile.z * a.T + tile.x) * a.r + row0;  // part c of a row: 128 c rows on
   float M[R], L[R], o[R][N];
+  uint32_t low = 0;  // rows with a part that saw nothing but minus infinity
 #pragma unroll
   for (int i = 0; i < R; i++) {
     M[i] = -FLT_MAX, L[i] = 0.f;
@@ -603,6 +613,8 @@ __global__ void __launch_bounds__(128) attention_join_tiles_kernel(const PArgs a
           L[i] = fmaf(w, x[i][k].y, L[i]);
 #pragma unroll
           for (int e = 0; e < N; e++) o[i][e] = fmaf(w, v[i][k][e], o[i][e]);
+        } else {
+          low |= (x[i][k].x == MINUS_INF ? 1u : 0u) << i;
         }
     }
   }
@@ -610,7 +622,7 @@ __global__ void __launch_bounds__(128) attention_join_tiles_kernel(const PArgs a
   for (int i = 0; i < R; i++) {
     if (i >= rows) break;
     const int tok = (row0 + i) / a.r, h = tile.z * a.r + row0 + i - tok * a.r;
-    const float inv = L[i] == 0.f ? 0.f : 1.0f / L[i];
+    const float inv = L[i] != 0.f ? 1.0f / L[i] : (low >> i) & 1u ? __int_as_float(0x7fc00000) : 0.f;
     __half *y = a.Y + (long)(tile.x + tok) * a.ystride + (long)h * D + N * lane;
 #pragma unroll
     for (int e = 0; e < N; e += 2)

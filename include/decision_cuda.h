@@ -321,8 +321,9 @@ DC_API int dc_kv_append(dc_ctx *ctx, const dc_kv_cache *cache, const dc_rope_pla
  * d_ptable[g * ptable_stride + i]; G = 0: no prefixes. Query row i of the n of a sequence reads its group's whole
  * prefix and its own tokens [0, lens - n + 1 + i): its last query row sees all, as after dc_kv_append of the n rows
  * (fewer own tokens than rows leave the first rows none). Y (ystride halves a row) gets softmax(scale q . k) v, heads
- * by GQA as in dc_attention; a row with no key gets zeros. Rows outside [d_qoff[0], d_qoff[S]) are not written and
- * have no influence (rows next to a sequence's may be fetched with it), nor has anything of the cache past a length.
+ * by GQA as in dc_attention; a row with no key gets zeros (one whose scores are all minus infinity NaN, as the formula).
+ * Rows outside [d_qoff[0], d_qoff[S]) are not written and have no influence (rows next to a sequence's may be fetched
+ * with it), nor has anything of the cache past a length.
  * Scores and sums are f32; the weights are rounded to f16 for the product with v, the output to f16 once. A value row
  * that is not finite stays out of the rows that do not see it; those that do get NaN in its columns or in the whole head.
  * Offsets must not fall, qoff must lie in [0, T], goff start at 0 and end at S, lens and plens fit their table's row;

@@ -183,3 +183,43 @@ def test_rotation_of_unequal_pairs(ctx, dev, layout, D, rot, op):
     ctx.sync(60000)
     want, tol = _rotate_terms(x.astype(np.float64), pos, freq, factor, rot, layout)
     _within(_f64(y).reshape(T, heads, D), want, tol)
+
+
+# few rows and many, whole tiles, tiles in parts joined by row, and by tile
+LOW = [(16, 8, 128, [(0, [(1, 40), (2, 70), (3, 20)]), (0, [(1, 33)])], 0), (16, 8, 128, [(0, [(1, 40), (2, 70), (3, 20)])], 600),
+       (16, 8, 128, [(0, [(1, 9000), (1, 30)])], 0), (2, 1, 64, [(0, [(1, 9000), (1, 30)])], 600), (4, 2, 256, [(0, [(1, 5000), (1, 90)])], 0),
+       (16, 8, 128, [(0, [(40, 2000 + i), (1, 7)]) for i in range(20)], 0), (32, 8, 64, [(0, [(40, 2000 + i), (1, 7)]) for i in range(20)], 4000),
+       (8, 2, 256, [(0, [(40, 2000 + i), (1, 7)]) for i in range(20)], 0)]
+
+
+@pytest.mark.filterwarnings("ignore:invalid value")  # the reference's own NaN
+@pytest.mark.parametrize("heads,kv,D,groups,after", LOW)
+def test_rows_whose_scores_are_all_minus_infinity(ctx, dev, heads, kv, D, groups, after):
+    """A row that sees keys and scores minus infinity with each is NaN, as softmax is; one more key, which scores anything
+    else, has all the weight; rows without a key stay zeros."""
+    import torch
+    c = Case(ctx, dev, groups, heads, kv, D, 16, after=after, seed=len(groups))
+    c.q[:, 0::D] = 1
+    c.dq.copy_(_half(c.q, dev))
+    for s, n in enumerate(c.lens):
+        if s % 2 == 0:  # every key of the even sequences
+            for j in range(n):
+                c.k[c.table[s, j // 16], :, j % 16, 0] = -np.inf
+    c.dk.copy_(_half(c.k, dev))
+    c.call()
+    ctx.sync(60000)
+    rows = lambda s: range(int(c.qoff[s]), int(c.qoff[s + 1]))  # noqa: E731
+    low = [t for s in range(0, len(c.lens), 2) for t in rows(s)]
+    assert torch.isnan(c.y[low]).all()
+    c.check(rows=set(range(c.T)) - set(low))
+    for s in range(0, len(c.lens), 2):  # its first key
+        c.k[c.table[s, 0], :, 0, 0] = 1
+    c.dk.copy_(_half(c.k, dev))
+    c.call()
+    ctx.sync(60000)
+    c.check()
+    c.meta["lens"].zero_()
+    torch.cuda.synchronize()
+    c.call()
+    ctx.sync(60000)
+    assert (c.y[int(c.qoff[0]):int(c.qoff[-1])] == 0).all()
