@@ -13,7 +13,8 @@ pytestmark = pytest.mark.gpu
 
 # One sequence over 9,000 tokens and many over a long prefix (tiles in parts, joined by row and by tile; both kernels).
 CUT = [(16, 8, 128, [(9000, [(1, 2000)])], 0), (16, 8, 128, [(9000, [(1, 2000)])], 700), (32, 8, 64, [(5000, [(3, 9)] * 12)], 0),
-       (32, 8, 64, [(5000, [(40, 90)] * 12), (300, [(70, 70)])], 0), (8, 2, 256, [(4000, [(1, 5), (30, 40)])], 0)]
+       (32, 8, 64, [(3000, [(40, 90)] * 4), (300, [(70, 70)])], 0), (8, 2, 256, [(4000, [(1, 5), (30, 40)])], 0),
+       (24, 8, 128, [(3000, [(33, 40)] * 3)], 1500), (24, 8, 256, [(1500, [(33, 40)] * 3), (0, [(1, 3000)])], 700)]
 
 
 @pytest.mark.parametrize("heads,kv,D,groups,after", CUT)
@@ -188,8 +189,8 @@ def test_rotation_of_unequal_pairs(ctx, dev, layout, D, rot, op):
 # few rows and many, whole tiles, tiles in parts joined by row, and by tile
 LOW = [(16, 8, 128, [(0, [(1, 40), (2, 70), (3, 20)]), (0, [(1, 33)])], 0), (16, 8, 128, [(0, [(1, 40), (2, 70), (3, 20)])], 600),
        (16, 8, 128, [(0, [(1, 9000), (1, 30)])], 0), (2, 1, 64, [(0, [(1, 9000), (1, 30)])], 600), (4, 2, 256, [(0, [(1, 5000), (1, 90)])], 0),
-       (16, 8, 128, [(0, [(40, 2000 + i), (1, 7)]) for i in range(20)], 0), (32, 8, 64, [(0, [(40, 2000 + i), (1, 7)]) for i in range(20)], 4000),
-       (8, 2, 256, [(0, [(40, 2000 + i), (1, 7)]) for i in range(20)], 0)]
+       (16, 8, 128, [(0, [(8, 1500 + i), (1, 7)]) for i in range(14)], 0), (32, 8, 64, [(0, [(8, 1500 + i), (1, 7)]) for i in range(14)], 4000),
+       (8, 2, 256, [(0, [(8, 1500 + i), (1, 7)]) for i in range(14)], 300)]
 
 
 @pytest.mark.filterwarnings("ignore:invalid value")  # the reference's own NaN
