@@ -263,7 +263,7 @@ int ops_rope(dc_ctx *ctx, const dc_rope_plan *p, const void *X, long xs, const i
   // Heads apart: 4 (a warp's threads cover 64 U halves in a row) unless that leaves the card without threads. 16,384 x 32
   // heads: 42.9 us with 4, 46.9 with 1, 69.8 with as many as fit (each thread works its angles out for fewer heads); one
   // token of 32 heads 2.3 us with 4, 1.8 with as many as fit.
-  const long want = (148L * 2048 / 2 + (long)T * U - 1) / ((long)T * U);
+  const long want = (1024L * ctx->sms + (long)T * U - 1) / ((long)T * U);
   const int most = std::max(1, std::min(heads, 256 / U));
   const int HS = (int)std::min<long>(most, std::max<long>(want, std::min(4, most)));
   const int tpb = std::max(1, 256 / (U * HS));
@@ -296,7 +296,7 @@ int ops_kv_append(dc_ctx *ctx, const dc_kv_cache *c, const dc_rope_plan *p, cons
   // Warps per token: one, which works the angles out once for all heads, unless that leaves the card without warps.
   // 16 x 1,024 tokens of 24 + 2 x 8 heads: 57 us with one, 131 with a warp to every pass; one token 6.5 us with one, 2.7
   // with a warp to every pass.
-  a.W = (int)std::max<long>(1, std::min<long>(npass, (148L * 32 + T - 1) / T));
+  a.W = (int)std::max<long>(1, std::min<long>(npass, (32L * ctx->sms + T - 1) / T));
   const dim3 grid((unsigned)(((long)T * a.W + 7) / 8));
   const bool inter = p && p->layout == DC_ROPE_INTERLEAVED;
 #define APPEND(DD)                                                                                               \
