@@ -89,6 +89,13 @@ static __device__ __noinline__ bool mbar_nap_on(uint32_t bar, uint32_t parity, v
     }
   }
 }
+// Where a wait ran out, before the CTA ends and its shared and tensor memory goes to another: waits for what it has started
+// (copies, products) and nobody waits for any more, for a second at most.
+__device__ __forceinline__ void mbar_settle(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer();
+  while (!mbar_nap(bar, parity) && globaltimer() - t0 < 1000000000ull) {
+  }
+}
 // For the one thread whose wake-up time everything else waits for: it polls (a sleeper is woken some hundred cycles
 // late), for 10,000 tries at most, then sleeps.
 __device__ __forceinline__ bool mbar_wait_alert(uint32_t bar, uint32_t parity, volatile int *abort, uint32_t *err,

@@ -45,8 +45,8 @@ struct FewCfg {
   static constexpr int BAR_OFF = V_OFF + VST * KV_BYTES;
   static constexpr int B_QF = 0, B_QE = 1, B_OD = 2, B_OE = 3, B_OR = 4, B_SF = 5, B_PF = B_SF + SB,
                        B_KF = B_PF + SB, B_KE = B_KF + KST, B_VF = B_KE + KST, B_VE = B_VF + VST, B_VS = B_VE + VST,
-                       B_IF = B_VS + VST, B_IE = B_IF + PA_RING, NBARS = B_IE + PA_RING;
-  static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15);
+                       B_IF = B_VS + VST, B_IE = B_IF + PA_RING, B_END = B_IE + PA_RING, NBARS = B_END + 2;
+  static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15), LOADED_OFF = MISC_OFF + 20;
   static constexpr int POISON_OFF = MISC_OFF + 32, SCAN_OFF = POISON_OFF + PA_MARK_BYTES,
                        RUN_OFF = SCAN_OFF + ((F_THREADS / 32 * 8 + 15) & ~15), GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run),
                        XCH_OFF = GOFF_OFF + PA_META;  // (turn, value), 64 bits [2 turns][2 halves][128 rows]
@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     for (int i = 0; i < C::NBARS; i++) {
       const int n = i == C::B_OE || (i >= C::B_PF && i < C::B_PF + SB) ? FS
                     : i >= C::B_VE && i < C::B_VE + VST                ? 2
-                    : i >= C::B_IE                                     ? FS + 2
+                    : i >= C::B_IE && i < C::B_END                     ? FS + 2
                                                                        : 1;
       mbar_init(k.bar(i), n);
     }
@@ -367,7 +367,10 @@ __global__ void __launch_bounds__(F_THREADS, 2)
 
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *k.abort()) a.hdr[0] = 1;  // a wait ran out: the records may be missing
+  if (*k.abort()) {  // a wait ran out
+    if (tid == 0) a.hdr[0] = 1;  // the records may be missing
+    settle<C>(k.smem, FW_M, FW_M);
+  }
   if (warp == FW_M) {
     tc_fence_after();
     tmem_dealloc(tmem, C::TCOLS);

@@ -71,9 +71,9 @@ struct WideCfg {
   static constexpr int B_QF = 0, B_QE = 1, B_OE = 2, B_OD = 3, B_XB = 7, B_SF = 23, B_PF = B_SF + PA_WG,
                        B_SE = B_PF + PA_WG, B_CH = B_SE + PA_WG, B_KF = B_CH + 4 * PA_WG, B_KE = B_KF + KST, B_VF = B_KE + KST,
                        B_VE = B_VF + VST, B_VS = B_VE + VST, B_IF = B_VS + VST, B_IE = B_IF + PA_RING,
-                       NBARS = B_IE + PA_RING;
-  static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15);
-  // misc: tmem slot, abort, start (s, offset); poison; scan; runs; groups; references and sums
+                       B_END = B_IE + PA_RING, NBARS = B_END + 2;
+  static constexpr int MISC_OFF = BAR_OFF + ((NBARS * 8 + 15) & ~15), LOADED_OFF = MISC_OFF + 20;
+  // misc: tmem slot, abort, start (s, offset), loaded; poison; scan; runs; groups; references and sums
   static constexpr int POISON_OFF = MISC_OFF + 32, SCAN_OFF = POISON_OFF + PA_MARK_BYTES,
                        RUN_OFF = SCAN_OFF + ((PA_THREADS / 32 * 8 + 15) & ~15), GOFF_OFF = RUN_OFF + PA_RING * (int)sizeof(Run),
                        XCH_OFF = GOFF_OFF + PA_META;
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       const int n = i == C::B_OE || (i >= C::B_PF && i < C::B_PF + PA_WG) ? 4
                     : i >= C::B_XB && i < C::B_XB + 16                     ? PA_WG - 1
                     : i >= C::B_VE && i < C::B_VE + VST                    ? 2
-                    : i >= C::B_IE                                         ? PA_SOFT + 3
+                    : i >= C::B_IE && i < C::B_END                         ? PA_SOFT + 3
                                                                            : 1;
       mbar_init(bar(i), n);
     }
@@ -420,7 +420,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *k.abort()) a.hdr[0] = 1;  // a wait ran out: the records may be missing
+  if (*k.abort()) {  // a wait ran out
+    if (tid == 0) a.hdr[0] = 1;  // the records may be missing
+    settle<C>(k.smem, PA_WM, PA_WP);
+  }
   if (warp == PA_WM) {
     tc_fence_after();
     tmem_dealloc(tmem, C::TCOLS);
