@@ -350,7 +350,7 @@ __device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, con
   const PArgs &a = k.a;
   const int lane = k.lane;
   const int *s_start = k.start();
-  int item = -1, n = 0, queries = 0;  // tiles, runs, loads of Q
+  int item = -1, n = 0;  // tiles, runs
   bool ok = true, first = true;
   long pos = st.p0, off = (long)(uint32_t)s_start[1] | (long)s_start[2] << 32;  // on the line; in the sequence's pieces
   int s = s_start[0], kvh = st.kvh, gi = a.G ? gs.of(s) : 0;
@@ -425,7 +425,6 @@ __device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, con
           for (int j = 0; j < NA; j++)
             tma_load_3d(k.base + j * C::Q_ROWS * 128, tmQ, 64 * j, r.kvh * a.r, r.tok0, k.bar(C::B_QF));
         }
-        queries++;
         __syncwarp();
       }
       if (b == r.nb) break;
@@ -442,7 +441,7 @@ __device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, con
     k.runs()[n % PA_RING].flags = RUN_END;
     mbar_arrive(k.bar(C::B_IF + n % PA_RING));
   }
-  if (lane == 0) reinterpret_cast<int *>(k.smem + C::LOADED_OFF)[values] = stage | turn << 8 | queries << 9;  // for settle
+  if (lane == 0) reinterpret_cast<int *>(k.smem + C::LOADED_OFF)[values] = stage | turn << 8 | item << 9;  // for settle
 }
 
 // After a wait ran out and every role has stopped (the whole CTA calls it): the loads and products still in flight. Of a ring
@@ -453,10 +452,10 @@ static __device__ __noinline__ void settle(uint8_t *smem, int mma0, int mma1) {
   const uint32_t bars = smem_u32(smem) + C::BAR_OFF;
   const int tid = threadIdx.x, warp = tid >> 5;
   if (tid < 2) {
-    const int x = reinterpret_cast<int *>(smem + C::LOADED_OFF)[tid], stage = x & 255, turn = x >> 8 & 1, queries = x >> 9;
+    const int x = reinterpret_cast<int *>(smem + C::LOADED_OFF)[tid], stage = x & 255, turn = x >> 8 & 1, item = x >> 9;
     for (int s = 0; s < (tid ? C::VST : C::KST); s++)
       mbar_settle(bars + 8 * ((tid ? C::B_VF : C::B_KF) + s), s < stage ? turn ^ 1 : turn);
-    if (queries) mbar_settle(bars + 8 * C::B_QF, (queries - 1) & 1);
+    if (tid == 0) mbar_settle(bars + 8 * C::B_QF, item & 1);  // (the last tile's Q, if it was asked for)
   }
   __syncwarp();
   if ((warp == mma0 || warp == mma1) && elect_one()) {
