@@ -224,3 +224,77 @@ def test_rows_whose_scores_are_all_minus_infinity(ctx, dev, heads, kv, D, groups
     c.call()
     ctx.sync(60000)
     assert (c.y[int(c.qoff[0]):int(c.qoff[-1])] == 0).all()
+
+
+@pytest.mark.parametrize("heads,kv,D,groups,after", CUT + [(16, 8, 128, [(300, [(17, 17), (40, 55), (1, 1)]), (129, [(64, 64), (23, 90)])], 0)])
+def test_error_of_the_attention(ctx, dev, heads, kv, D, groups, after):
+    """The weights of the product with v are rounded to f16, off by 2^-11 of themselves; their sum is of the f32 ones. Scores
+    (D products summed in f32) and the exponential add less than 2^-11 again for the values here, the output rounds once: two
+    half steps of sum p |v| and one of the result."""
+    c = Case(ctx, dev, groups, heads, kv, D, 64, after=after, seed=21)
+    c.call()
+    ctx.sync(60000)
+    got = _f64(c.y)[:, :heads * D]
+    for t, (a, size) in c.want().items():
+        _within(got[t].reshape(heads, D), a, R.HALF_STEP * np.abs(a) + 2 * R.HALF_STEP * size + SMALL)
+
+
+@pytest.mark.parametrize("heads,kv,D,S", [(16, 8, 128, 5), (32, 8, 64, 3), (8, 2, 256, 4)])
+def test_a_captured_decode_step(ctx, dev, pkg, heads, kv, D, S):
+    """Append and attention of one token a sequence in one graph, replayed step after step with positions, slots and lengths
+    in the same arrays: each row is attention over all that was appended, from the cache's own contents."""
+    import torch
+    rng = np.random.default_rng(D)
+    page, state, steps = 16, 75, 6
+    width = 3
+    ids = list(rng.permutation(S * width + -(-state // page)))
+    trunk, own = [ids.pop() for _ in range(-(-state // page))], [[ids.pop() for _ in range(width)] for _ in range(S)]
+    n = S * width + len(trunk)
+    k, v = (torch.full((n, kv, page, D), float("nan"), dtype=torch.float16, device=dev) for _ in range(2))
+    for c in (k, v):
+        for i, p in enumerate(trunk):
+            m = min(page, state - i * page)
+            c[p, :, :m] = _half(_f16(rng, kv, m, D), dev)
+    cache, plan = ctx.kv_cache(k, v), ctx.rope_plan(D, scaling="linear", factor=2.0)
+    table, ptable, plens, goff, qoff = (_i32(x, dev) for x in (own, [trunk], [state], [0, S], range(S + 1)))
+    pos, slots, lens = (torch.zeros(S, dtype=torch.int32, device=dev) for _ in range(3))
+    w = (heads + 2 * kv) * D
+    z, y = torch.zeros(S, w, dtype=torch.float16, device=dev), torch.zeros(S, heads * D, dtype=torch.float16, device=dev)
+    ws = torch.empty(ctx.attention_paged_workspace(cache, S, heads, S, 1), dtype=torch.uint8, device=dev)
+
+    def step():
+        ctx.call("kv_append", cache, plan, z, w, None, None, 1e-6, 1, pos, slots, z, w, S, heads)
+        ctx.call("attention_paged", cache, z, w, table, width, lens, qoff, S, ptable, len(trunk), plens, goff, 1, y, heads * D, S, heads,
+                 D ** -0.5, ws, ws.numel())
+
+    def fill(have):
+        pos.copy_(_i32([state + h for h in have], dev)), lens.copy_(_i32([h + 1 for h in have], dev))
+        slots.copy_(_i32([pkg.kv_slots(own[s], page, h, 1)[0] for s, h in enumerate(have)], dev))
+        z.copy_(_half(_f16(rng, S, w), dev))
+        torch.cuda.synchronize()
+
+    have = [0] * S
+    fill(have)
+    step()  # (a kernel's first call sets its attributes)
+    ctx.sync(60000)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.ExternalStream(ctx.stream, device=dev)):
+        step()
+    for i in range(steps):
+        have = [h + 1 + (s * 7 if i == 2 else 0) % 11 for s, h in enumerate(have)] if i else [page - 2] * S
+        for s in range(S):  # what lies between is filled as an append would
+            for h in range(have[s]):
+                for c in (k, v):
+                    row = c[own[s][h // page], :, h % page]
+                    if torch.isnan(row).any():
+                        row.copy_(_half(_f16(rng, kv, D), dev))
+        fill(have)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = R.attention(_f64(z)[:, :heads * D].reshape(S, heads, D), _f64(k), _f64(v), own, [trunk],
+                           [(state, [(1, h + 1) for h in have])], 0, heads, kv, D ** -0.5)
+        got = _f64(y).reshape(S, heads, D)
+        for t, (a, size) in want.items():
+            _within(got[t], a, R.HALF_STEP * np.abs(a) + 2 * R.HALF_STEP * size + SMALL)
+    ctx.sync(60000)
+    del graph
