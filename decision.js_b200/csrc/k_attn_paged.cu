@@ -32,9 +32,9 @@
 // tile's last block sees to while the other two go on.
 //
 // What bounds it. Many rows over a long prefix (49 sequences of up to 50 tokens, 12,800 keys, 24 heads over 8, D = 128):
-// 208 to 220 us with the power clock, about 850 TFLOP/s, half the measured matrix rate; without the softmax it still takes
+// 208 to 224 us with the power clock, 810 to 870 TFLOP/s, half the measured matrix rate; without the softmax it still takes
 // 167, as every tile of 128 rows brings all its keys from L2 (about 39 bytes a clock and SM): only tiles of 256 rows would
-// change that, and tensor memory has no room for their scores next to two accumulators. Short tiles (a few blocks each):
+// change that, for which the tensor memory of one SM has no room (scores next to two accumulators), that of two would. Short tiles (a few blocks each):
 // the chain from a tile's last product over its stores to the next tile's first product, and the instruction caches, which
 // the roles' code (70 KB) does not fit: a look-up in four missed, and every loop that was rolled and every path that two
 // roles share has shortened such calls. Steps measured: two softmax warpgroups in turn 264 -> 245 us, three with 128-key

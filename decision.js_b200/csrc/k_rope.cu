@@ -13,8 +13,8 @@
 // with the series in every lane, 9.3 shared; 2,332 rows of 32 + 2 x 8 heads of 64 appended 6.7, 7.6 and 6.6).
 //
 // Both kernels read and write each row once and are bound by memory (many tokens) or by the launch (few): the rotation of
-// 16,384 x 32 heads of 128 takes 42.9 us, 96% of the measured copy rate, the append of 16 x 1,024 tokens of 24 + 2 x 8 heads
-// 57.3 us, 90% of it; one token takes 1.8 and 2.7 us within a graph.
+// 16,384 x 32 heads of 128 takes 42.2 us, 97% of the measured copy rate, the append of 16 x 1,024 tokens of 24 + 2 x 8 heads
+// 56.6 us, 91% of it; one token takes 1.6 and 2.5 us (all within a graph).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -164,7 +164,7 @@ struct AppendArgs {
 
 // W warps per token; a pass of a warp covers 32 / (D/16) of the token's q, k and v heads, U = D/16 lanes to a head
 // (one unit each). NP passes are loaded at a time, the next NP while these are worked on: 16 x 1,024 tokens take 57 us with
-// two passes at three blocks an SM, 68 with four at two blocks, 63 with two at four, 70 with three at three.
+// two passes at three blocks an SM, 67 with four at two blocks, 62 with two at four, 69 with three at three.
 template <int D, bool INTER>
 __global__ void __launch_bounds__(256, 3) kv_append_kernel(const AppendArgs a) {
   dc_pdl_begin();
@@ -261,14 +261,15 @@ int ops_rope(dc_ctx *ctx, const dc_rope_plan *p, const void *X, long xs, const i
              int heads, int D) {
   const int U = D / 16;
   // Heads apart: 4 (a warp's threads cover 64 U halves in a row) unless that leaves the card without threads. 16,384 x 32
-  // heads: 42.9 us with 4, 46.9 with 1, 69.8 with as many as fit (each thread works its angles out for fewer heads); one
-  // token of 32 heads 2.3 us with 4, 1.8 with as many as fit.
+  // heads: 42.2 us with 4, 57.6 with 1 (whose lanes share no angles), 68.6 with as many as fit (each thread has its angles for
+  // fewer heads); one token of 32 heads 2.4 us with 4, 1.6 with as many as fit.
   const long want = (1024L * ctx->sms + (long)T * U - 1) / ((long)T * U);
   const int most = std::max(1, std::min(heads, 256 / U));
   const int HS = (int)std::min<long>(most, std::max<long>(want, std::min(4, most)));
   const int tpb = std::max(1, 256 / (U * HS));
   const dim3 grid((unsigned)((T + (long)tpb - 1) / tpb));
-  // lanes of a warp with one unit and token: those of up to 32 / U heads
+  // Lanes of a warp with one unit and token, which share the angles' work: 4,099 x 10 heads of 256 9.3 us with two, 10.0 with
+  // one.
   const int SH = 32 % U ? 1 : 32 / U >= 4 && HS % 4 == 0 ? 4 : 32 / U >= 2 && HS % 2 == 0 ? 2 : 1;
   const bool inter = p->layout == DC_ROPE_INTERLEAVED;
   auto *kernel = SH == 4   ? (inter ? rope_kernel<true, 4> : rope_kernel<false, 4>)
@@ -294,7 +295,7 @@ int ops_kv_append(dc_ctx *ctx, const dc_kv_cache *c, const dc_rope_plan *p, cons
   a.vnorm = vnorm, a.eps = eps;
   const int npass = (heads + 2 * c->kv + 512 / c->D - 1) / (512 / c->D);
   // Warps per token: one, which works the angles out once for all heads, unless that leaves the card without warps.
-  // 16 x 1,024 tokens of 24 + 2 x 8 heads: 57 us with one, 131 with a warp to every pass; one token 6.5 us with one, 2.7
+  // 16 x 1,024 tokens of 24 + 2 x 8 heads: 57 us with one, 125 with a warp to every pass; one token 6.6 us with one, 2.5
   // with a warp to every pass.
   a.W = (int)std::max<long>(1, std::min<long>(npass, (32L * ctx->sms + T - 1) / T));
   const dim3 grid((unsigned)(((long)T * a.W + 7) / 8));
