@@ -441,12 +441,13 @@ __device__ __forceinline__ void walk_line(const Cta<C> &k, const Groups &gs, con
     k.runs()[n % PA_RING].flags = RUN_END;
     mbar_arrive(k.bar(C::B_IF + n % PA_RING));
   }
-  if (lane == 0) reinterpret_cast<int *>(k.smem + C::LOADED_OFF)[values] = stage | turn << 8 | item << 9;  // for settle
+  int *loaded = reinterpret_cast<int *>(k.smem + C::LOADED_OFF);  // for settle
+  if (lane == 0) loaded[values] = stage | turn << 8 | item << 9;
 }
 
 // After a wait ran out and every role has stopped (the whole CTA calls it): the loads and products still in flight. Of a ring
-// the stages below `stage` hold this round's loads, the others those of the round before (or none, which passes). Warps mma0
-// and mma1 issued the products, from the thread that elect_one names.
+// the stages below `stage` hold the loads of the last time around, the others those of the time before (or none, which passes).
+// Warps mma0 and mma1 issued the products, from the thread that elect_one names.
 template <class C>
 static __device__ __noinline__ void settle(uint8_t *smem, int mma0, int mma1) {
   const uint32_t bars = smem_u32(smem) + C::BAR_OFF;

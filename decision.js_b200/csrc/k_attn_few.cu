@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
         tc_fence_after();
         if (anyv) {
           if (seen && ((k.poison(r.item)[irow >> 5] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
-          if (seen && lt == 0.f) ref = MINUS_INF, lt = direct ? __int_as_float(0x7fc00000) : 0.f;  // nothing but minus infinity
+          if (seen && lt == 0.f) ref = MINUS_INF, lt = direct ? __int_as_float(0x7fc00000) : 0.f;  // all keys minus infinity
           const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
           if (a.by_row && valid && jrow == 0 && hf == 0) {
             if (tfirst) a.first[(long)r.kvh * a.T + t] = direct ? -1 : (int)blockIdx.x;

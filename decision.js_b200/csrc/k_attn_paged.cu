@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
               lt += x.x * ex2_approx(x.y - ref);
             }
             if (seen && ((k.poison(r.item)[irow >> 5] >> (irow & 31)) & 1u)) lt = __int_as_float(0x7fc00000);
-            if (seen && lt == 0.f) ref = MINUS_INF, lt = direct ? __int_as_float(0x7fc00000) : 0.f;  // nothing but minus infinity
+            if (seen && lt == 0.f) ref = MINUS_INF, lt = direct ? __int_as_float(0x7fc00000) : 0.f;  // all keys minus infinity
             const long prow = ((long)r.kvh * a.T + r.tok0) * a.r + 128L * blockIdx.x + row;
             if (!direct && valid) a.ml[prow] = make_float2(ref, lt);
             if (a.by_row && valid && jrow == 0) {
